@@ -37,6 +37,7 @@ extern "C" {
 
 #define OMNI_F32 0
 #define OMNI_BF16 1
+#define OMNI_E4M3 2 /* a paged cache's elements: 8 bits, one exponent byte for each vector */
 
 /* verify-attention flags */
 #define OMNI_ATTN_SEPARATE_COMBINE 1 /* merge key splits in a second launch, not in the last split */
@@ -402,6 +403,79 @@ int omni_rms_norm(const void *x, int64_t x_stride, const void *weight, void *y, 
  */
 int omni_silu_mul(const void *gate_inner, int64_t gate_inner_stride, void *out, int64_t out_stride,
                   int32_t rows, int32_t ffn, int32_t dtype, void *stream);
+
+/*
+ * The paged key-value cache of the entry points below.  No counterpart in the reference, whose caches hold a full-length
+ * row for every slot (src/omniasr_trt/decode.py:98).
+ *
+ * ``k_pages`` / ``v_pages`` [pages, kv_heads, page, head_dim] contiguous; ``page`` positions a page, a power of two from
+ * 16 to 256; ``table`` [rows, width] int32 (row stride ``table_stride``): position p of cache row r is offset p % page of
+ * page table[r, p / page].  head_dim: 128, 256 or 512.  ``cache_dtype`` OMNI_BF16, or OMNI_E4M3 with ``k_scale`` /
+ * ``v_scale`` [pages, kv_heads, page] bytes: a vector's values are code * 2^(byte - 127) (bytes are 1..254).
+ * Two rows may share pages (a common beginning); pages and entries behind a row's positions in use are never read.
+ */
+
+/*
+ * omni_rope_kv_append into a paged cache, with as many key heads as there are: ``qkv`` [n_tokens, (heads + 2 kv_heads) *
+ * head_dim] bf16 (q | k | v).  The rotated q goes to ``q_out`` [n_tokens, heads, head_dim]; the rotated k and the v of
+ * token n to position cache_pos[n] (NULL: pos[n]) of cache row slots[n] (NULL: n).  Tokens whose row, position or page is
+ * outside the cache are not written.  A call's (row, position) pairs are distinct: of two equal ones either token's values
+ * may stay, in part.  ``k_out`` [n_tokens, kv_heads, head_dim], if not NULL, gets the rotated k in bf16 as well, for
+ * omni_packed_attention over the same prompts.
+ * OMNI_E4M3: exponent e of a vector x is the least integer with max |x| <= 448 * 2^e, over the finite x and at least -126
+ * (0 for a vector of zeros); the code is x * 2^-e to the nearest e4m3, ties to even, from the rotated fp32 k (at e = 120, where
+ * bf16 ends, at most 240); infinities, which e4m3 lacks, and NaN become NaN.
+ */
+int omni_rope_kv_paged(const void *qkv, int64_t qkv_row_stride, const float *cs, int64_t cs_rows,
+                       const int64_t *pos, const int64_t *slots, const int64_t *cache_pos, void *q_out,
+                       void *k_out, void *k_pages, void *v_pages, void *k_scale, void *v_scale,
+                       int32_t pages, int32_t page, const int32_t *table, int64_t table_stride,
+                       int64_t rows, int32_t width, int64_t n_tokens, int32_t heads, int32_t kv_heads,
+                       int32_t head_dim, int32_t cache_dtype, int32_t dtype, void *stream);
+
+/*
+ * Cached vectors read back: k_out[n], v_out[n] ([n_tokens, kv_heads, head_dim] bf16) = the K and V of position pos[n] of
+ * cache row slots[n]; zeros where the row, position or page is outside the cache.  Exact: bf16 holds code * 2^e.
+ */
+int omni_paged_read(const void *k_pages, const void *v_pages, const void *k_scale, const void *v_scale,
+                    int32_t pages, int32_t page, const int32_t *table, int64_t table_stride, int64_t rows,
+                    int32_t width, const int64_t *slots, const int64_t *pos, int64_t n_tokens,
+                    int32_t kv_heads, int32_t head_dim, int32_t cache_dtype, void *k_out, void *v_out,
+                    void *stream);
+
+/* Bytes of workspace omni_paged_attention needs. */
+size_t omni_paged_attention_workspace(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                      int32_t head_dim, int32_t page, int32_t width);
+
+/*
+ * omni_verify_attention over a paged cache with grouped heads: query i of row b (``q`` [rows*tokens, heads, head_dim]
+ * bf16, row b's ``tokens`` queries at rows b*tokens ..) attends to keys [0, lengths[b] + i) of the pages of table row b,
+ * head h to key head h / (heads / kv_heads); softmax in fp32; an empty key range gives zeros.  Key counts are held in
+ * [0, width * page], page numbers in [0, pages).  tokens: 1..16; heads a multiple of kv_heads; scale > 0.
+ * ``workspace``: omni_paged_attention_workspace() bytes, 256-byte aligned, any content.  Results do not depend on timing.
+ */
+int omni_paged_attention(const void *q, const void *k_pages, const void *v_pages, const void *k_scale,
+                         const void *v_scale, int32_t pages, int32_t page, const int32_t *table,
+                         int64_t table_stride, int32_t width, const int64_t *lengths, int32_t rows,
+                         int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
+                         void *out, void *workspace, size_t workspace_bytes, int32_t cache_dtype,
+                         int32_t dtype, void *stream);
+
+/*
+ * Causal attention of packed prompts of different lengths (omni_prefill_attention without the padding, over keys that
+ * need not be in a cache).  Sequence s: queries starts[s] .. starts[s+1]-1 of ``q`` [queries, heads, head_dim], keys
+ * k_starts[s] .. k_starts[s+1]-1 of ``k`` / ``v`` [keys, kv_heads, head_dim] (element strides, multiples of 8, unit stride
+ * in head_dim).  Query i of the sequence's nq sees its keys [0, i + nk - nq] of nk -- with nk > nq the prompt goes on
+ * behind nk - nq earlier keys -- and none gives zeros.  ``starts`` / ``k_starts`` [sequences + 1], not decreasing; held
+ * within q and k.  ``longest``: at least the longest sequence's queries (it sizes the grid; queries past it are not
+ * computed).  Rows of ``out`` [queries, heads, head_dim] in no sequence are left as they are.  bf16, fp32 accumulation,
+ * head_dim 128, 256 or 512; heads a multiple of kv_heads; scale > 0.  No workspace.
+ */
+int omni_packed_attention(const void *q, const void *k, const void *v, int64_t k_stride_pos,
+                          int64_t k_stride_head, int64_t v_stride_pos, int64_t v_stride_head,
+                          const int64_t *starts, const int64_t *k_starts, int32_t sequences,
+                          int64_t queries, int64_t keys, int32_t longest, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, float scale, void *out, int32_t dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -14,10 +14,10 @@ from pathlib import Path
 import torch  # noqa: F401  (must be loaded first: its HIP runtime is the one the library uses)
 
 PATH = Path(__file__).resolve().with_name("libomniasr_mi355x.so")
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 OK = 0
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
 ATTN_SEPARATE_COMBINE = 1
 ATTN_SPLIT_K = 2
 STATIC_WORKSPACE_BYTES = 32 << 20  # OMNI_STATIC_WORKSPACE_BYTES
@@ -67,6 +67,16 @@ _SIGNATURES = {
     "omni_silu_mul": (c_int, [_P, c_int64, _P, c_int64, c_int32, c_int32, c_int32, _P]),
     "omni_beam_take_over": (c_int, [c_int32, c_int32, c_int64, _P, _P, _P, c_int64, c_int64, _P, c_int64, c_int64,
                                     _P, _P, c_int32, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, _P]),
+    "omni_rope_kv_paged": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int32, _P,
+                                   c_int64, c_int64, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                   _P]),
+    "omni_paged_read": (c_int, [_P, _P, _P, _P, c_int32, c_int32, _P, c_int64, c_int64, c_int32, _P, _P, c_int64,
+                                c_int32, c_int32, c_int32, _P, _P, _P]),
+    "omni_paged_attention_workspace": (c_size_t, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "omni_paged_attention": (c_int, [_P, _P, _P, _P, _P, c_int32, c_int32, _P, c_int64, c_int32, _P, c_int32, c_int32,
+                                     c_int32, c_int32, c_int32, c_float, _P, _P, c_size_t, c_int32, c_int32, _P]),
+    "omni_packed_attention": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int32, c_int64,
+                                      c_int64, c_int32, c_int32, c_int32, c_int32, c_float, _P, c_int32, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

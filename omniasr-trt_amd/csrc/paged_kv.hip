@@ -1,0 +1,210 @@
+// Writing and reading a paged key-value cache on gfx950.
+//
+// Write: the new tokens' q and k rotated as rope_kv_append rotates them (each product rounded on its own), k and v put
+// into their pages in bf16 or quantised to e4m3.  A quantised vector x of one (token, kv head) keeps one exponent e, the
+// least with max |x| <= 448 * 2^e: x * 2^-e is exact, so a value is rounded once, to the nearest e4m3 (ties to even), and
+// what is read back, code * 2^e, is exact in bf16.  (A scale max |x| / 448 would use up to one more binade of e4m3's range
+// and cost a second rounding at the division and a third when read; e4m3's relative precision is the same in every
+// binade above 2^-6, 14 below the largest.)  k is quantised from the rotated fp32 values, not from their bf16 rounding.
+//
+// Both kernels are one pass over their bytes, 16 (8 for e4m3) of one vector a thread: a step's launch is latency, a
+// prompt's is HBM.
+#include "common.h"
+#include "paged.h"
+
+namespace omni {
+
+// (re, im) -> (re*c - im*s, re*s + im*c), every operation rounded separately.
+__device__ __forceinline__ void turn_pair(float& re, float& im, float c, float s) {
+#pragma clang fp contract(off)
+  const float a = re * c;
+  const float b = im * s;
+  const float d = re * s;
+  const float e = im * c;
+  re = a - b;
+  im = d + e;
+}
+
+// The exponent of a vector whose largest finite |x| has the bits ``top``: 448 = 1.75 * 2^8.  Vectors below 2^-126 * 448
+// keep e = -126, so that 2^e and 2^-e are normal numbers.
+__device__ __forceinline__ int e4m3_exponent(uint32_t top) {
+  const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return top == 0 ? 0 : max(-126, e);
+}
+
+// x * down as e4m3; an infinity, which e4m3 does not have, as NaN.  At the last exponent, 120, values of 248 and more would
+// round to 256 * 2^120, which bf16 does not have: they are held at 240.
+__device__ __forceinline__ float to_e4m3_range(float x, float down, bool last) {
+  const float y = x * down;
+  if ((__float_as_uint(x) & 0x7fffffffu) == 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return last && fabsf(y) > 240.f ? copysignf(240.f, y) : y;
+}
+
+struct PagedWrite {
+  const uint16_t* qkv;  // [tokens, (heads + 2 kv) * D]
+  int64_t qkv_stride;
+  const float* cs;
+  int64_t cs_rows;
+  const int64_t* pos;
+  const int64_t* slots;
+  const int64_t* cache_pos;
+  uint16_t* q_out;  // [tokens, heads, D]
+  uint16_t* k_out;  // [tokens, kv, D] or nullptr
+  int heads;
+};
+
+template <int D, bool kF8>
+__global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite w, PagedCache a) {
+  constexpr int kLanes = D / 8;  // of one vector; a vector never spans two waves
+  const int piece = blockIdx.y * blockDim.x + threadIdx.x;
+  const int vec = piece / kLanes, e0 = piece % kLanes * 8;
+  if (vec >= w.heads + 2 * a.kv) return;
+  const int64_t n = blockIdx.x;
+  const u32x4_t raw = *reinterpret_cast<const u32x4_t*>(w.qkv + n * w.qkv_stride + vec * D + e0);
+  const int64_t p = w.pos[n];
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = bf16x8_elem(raw, e);
+  if (vec < w.heads + a.kv) {
+    const f32x4_t* row = reinterpret_cast<const f32x4_t*>(w.cs + clamp64(p, 0, w.cs_rows - 1) * D + e0);
+    const f32x4_t t0 = row[0], t1 = row[1];
+    turn_pair(x[0], x[1], t0[0], t0[1]);
+    turn_pair(x[2], x[3], t0[2], t0[3]);
+    turn_pair(x[4], x[5], t1[0], t1[1]);
+    turn_pair(x[6], x[7], t1[2], t1[3]);
+  }
+  u32x4_t bf;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bf[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+  if (vec < w.heads) {
+    *reinterpret_cast<u32x4_t*>(w.q_out + (n * w.heads + vec) * D + e0) = bf;
+    return;
+  }
+  const bool is_k = vec < w.heads + a.kv;
+  const int head = vec - w.heads - (is_k ? 0 : a.kv);
+  if (is_k && w.k_out) *reinterpret_cast<u32x4_t*>(w.k_out + (n * a.kv + head) * D + e0) = bf;
+  const int64_t cell = paged_cell(a, w.slots ? w.slots[n] : n, w.cache_pos ? w.cache_pos[n] : p, head);
+  char* pages = is_k ? a.k : a.v;
+  if constexpr (!kF8) {
+    if (cell < 0) return;
+    *reinterpret_cast<u32x4_t*>(pages + (cell * D + e0) * 2) = is_k ? bf : raw;
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t u = __float_as_uint(x[e]) & 0x7fffffffu;
+      top = max(top, u < 0x7f800000u ? u : 0u);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
+    if (cell < 0) return;
+    const int exponent = e4m3_exponent(top);
+    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = to_e4m3_range(x[e], down, exponent == 120);
+    u32x2_t codes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int half = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+      codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], half, true);
+    }
+    *reinterpret_cast<u32x2_t*>(pages + cell * D + e0) = codes;
+    if (e0 == 0) (is_k ? a.k_scale : a.v_scale)[cell] = (uint8_t)(exponent + 127);
+  }
+}
+
+struct PagedRead {
+  const int64_t* slots;
+  const int64_t* pos;
+  uint16_t* k;  // [tokens, kv, D]
+  uint16_t* v;
+};
+
+template <int D, bool kF8>
+__global__ __launch_bounds__(256) void paged_read_kernel(PagedRead r, PagedCache a) {
+  constexpr int kLanes = D / 8;
+  const int piece = blockIdx.y * blockDim.x + threadIdx.x;
+  const int vec = piece / kLanes, e0 = piece % kLanes * 8;
+  if (vec >= 2 * a.kv) return;
+  const int64_t n = blockIdx.x;
+  const bool is_k = vec < a.kv;
+  const int head = vec - (is_k ? 0 : a.kv);
+  const int64_t cell = paged_cell(a, r.slots[n], r.pos[n], head);
+  u32x4_t out = {0u, 0u, 0u, 0u};
+  if (cell >= 0) {
+    const char* pages = is_k ? a.k : a.v;
+    if constexpr (kF8) {
+      out = e4m3x8_to_bf16(*reinterpret_cast<const u32x2_t*>(pages + cell * D + e0),
+                           scale_of((is_k ? a.k_scale : a.v_scale)[cell]));
+    } else {
+      out = *reinterpret_cast<const u32x4_t*>(pages + (cell * D + e0) * 2);
+    }
+  }
+  *reinterpret_cast<u32x4_t*>((is_k ? r.k : r.v) + (n * a.kv + head) * D + e0) = out;
+}
+
+}  // namespace omni
+
+using namespace omni;
+
+// The instance of ``kernel`` for a head dim and cache type.
+#define OMNI_PAGED_LAUNCH(kernel, head_dim, f8, grid, stream, ...)                                  \
+  do {                                                                                              \
+    if (head_dim == 128) {                                                                          \
+      if (f8) kernel<128, true><<<grid, 256, 0, stream>>>(__VA_ARGS__);                             \
+      else kernel<128, false><<<grid, 256, 0, stream>>>(__VA_ARGS__);                               \
+    } else if (head_dim == 256) {                                                                   \
+      if (f8) kernel<256, true><<<grid, 256, 0, stream>>>(__VA_ARGS__);                             \
+      else kernel<256, false><<<grid, 256, 0, stream>>>(__VA_ARGS__);                               \
+    } else {                                                                                        \
+      if (f8) kernel<512, true><<<grid, 256, 0, stream>>>(__VA_ARGS__);                             \
+      else kernel<512, false><<<grid, 256, 0, stream>>>(__VA_ARGS__);                               \
+    }                                                                                               \
+  } while (0)
+
+extern "C" int omni_rope_kv_paged(const void* qkv, int64_t qkv_row_stride, const float* cs, int64_t cs_rows,
+                                  const int64_t* pos, const int64_t* slots, const int64_t* cache_pos, void* q_out,
+                                  void* k_out, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
+                                  int32_t pages, int32_t page, const int32_t* table, int64_t table_stride,
+                                  int64_t rows, int32_t width, int64_t n_tokens, int32_t heads, int32_t kv_heads,
+                                  int32_t head_dim, int32_t cache_dtype, int32_t dtype, void* stream) {
+  if (dtype != OMNI_BF16) return OMNI_ERR_DTYPE;
+  if (n_tokens < 0 || n_tokens > 0x7fffffffLL || heads <= 0 || kv_heads <= 0) return OMNI_ERR_INVALID;
+  if (n_tokens == 0) return OMNI_OK;
+  const int status = omni_check_pages(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, head_dim, table,
+                                      table_stride, rows, width, cache_dtype);
+  if (status != OMNI_OK) return status;
+  if (heads > 4096 || kv_heads > 4096) return OMNI_ERR_SHAPE;
+  if (!qkv || !cs || !pos || !q_out || cs_rows <= 0) return OMNI_ERR_INVALID;
+  if (((uintptr_t)qkv | (uintptr_t)cs | (uintptr_t)q_out | (uintptr_t)k_out) & 15u) return OMNI_ERR_INVALID;
+  if (qkv_row_stride % 8 || qkv_row_stride < (heads + 2LL * kv_heads) * head_dim) return OMNI_ERR_INVALID;
+  const PagedWrite w{(const uint16_t*)qkv, qkv_row_stride, cs, cs_rows, pos, slots, cache_pos, (uint16_t*)q_out,
+                     (uint16_t*)k_out, heads};
+  const PagedCache a =
+      omni_paged_cache(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, table, table_stride, rows, width);
+  const int pieces = (heads + 2 * kv_heads) * (head_dim / 8);
+  const dim3 grid((unsigned)n_tokens, (unsigned)((pieces + 255) / 256));
+  OMNI_PAGED_LAUNCH(paged_write_kernel, head_dim, cache_dtype == OMNI_E4M3, grid, (hipStream_t)stream, w, a);
+  return omni_launch_status();
+}
+
+extern "C" int omni_paged_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                               int32_t pages, int32_t page, const int32_t* table, int64_t table_stride, int64_t rows,
+                               int32_t width, const int64_t* slots, const int64_t* pos, int64_t n_tokens,
+                               int32_t kv_heads, int32_t head_dim, int32_t cache_dtype, void* k_out, void* v_out,
+                               void* stream) {
+  if (n_tokens < 0 || n_tokens > 0x7fffffffLL || kv_heads <= 0) return OMNI_ERR_INVALID;
+  if (n_tokens == 0) return OMNI_OK;
+  const int status = omni_check_pages(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, head_dim, table,
+                                      table_stride, rows, width, cache_dtype);
+  if (status != OMNI_OK) return status;
+  if (kv_heads > 4096) return OMNI_ERR_SHAPE;
+  if (!slots || !pos || !k_out || !v_out || (((uintptr_t)k_out | (uintptr_t)v_out) & 15u)) return OMNI_ERR_INVALID;
+  const PagedRead r{slots, pos, (uint16_t*)k_out, (uint16_t*)v_out};
+  const PagedCache a =
+      omni_paged_cache(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, table, table_stride, rows, width);
+  const int pieces = 2 * kv_heads * (head_dim / 8);
+  const dim3 grid((unsigned)n_tokens, (unsigned)((pieces + 255) / 256));
+  OMNI_PAGED_LAUNCH(paged_read_kernel, head_dim, cache_dtype == OMNI_E4M3, grid, (hipStream_t)stream, r, a);
+  return omni_launch_status();
+}

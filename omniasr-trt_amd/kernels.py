@@ -20,6 +20,10 @@ tokens / positions / cache rows / key counts in one launch) and :func:`greedy_ac
 the verify logits and the acceptance); for the prefill: :func:`prefill_attention` (causal attention of whole
 contexts, the reference's ``F.scaled_dot_product_attention(is_causal=True)``).
 
+For caches in pages, bf16 or quantised to e4m3, with as many key heads as there are (none of it in the reference):
+:func:`rope_kv_paged` writes, :func:`paged_read` reads back, :func:`paged_attention` is the step's attention and
+:func:`packed_attention` the prompts', without padding.
+
 Nothing here synchronises or allocates beyond the outputs and the attention workspace (from torch's
 allocator, so from a graph's pool under capture), so every function can be captured in a HIP graph.  There is
 no other code path: on a GPU without the library these functions raise.
@@ -28,6 +32,7 @@ no other code path: on a GPU without the library these functions raise.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 
 import torch
 import torch.nn.functional as F
@@ -609,6 +614,174 @@ def beam_select(logits: torch.Tensor, score: torch.Tensor, count: torch.Tensor, 
                                   tickets.data_ptr(), kind, _lib.BF16, _stream(logits))
     _lib.check(status, "beam_select")
     return best, flat
+
+
+# ---------------------------------------------------------------------------------------------- paged caches
+
+def _current(device: torch.device):
+    """The context a launch on ``device`` runs in: a stream is used with its own device current."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k_scale: torch.Tensor | None,
+           v_scale: torch.Tensor | None) -> int:
+    """Checks a paged cache; returns its element type.  ``k_pages`` / ``v_pages`` [pages, kv heads, page, D], bf16 or
+    float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8; ``table`` [rows, width] int32."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    _need(len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype and k_pages.is_contiguous()
+          and v_pages.is_contiguous(), "k_pages / v_pages: contiguous [pages, kv heads, page, D] of one dtype")
+    _need(shape[3] in (128, 256, 512) and shape[2] in (16, 32, 64, 128, 256),
+          "k_pages / v_pages: head dim 128, 256 or 512, pages of 16, 32, 64, 128 or 256 positions")
+    _need(table.dtype == torch.int32 and table.dim() == 2 and (table.stride(1) == 1 or table.size(1) <= 1),
+          "table: [rows, width] int32 with unit stride in width")
+    device = k_pages.device
+    if dtype == torch.float8_e4m3fn:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _need(t is not None and t.dtype == torch.uint8 and t.shape == shape[:3] and t.is_contiguous()
+                  and t.device == device, f"{name}: contiguous uint8 [pages, kv heads, page] for e4m3 pages")
+    else:
+        _need(dtype == torch.bfloat16, "k_pages / v_pages: bfloat16 or float8_e4m3fn")
+        _need(k_scale is None and v_scale is None, "k_scale / v_scale: for e4m3 pages only")
+    _need(v_pages.device == device and table.device == device, "pages and table: one device")
+    return _lib.BF16 if dtype == torch.bfloat16 else _lib.E4M3
+
+
+def _row_stride(table: torch.Tensor) -> int:
+    return table.stride(0) if table.size(0) > 1 else max(table.stride(0), table.size(1))
+
+
+def rope_kv_paged(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_pages: torch.Tensor,
+                  v_pages: torch.Tensor, table: torch.Tensor, heads: int, slots: torch.Tensor | None = None,
+                  cache_pos: torch.Tensor | None = None, *, k_scale: torch.Tensor | None = None,
+                  v_scale: torch.Tensor | None = None, rotated: bool = False):
+    """:func:`rope_kv` into a paged cache: ``qkv`` [N, (heads + 2 * kv heads) * D] bf16 (q|k|v of N tokens) rotated at
+    ``pos[n]``; token n's k, v go to position ``cache_pos[n]`` (default ``pos[n]``) of cache row ``slots[n]`` (default n),
+    that is to page ``table[slots[n], position // page]`` of ``k_pages`` / ``v_pages`` [pages, kv heads, page, D].  Tokens
+    whose row, position or page is outside the cache (a negative row marks padding) are not written; the (row, position)
+    pairs of a call are distinct.  Returns the rotated q [N, heads, D]; with ``rotated`` also the rotated k
+    [N, kv heads, D], which :func:`packed_attention` takes beside the v in ``qkv``.
+
+    Pages are bf16, or float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8: a vector x is kept as
+    the e4m3 nearest to x * 2^-e, and the byte e + 127, e the least integer with max |x| <= 448 * 2^e."""
+    lib = _lib.load()
+    cache = _paged(k_pages, v_pages, table, k_scale, v_scale)
+    pages, kv, page, dim = k_pages.shape
+    _need(qkv.dim() == 2 and heads >= 1 and qkv.size(1) == (heads + 2 * kv) * dim and qkv.stride(1) == 1,
+          "qkv: [N, (heads + 2 * kv heads) * D] with unit stride in the last dimension")
+    n, device = qkv.size(0), qkv.device
+    _need(qkv.dtype == torch.bfloat16, "qkv: bfloat16")
+    _need(cs.dtype == torch.float32 and cs.is_contiguous() and cs.dim() == 3 and cs.size(1) * 2 == dim
+          and cs.size(2) == 2, "cs: contiguous [P, D/2, 2] fp32")
+    for name, t in (("pos", pos), ("slots", slots), ("cache_pos", cache_pos)):
+        if t is not None:
+            _index(t, name)
+            _need(t.numel() == n and t.device == device, f"{name}: [N] on qkv's device")
+    _need(k_pages.device == device and cs.device == device, "qkv, cs and the cache: one device")
+    q = torch.empty(n, heads, dim, device=device, dtype=qkv.dtype)
+    k = torch.empty(n, kv, dim, device=device, dtype=qkv.dtype) if rotated else None
+    with _current(device):
+        status = lib.omni_rope_kv_paged(
+            qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.size(1), cs.data_ptr(), cs.size(0), pos.data_ptr(),
+            _ptr(slots), _ptr(cache_pos), q.data_ptr(), _ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
+            _ptr(v_scale), pages, page, table.data_ptr(), _row_stride(table), table.size(0), table.size(1), n, heads,
+            kv, dim, cache, _lib.BF16, _stream(qkv))
+    _lib.check(status, "rope_kv_paged")
+    return (q, k) if rotated else q
+
+
+def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, slots: torch.Tensor,
+               pos: torch.Tensor, *, k_scale: torch.Tensor | None = None,
+               v_scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached k and v at position ``pos[n]`` of cache row ``slots[n]``, bf16 [N, kv heads, D] each (exact: e4m3 times
+    its power of two is a bf16 number), zeros where the row, position or page is outside the cache.  What a prompt that
+    goes on behind cached positions attends to (:func:`packed_attention`).  The cache as for :func:`rope_kv_paged`."""
+    lib = _lib.load()
+    cache = _paged(k_pages, v_pages, table, k_scale, v_scale)
+    pages, kv, page, dim = k_pages.shape
+    device = k_pages.device
+    for name, t in (("slots", slots), ("pos", pos)):
+        _index(t, name)
+        _need(t.numel() == slots.numel() and t.device == device, f"{name}: [N] on the cache's device")
+    n = slots.numel()
+    k = torch.empty(n, kv, dim, device=device, dtype=torch.bfloat16)
+    v = torch.empty(n, kv, dim, device=device, dtype=torch.bfloat16)
+    with _current(device):
+        status = lib.omni_paged_read(
+            k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), pages, page, table.data_ptr(),
+            _row_stride(table), table.size(0), table.size(1), slots.data_ptr(), pos.data_ptr(), n, kv, dim, cache,
+            k.data_ptr(), v.data_ptr(), _stream(k))
+    _lib.check(status, "paged_read")
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                    lengths: torch.Tensor, tokens: int, scale: float, *, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`draft_attention` over a paged cache with grouped heads: ``q`` [B*T, H, D] bf16 (T = ``tokens``, 1..16), row
+    b's query i attends to keys [0, lengths[b] + i) of the pages of ``table[b]``; head h reads kv head h // (H / kv heads).
+    No key gives zeros.  Returns [B*T, H, D].  Calls may overlap: each has its own workspace.  The cache as for
+    :func:`rope_kv_paged`."""
+    lib = _lib.load()
+    cache = _paged(k_pages, v_pages, table, k_scale, v_scale)
+    pages, kv, page, dim = k_pages.shape
+    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.is_contiguous() and q.size(2) == dim
+          and q.size(1) % kv == 0 and q.size(1) >= kv, "q: contiguous bf16 [B*T, H, D], H a multiple of the kv heads")
+    _need(1 <= tokens <= 16 and q.size(0) % tokens == 0, "tokens: 1..16, q: [B*T, H, D]")
+    device, heads, rows = q.device, q.size(1), q.size(0) // tokens
+    _need(table.size(0) >= rows, "table: at least B rows")
+    _need(pages > 0 and table.size(1) > 0, "the cache: at least one page and one table entry")
+    _index(lengths, "lengths")
+    _need(lengths.numel() >= rows, "lengths: [B]")
+    _need(lengths.device == device and k_pages.device == device, "q, lengths and the cache: one device")
+    out = torch.empty_like(q)
+    width = table.size(1)
+    with _current(device):
+        ws = lib.omni_paged_attention_workspace(rows, tokens, heads, kv, dim, page, width)
+        workspace = torch.empty(max(ws, 256), device=device, dtype=torch.uint8)
+        status = lib.omni_paged_attention(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), pages, page,
+            table.data_ptr(), _row_stride(table), width, lengths.data_ptr(), rows, tokens, heads, kv, dim, scale,
+            out.data_ptr(), workspace.data_ptr(), workspace.numel(), cache, _lib.BF16, _stream(q))
+    _lib.check(status, "paged attention")
+    return out
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, longest: int,
+                     scale: float, *, k_starts: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed prompts: :func:`prefill_attention` without padding, over k and v as the projections
+    leave them.  ``q`` [N, H, D] bf16, ``k`` / ``v`` [M, kv heads, D] bf16 with unit stride in D (16-byte rows); sequence s
+    is queries ``starts[s]`` .. ``starts[s + 1] - 1`` and keys ``k_starts[s]`` .. (default: ``starts``), both [S + 1]
+    int64, not decreasing.  Query i of its nq sees keys [0, i + nk - nq] of its nk: with more keys than queries the prompt
+    goes on behind earlier positions (:func:`paged_read`).  No key gives zeros.  ``longest``: at least the queries of the
+    longest sequence.  Returns ``out`` [N, H, D] (new by default); rows in no sequence are left as they are in it."""
+    lib = _lib.load()
+    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.is_contiguous() and q.size(2) in (128, 256, 512),
+          "q: contiguous bf16 [N, H, D], D = 128, 256 or 512")
+    n, heads, dim = q.shape
+    _need(k.dim() == 3 and k.shape == v.shape and k.size(2) == dim and k.dtype == q.dtype == v.dtype,
+          "k / v: bf16 [M, kv heads, D]")
+    m, kv = k.size(0), k.size(1)
+    _need(kv >= 1 and heads % kv == 0 and heads >= kv, "q: a multiple of k's heads")
+    _need(k.stride(2) == 1 and v.stride(2) == 1, "k / v: unit stride in D")
+    k_starts = starts if k_starts is None else k_starts
+    device = q.device
+    for name, t in (("starts", starts), ("k_starts", k_starts)):
+        _index(t, name)
+        _need(t.numel() == starts.numel() >= 1 and t.device == device, f"{name}: [S + 1] on q's device")
+    _need(k.device == device and v.device == device, "q, k and v: one device")
+    _need(longest >= 0, "longest: at least the longest sequence's queries")
+    if out is None:
+        out = torch.empty_like(q)
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == device,
+          "out: contiguous, q's shape, dtype and device")
+    with _current(device):
+        status = lib.omni_packed_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            starts.data_ptr(), k_starts.data_ptr(), starts.numel() - 1, n, m, min(longest, n), heads, kv, dim, scale,
+            out.data_ptr(), _lib.BF16, _stream(q))
+    _lib.check(status, "packed attention")
+    return out
 
 
 def layer_ops_supported(x: torch.Tensor) -> bool:

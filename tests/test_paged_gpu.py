@@ -1,0 +1,484 @@
+"""The paged cache's operators on an MI355X against their restatement in float64 (oracle/paged.py).
+
+Bounds: an output is rounded to bf16 once (2^-8 of it) and each weight once before its product with v (2^-8 of the sum of
+weights times |v|, ``size``); a score's fp32 sum of D products is off by at most D * 2^-24 * sum |q k| and enters both the
+weight and the sum of weights; the rest (exp2, the sums, the merge of splits) is within 2^-16 of ``size``."""
+
+import sys
+
+import pytest
+import torch
+
+from oracle import paged as op
+from omniasr_trt_amd import batching, kernels, modeling
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+SHAPES = [(4, 4, 512), (4, 4, 128), (8, 2, 128), (16, 2, 256), (6, 1, 128)]  # heads, kv heads, D
+
+
+def say(*a):
+    print(*a, flush=True, file=sys.stderr)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(shape, g, cuda):
+    return torch.randn(shape, generator=g).to(BF).to(cuda)
+
+
+def close(got, want, size, q, k, scale):
+    """``got`` bf16 against ``want`` with the bounds of this file; ``q`` / ``k`` give the largest sum of |q k|."""
+    dim = q.size(-1)
+    kn = k[k.isfinite().all(-1)] if k.numel() else k
+    reach = float(q.double().norm(dim=-1).max() * (kn.double().norm(dim=-1).max() if kn.numel() else 0.0)) * scale
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -16 + 2 * dim * 2.0 ** -24 * reach) * size + 1e-30
+    off = (got.double() - want).abs()
+    worst = float((off / bound).max()) if off.numel() else 0.0
+    assert bool((off <= bound).all()), f"{worst:.2f} of the bound"
+
+
+def make_cache(cuda, g, kv, dim, page, reach, fp8, spare=5, shared=0):
+    """Pages of random keys for rows of ``reach`` positions, in random order; the rest of the pool and of the last pages
+    holds NaN, the table behind a row's pages is out of range; the first ``shared`` pages of row 1 are row 0's."""
+    need = [-(-n // page) for n in reach]
+    pool = sum(need) + spare
+    order = torch.randperm(pool, generator=g)
+    table = torch.full((len(reach), max(max(need), 1) + 2), 2 ** 30, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n].int()
+        at += n
+    if shared:
+        table[1, :shared] = table[0, :shared]
+    k, v = (torch.full((pool, kv, page, dim), float("nan")) for _ in "kv")
+    for b, n in enumerate(reach):
+        for i in range(need[b]):
+            rows = min(page, n - i * page)
+            for x in (k, v):
+                x[int(table[b, i]), :, :rows] = torch.randn(kv, rows, dim, generator=g)
+    scales = {}
+    out = []
+    for name, x in (("k_scale", k), ("v_scale", v)):
+        if fp8:
+            values, byte = op.quantise(x.to(BF).float())
+            codes = (values / torch.exp2(byte.double() - 127)[..., None]).float().to(torch.float8_e4m3fn)
+            scales[name] = byte.to(cuda)
+            out.append(codes.to(cuda))
+        else:
+            out.append(x.to(BF).to(cuda))
+    return out[0], out[1], table.to(cuda), scales
+
+
+# ---------------------------------------------------------------------------------------------- write and read
+
+def written(qkv, cs, pos, heads, kv, dim, fp8):
+    """(q, k, v, rotated k) as they are kept, from the oracle on the CPU: k and v float64."""
+    x = qkv.cpu().float().view(len(pos), heads + 2 * kv, dim)
+    turned = op.rotate(x[:, : heads + kv], cs.cpu()[pos.cpu()])
+    k, v = turned[:, heads:], x[:, heads + kv:]
+    kept = [op.quantise(a)[0] for a in (k, v)] if fp8 else [k.to(BF).double(), v.double()]
+    return turned[:, :heads].to(BF), *kept, turned[:, heads:].to(BF)
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("page", [16, 128])
+def test_write_and_read_back(cuda, heads, kv, dim, page, fp8):
+    g = gen(heads * dim + page)
+    say(f"write heads={heads} kv={kv} dim={dim} page={page} fp8={fp8}")
+    lengths = [1, 40, 17]
+    k, v, table, scales = make_cache(cuda, g, kv, dim, page, [300, 160, 33], fp8)
+    before = [x.clone().view(torch.uint8) for x in (k, v)]
+    slots = torch.repeat_interleave(torch.arange(3), torch.tensor(lengths))
+    pos = torch.cat([torch.arange(n) + f for n, f in zip(lengths, (299, 100, 0))])
+    n = len(pos)
+    big = torch.randn(n, heads + 2 * kv, dim + 8, generator=g) * torch.exp2(torch.randint(-30, 30, (n, heads + 2 * kv, 1),
+                                                                            generator=g).float())
+    wide = big[..., :dim].flatten(1).to(BF).to(cuda)
+    qkv = torch.cat([wide, wide], 1)[:, : wide.size(1)]  # a row stride of its own
+    cs = modeling.rope_table(modeling.DecoderConfig(model_dim=heads * dim, num_heads=heads, max_seq_len=512)).to(cuda)
+    q, rotated = kernels.rope_kv_paged(qkv, cs, pos.to(cuda), k, v, table, heads, slots.to(cuda), rotated=True, **scales)
+    kk, vv = kernels.paged_read(k, v, table, slots.to(cuda), pos.to(cuda), **scales)
+    torch.cuda.synchronize()
+    wq, wk, wv, wr = written(qkv, cs, pos, heads, kv, dim, fp8)
+    assert torch.equal(q.cpu(), wq) and torch.equal(rotated.cpu(), wr)
+    assert torch.equal(kk.cpu().double(), wk) and torch.equal(vv.cpu().double(), wv)
+    # nothing else has changed
+    mask = torch.zeros(k.shape[:3], dtype=torch.bool)
+    for s, p in zip(slots.tolist(), pos.tolist()):
+        page_at, off = op.cell(table, page, k.size(0), s, p)
+        mask[page_at, :, off] = True
+    for now, was in zip((k, v), before):
+        assert torch.equal(now.view(torch.uint8).cpu()[~mask], was.cpu()[~mask])
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+def test_write_outside_the_cache(cuda, fp8):
+    """Padding (a negative row), rows and positions past the table and pages past the pool are not written and read as
+    zeros; cache positions of their own."""
+    g, heads, kv, dim, page = gen(7), 4, 2, 128, 16
+    k, v, table, scales = make_cache(cuda, g, kv, dim, page, [40, 20], fp8)
+    wide = table.size(1) * page
+    slots = torch.tensor([0, -1, 2, 0, 0, 1, 1, 0])
+    at = torch.tensor([3, 3, 3, wide, -1, 39, 2 ** 40, 45])  # 39 of row 1 and 45.. of row 0 partly unset in the table
+    table[0, 2] = -5
+    cells = [op.cell(table, page, k.size(0), s, p) for s, p in zip(slots.tolist(), at.tolist())]
+    assert cells[0] is not None and all(c is None for c in cells[1:])
+    before = [x.clone().view(torch.uint8) for x in (k, v, *scales.values())]
+    qkv = normal((8, (heads + 2 * kv) * dim), g, cuda)
+    cs = modeling.rope_table(modeling.DecoderConfig(model_dim=heads * dim, num_heads=heads, max_seq_len=64)).to(cuda)
+    pos = torch.arange(8, device=cuda) * 9
+    q = kernels.rope_kv_paged(qkv, cs, pos.clamp(max=63), k, v, table, heads, slots.to(cuda), at.to(cuda), **scales)
+    kk, vv = kernels.paged_read(k, v, table, slots.to(cuda), at.to(cuda), **scales)
+    torch.cuda.synchronize()
+    wq, wk, wv, _ = written(qkv, cs, pos.clamp(max=63), heads, kv, dim, fp8)
+    assert torch.equal(q.cpu(), wq)
+    assert torch.equal(kk[0].cpu().double(), wk[0]) and torch.equal(vv[0].cpu().double(), wv[0])
+    assert not kk[1:].any() and not vv[1:].any()
+    for now, was in zip((k, v, *scales.values()), before):
+        changed = (now.view(torch.uint8) != was).flatten(3).any(-1) if now.dim() == 4 else now != was
+        where = changed.nonzero().cpu()
+        assert all((r[0].item(), r[2].item()) == cells[0] for r in where)
+
+
+def test_quantised_vectors_of_zeros_extremes_and_what_is_not_finite(cuda):
+    heads, kv, dim, page = 1, 1, 128, 16
+    rows = torch.randn(8, dim, generator=gen(3))
+    rows[0] = 0
+    rows[1, 7] = float("inf")
+    rows[2, 9] = float("nan")
+    rows[3] = float("-inf")
+    rows[4] *= 2.0 ** -133  # bf16 subnormals
+    rows[5, 0] = torch.finfo(BF).max
+    rows[6] = rows[6].sign() * 448
+    rows[7] = (torch.arange(dim) - 64) * 2.0 ** -9  # every subnormal e4m3 code of its scale
+    rows[7, 0] = 448 * 2.0
+    v = rows.to(BF)
+    qkv = torch.cat([torch.zeros(8, 2 * dim, dtype=BF), v], 1).to(cuda)
+    k_pages = torch.zeros(1, kv, page, dim, device=cuda).to(torch.float8_e4m3fn)
+    v_pages, scale = k_pages.clone(), torch.zeros(1, kv, page, dtype=torch.uint8, device=cuda)
+    scales = {"k_scale": scale, "v_scale": scale.clone()}
+    table = torch.zeros(1, 1, dtype=torch.int32, device=cuda)
+    pos, slots = torch.arange(8, device=cuda), torch.zeros(8, dtype=torch.long, device=cuda)
+    cs = modeling.rope_table(modeling.DecoderConfig(model_dim=dim, num_heads=1, max_seq_len=16)).to(cuda)
+    kernels.rope_kv_paged(qkv, cs, pos, k_pages, v_pages, table, heads, slots, **scales)
+    kk, vv = kernels.paged_read(k_pages, v_pages, table, slots, pos, **scales)
+    torch.cuda.synchronize()
+    want, byte = op.quantise(v.float())
+    assert scales["v_scale"][0, 0, :8].tolist() == byte.tolist() and (scales["k_scale"][0, 0, :8] == 127).all()
+    assert not kk.any()
+    got = vv[:, 0].cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+
+
+def test_read_and_write_nothing(cuda):
+    k, v, table, scales = make_cache(cuda, gen(1), 2, 128, 16, [20], True)
+    none = torch.zeros(0, dtype=torch.long, device=cuda)
+    kk, vv = kernels.paged_read(k, v, table, none, none, **scales)
+    assert kk.shape == vv.shape == (0, 2, 128)
+    cs = torch.zeros(4, 64, 2, device=cuda)
+    q = kernels.rope_kv_paged(torch.zeros(0, 8 * 128, dtype=BF, device=cuda), cs, none, k, v, table, 4, none, **scales)
+    assert q.shape == (0, 4, 128)
+    out = kernels.paged_attention(torch.zeros(0, 4, 128, dtype=BF, device=cuda), k, v, table, none, 3, 0.1, **scales)
+    assert out.shape == (0, 4, 128)
+
+
+# ---------------------------------------------------------------------------------------------- paged attention
+
+def attention_case(cuda, heads, kv, dim, page, tokens, lengths, fp8, seed, shared=0, scale=None):
+    say(f"paged attention heads={heads} kv={kv} dim={dim} page={page} T={tokens} lengths={lengths[:9]} fp8={fp8}")
+    g = gen(seed)
+    cache = make_cache(cuda, g, kv, dim, page, [n + tokens - 1 for n in lengths], fp8, shared=shared)
+    k, v, table, scales = cache
+    q = normal((len(lengths) * tokens, heads, dim), g, cuda)
+    n = torch.tensor(lengths, device=cuda)
+    scale = dim ** -0.5 if scale is None else scale
+    out = kernels.paged_attention(q, k, v, table, n, tokens, scale, **scales)
+    torch.cuda.synchronize()
+    want, size = op.paged_attention(q, k, v, table, lengths, tokens, scale, **scales)
+    kf = k.float() * (torch.exp2(scales["k_scale"].float() - 127)[..., None] if fp8 else 1.0)
+    close(out, want, size, q, kf, scale)
+    return out
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_paged_attention(cuda, heads, kv, dim, tokens, fp8):
+    attention_case(cuda, heads, kv, dim, 64, tokens, [1, 700, 0, 33, 64], fp8, heads * dim + tokens)
+    attention_case(cuda, heads, kv, dim, 16, tokens, [31, 257], fp8, heads * dim + tokens + 1, shared=1)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_paged_attention_lengths_around_tiles_and_pages(cuda, page):
+    lengths = [page - 1, page, page + 1, 2 * page + 15, 31, 32, 33, 1]
+    attention_case(cuda, 4, 2, 128, page, 1, lengths, True, page)
+    attention_case(cuda, 2, 2, 512, page, 3, lengths, False, page + 1)
+
+
+@pytest.mark.parametrize("tokens", [9, 16])
+def test_paged_attention_many_columns(cuda, tokens):
+    """More query columns of a kv head than one block of 16."""
+    attention_case(cuda, 8, 2, 128, 32, tokens, [40, 0, 300], True, tokens)
+    attention_case(cuda, 8, 1, 256, 32, tokens, [77], False, tokens + 1)
+    attention_case(cuda, 3, 1, 512, 16, tokens, [130, 2], True, tokens + 2)
+
+
+def test_paged_attention_of_long_rows_and_many_rows(cuda):
+    attention_case(cuda, 2, 1, 128, 256, 1, [8188], True, 1)
+    attention_case(cuda, 2, 2, 128, 64, 1, [8188, 5, 1433], False, 2)
+    attention_case(cuda, 2, 1, 128, 16, 2, [(37 * i) % 91 for i in range(70)], True, 3)
+
+
+def test_paged_attention_with_large_scores(cuda):
+    """Scores of hundreds: the reference maximum moves, weights underflow."""
+    attention_case(cuda, 4, 2, 128, 32, 3, [500, 40], False, 5, scale=1.0)
+    attention_case(cuda, 2, 2, 512, 32, 1, [900], True, 6, scale=1.0)
+
+
+def test_paged_attention_key_counts_are_held_in_the_cache(cuda):
+    g = gen(9)
+    k, v, table, scales = make_cache(cuda, g, 2, 128, 16, [64, 64], True)
+    table = table[:, :4].contiguous()
+    q = normal((4, 4, 128), g, cuda)
+    out = kernels.paged_attention(q, k, v, table, torch.tensor([2 ** 50, -7], device=cuda), 2, 0.1, **scales)
+    same = kernels.paged_attention(q, k, v, table, torch.tensor([64, 0], device=cuda), 2, 0.1, **scales)
+    torch.cuda.synchronize()
+    assert torch.equal(out, same) and out.isfinite().all()
+    want, size = op.paged_attention(q, k, v, table, [64, 0], 2, 0.1, **scales)
+    close(out, want, size, q, torch.full((1, 128), 4.0, device=cuda), 0.1)
+    assert not out[2].any()
+
+
+def test_paged_attention_page_numbers_are_held_in_the_pool(cuda):
+    """Page numbers out of the pool read some page of it: no fault, and the other rows keep their results."""
+    g = gen(10)
+    k, v, table, scales = make_cache(cuda, g, 2, 128, 16, [64, 100], True, spare=0)
+    k, v = (torch.where(x.float().isnan(), torch.zeros((), device=cuda), x.float()).to(torch.float8_e4m3fn) for x in (k, v))
+    q = normal((2, 4, 128), g, cuda)
+    n = torch.tensor([64, 100], device=cuda)
+    good = kernels.paged_attention(q, k, v, table, n, 1, 0.1, **scales)
+    table[0, 0], table[0, 1], table[0, 2] = -1, 2 ** 31 - 1, -2 ** 31
+    out = kernels.paged_attention(q, k, v, table, n, 1, 0.1, **scales)
+    torch.cuda.synchronize()
+    assert torch.equal(out[1], good[1]) and out.isfinite().all()
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("dim", [128, 512])
+def test_paged_attention_does_not_see_what_is_masked(cuda, dim, fp8):
+    """The newest tokens' keys and values hold NaN (bf16: an infinity too): the earlier queries of the step do not see
+    them, the later ones do."""
+    g, tokens, n = gen(dim), 4, 45
+    k, v, table, scales = make_cache(cuda, g, 2, dim, 16, [n + tokens - 1, 70], fp8)
+    q = normal((2 * tokens, 4, dim), g, cuda)
+    at = {p: op.cell(table, 16, k.size(0), 0, p) for p in (n, n + 1)}
+    flat = [x.view(torch.uint8) if fp8 else x for x in (k, v)]
+    nan = 0x7F if fp8 else float("nan")
+    flat[1][at[n][0], 1, at[n][1], 5] = nan if fp8 else float("inf")  # seen from query 1 on
+    flat[0][at[n + 1][0], 0, at[n + 1][1], 3] = nan  # seen from query 2 on
+    flat[1][at[n + 1][0], 1, at[n + 1][1], 77] = nan
+    lengths = torch.tensor([n, 67], device=cuda)
+    out = kernels.paged_attention(q, k, v, table, lengths, tokens, dim ** -0.5, **scales)
+    torch.cuda.synchronize()
+    want, size = op.paged_attention(q, k, v, table, lengths.tolist(), tokens, dim ** -0.5, **scales)
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want.isposinf())
+    assert out[0].isfinite().all() and out[1, :2].isfinite().all() and out[2, :2].isnan().all()
+    fine = want.isfinite()
+    close(torch.where(fine, out.double(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, size, 0.0), q,
+          torch.full((1, dim), 4.0, device=cuda), dim ** -0.5)
+
+
+# ---------------------------------------------------------------------------------------------- packed attention
+
+def packed_case(cuda, heads, kv, dim, queries, past, seed, longest=None, behind=0, strided=True, scale=None):
+    say(f"packed attention heads={heads} kv={kv} dim={dim} queries={queries} past={past}")
+    g = gen(seed)
+    past = [past] * len(queries) if isinstance(past, int) else past
+    keys = [n + p for n, p in zip(queries, past)]
+    starts = torch.tensor([0, *queries]).cumsum(0)
+    k_starts = torch.tensor([0, *keys]).cumsum(0)
+    n, m = int(starts[-1]) + behind, max(int(k_starts[-1]), 0) + behind
+    q, k = normal((n, heads, dim), g, cuda), normal((m, kv, dim), g, cuda)
+    v = normal((m, heads + 2 * kv, dim), g, cuda)[:, heads + kv:] if strided else normal((m, kv, dim), g, cuda)
+    out = torch.full((n, heads, dim), 7.0, dtype=BF, device=cuda)
+    scale = dim ** -0.5 if scale is None else scale
+    got = kernels.packed_attention(q, k, v, starts.to(cuda), max(queries) if longest is None else longest, scale,
+                                   k_starts=None if not any(past) else k_starts.to(cuda), out=out)
+    torch.cuda.synchronize()
+    assert got is out
+    want, size = op.packed_attention(q, k, v, starts.tolist(), k_starts.tolist(), scale)
+    used = int(starts[-1])
+    close(out[:used], want[:used], size[:used], q, k, scale)
+    assert (out[used:] == 7.0).all()
+    return out
+
+
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+def test_packed_attention(cuda, heads, kv, dim):
+    packed_case(cuda, heads, kv, dim, [1, 70, 0, 16, 130, 33], 0, heads * dim, behind=3)
+    packed_case(cuda, heads, kv, dim, [5, 129], [300, 31], heads * dim + 1, strided=False)
+
+
+@pytest.mark.parametrize("dim", [128, 256, 512])
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 191, 193, 256, 257, 400])
+def test_packed_attention_lengths_around_blocks(cuda, dim, n):
+    packed_case(cuda, 2, 1, dim, [n, 3], 0, n + dim)
+    packed_case(cuda, 2, 1, dim, [n], [n % 70 + 1], n + dim + 1)
+
+
+def test_packed_attention_fewer_keys_than_queries(cuda):
+    """Queries before the first key see none: zeros."""
+    out = packed_case(cuda, 4, 2, 128, [100, 40, 300], [-30, -40, -290], 4)
+    assert not out[:30].any() and not out[100:140].any() and not out[140:430].any()
+    packed_case(cuda, 2, 2, 512, [100, 70], [-30, -70], 5)
+    packed_case(cuda, 2, 2, 256, [100, 70], [-64, -70], 6)
+
+
+def test_packed_attention_long_prompt_and_many_short_ones(cuda):
+    packed_case(cuda, 1, 1, 128, [2100], 0, 1)
+    packed_case(cuda, 1, 1, 512, [1500], 600, 2)
+    packed_case(cuda, 8, 2, 128, [(13 * i) % 40 for i in range(40)], 0, 3)
+    packed_case(cuda, 8, 8, 128, [(13 * i) % 40 for i in range(40)], [(7 * i) % 50 for i in range(40)], 4, longest=1000)
+
+
+def test_packed_attention_with_large_scores(cuda):
+    packed_case(cuda, 2, 2, 128, [300, 90], 0, 8, scale=1.0)
+    packed_case(cuda, 2, 1, 512, [200], 50, 9, scale=1.0)
+
+
+def test_packed_attention_nothing(cuda):
+    q = torch.zeros(4, 2, 128, dtype=BF, device=cuda)
+    k = torch.zeros(0, 2, 128, dtype=BF, device=cuda)
+    starts, none = torch.tensor([0, 4], device=cuda), torch.tensor([0, 0], device=cuda)
+    out = kernels.packed_attention(q, k, k, starts, 4, 0.1, k_starts=none)
+    assert not out.any()
+    full = torch.full_like(q, 3.0)
+    assert (kernels.packed_attention(q, q, q, none[:1], 4, 0.1, out=full) == 3).all()
+    assert (kernels.packed_attention(q, q, q, none, 0, 0.1, out=full) == 3).all()
+
+
+@pytest.mark.parametrize("dim", [128, 256, 512])
+def test_packed_attention_does_not_see_what_is_masked(cuda, dim):
+    """NaN and infinities in later positions of a prompt, and in its neighbours, do not reach the queries before them."""
+    g, heads, kv = gen(dim + 1), 2, 1
+    q, k, v = (normal((230, h, dim), g, cuda) for h in (heads, kv, kv))
+    starts = torch.tensor([0, 100, 230], device=cuda)
+    k[90, 0, 3], v[95, 0, 7], v[96, 0, 100], v[100] = float("nan"), float("inf"), float("nan"), float("nan")
+    out = kernels.packed_attention(q, k, v, starts, 130, dim ** -0.5)
+    torch.cuda.synchronize()
+    want, size = op.packed_attention(q, k, v, starts.tolist(), starts.tolist(), dim ** -0.5)
+    fine = want.isfinite()
+    assert fine[:90].all() and not fine[90:].all()
+    assert torch.equal(out.isfinite(), fine)
+    close(torch.where(fine, out.double(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, size, 0.0), q,
+          torch.full((1, dim), 4.0, device=cuda), dim ** -0.5)
+
+
+# ---------------------------------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 512), (8, 2, 128)])
+def test_prompts_then_steps_then_a_continued_prompt(cuda, heads, kv, dim, fp8):
+    """As a decoder uses them: packed prompts into the cache and through the attention, drafted steps over it (captured
+    and replayed), then prompts that go on behind what is cached -- each result against the oracle over the keys and
+    values kept so far."""
+    g, page, tokens, prompts = gen(dim), 32, 3, [50, 1, 90]
+    scale, vecs = dim ** -0.5, heads + 2 * kv
+    cs = modeling.rope_table(modeling.DecoderConfig(model_dim=heads * dim, num_heads=heads, max_seq_len=512)).to(cuda)
+    pool = 3 * 8
+    k, v = (torch.zeros(pool, kv, page, dim, device=cuda).to(torch.float8_e4m3fn if fp8 else BF) for _ in "kv")
+    scales = {a: torch.zeros(pool, kv, page, dtype=torch.uint8, device=cuda) for a in ("k_scale", "v_scale")} if fp8 else {}
+    table = torch.randperm(pool, generator=g).int().view(3, 8).to(cuda)
+
+    def fill(counts, first):
+        slots = torch.repeat_interleave(torch.arange(3), torch.tensor(counts)).to(cuda)
+        pos = torch.cat([torch.arange(n) + f for n, f in zip(counts, first)]).to(cuda)
+        return slots, pos, torch.tensor([0, *counts]).cumsum(0).to(cuda)
+
+    slots, pos, starts = fill(prompts, [0, 0, 0])
+    qkv = normal((len(pos), vecs * dim), g, cuda)
+    q, kr = kernels.rope_kv_paged(qkv, cs, pos, k, v, table, heads, slots, rotated=True, **scales)
+    vr = qkv.view(len(pos), vecs, dim)[:, heads + kv:]
+    out = kernels.packed_attention(q, kr, vr, starts, max(prompts), scale)
+    want, size = op.packed_attention(q, kr, vr, starts.tolist(), starts.tolist(), scale)
+    close(out, want, size, q, kr, scale)
+
+    # two drafted steps through one captured graph
+    step_qkv = torch.zeros(3 * tokens, vecs * dim, dtype=BF, device=cuda)
+    lengths = torch.tensor(prompts, device=cuda) + 1
+    held = {}
+
+    def step():
+        at = (lengths[:, None] - 1 + torch.arange(tokens, device=cuda)).flatten()
+        rows = torch.arange(3, device=cuda).repeat_interleave(tokens)
+        held["q"] = kernels.rope_kv_paged(step_qkv, cs, at, k, v, table, heads, rows, **scales)
+        held["out"] = kernels.paged_attention(held["q"], k, v, table, lengths, tokens, scale, **scales)
+
+    graphs = batching.GraphCache(cuda, True)
+    run = graphs.runner("step", step, lambda: [])
+    captured = dict(held)  # the graph's own outputs
+    for _ in range(3):
+        step_qkv.copy_(normal(step_qkv.shape, g, cuda))
+        run()
+        torch.cuda.synchronize()
+        n = lengths.tolist()
+        want, size = op.paged_attention(captured["q"], k, v, table, n, tokens, scale, **scales)
+        kf = torch.cat([op.cached(k, scales.get("k_scale"), table[b], n[b], 0) for b in range(3)])
+        close(captured["out"], want, size, captured["q"], kf * 1.5, scale)
+        step()
+        assert torch.equal(captured["out"], held["out"])
+        lengths += 2
+
+    # prompts that go on behind the cached positions
+    past = (lengths - 1).tolist()
+    more = [20, 70, 3]
+    slots, pos, starts = fill(more, past)
+    qkv = normal((len(pos), vecs * dim), g, cuda)
+    q = kernels.rope_kv_paged(qkv, cs, pos, k, v, table, heads, slots, **scales)
+    total = [a + b for a, b in zip(past, more)]
+    all_slots, all_pos, k_starts = fill(total, [0, 0, 0])
+    kk, vv = kernels.paged_read(k, v, table, all_slots, all_pos, **scales)
+    out = kernels.packed_attention(q, kk, vv, starts, max(more), scale, k_starts=k_starts)
+    torch.cuda.synchronize()
+    for b in range(3):
+        kept = op.cached(k, scales.get("k_scale"), table[b], total[b], 1)
+        assert torch.equal(kk[k_starts[b]:k_starts[b + 1], 1].double(), kept)
+    want, size = op.packed_attention(q, kk, vv, starts.tolist(), k_starts.tolist(), scale)
+    close(out, want, size, q, kk, scale)
+
+
+def test_as_the_full_length_caches(cuda):
+    """The same step over a full-length cache and over pages of it: the two kernels agree to their roundings."""
+    g, b, t, h, d, cap, page = gen(11), 3, 5, 4, 128, 256, 64
+    kc, vc, q = normal((b, h, cap, d), g, cuda), normal((b, h, cap, d), g, cuda), normal((b * t, h, d), g, cuda)
+    lengths = torch.tensor([200, 0, 77], device=cuda)
+    pages = [x.view(b, h, cap // page, page, d).transpose(1, 2).flatten(0, 1).contiguous() for x in (kc, vc)]
+    table = torch.arange(b * (cap // page), dtype=torch.int32, device=cuda).view(b, -1)
+    one = kernels.draft_attention(q, kc, vc, lengths, t, cap, d ** -0.5)
+    two = kernels.paged_attention(q, *pages, table, lengths, t, d ** -0.5)
+    _, size = op.paged_attention(q, *pages, table, lengths.tolist(), t, d ** -0.5)
+    assert bool(((one.double() - two.double()).abs() <= 2 * (2.0 ** -8 * two.double().abs()
+                                                             + (2.0 ** -8 + 2.0 ** -12) * size)).all())
+
+
+def test_two_streams_at_once(cuda):
+    """Calls on two streams share nothing: each equals the call alone."""
+    g = gen(12)
+    cases = []
+    for lengths in ([700, 33], [90, 1200]):
+        k, v, table, scales = make_cache(cuda, g, 2, 128, 32, lengths, True)
+        cases.append((normal((2, 8, 128), g, cuda), k, v, table, torch.tensor(lengths, device=cuda), scales))
+    alone = [kernels.paged_attention(q, k, v, t, n, 1, 0.1, **s) for q, k, v, t, n, s in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(20):
+        for i, (q, k, v, t, n, s) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(kernels.paged_attention(q, k, v, t, n, 1, 0.1, **s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, alone[i]) for x in got[i])
