@@ -2,6 +2,10 @@
 //     F.scaled_dot_product_attention(q, k, v, is_causal=True)
 // (src/omniasr_trt/decode.py:163-164) over the cache rows ``kernels.rope_kv`` has just written.  Query p of context
 // b attends to keys [0, p] of its cache row; fp32 accumulation, bf16 in and out, head_dim 128, 256 or 512.
+//
+// The same kernels (kPacked) attend packed prompts of different lengths with grouped heads over k and v as a projection
+// leaves them: sequence s has queries starts[s] .. of q and keys k_starts[s] .. of k / v, and its query i of nq sees its
+// keys [0, i + nk - nq] of nk.
 #include <math.h>
 
 #include <algorithm>
@@ -27,7 +31,56 @@ struct PrefillArgs {
   float scale_log2;
   uint16_t* out;  // [B * width, H, D] bf16
   int units8, group;  // head dim 512 in chains: heads x contexts / 8, and how many of them are listed together
+  // Packed prompts (width: the longest's queries); element strides of a key and of a head in k and v.
+  const int64_t* starts = nullptr;    // [sequences + 1]
+  const int64_t* k_starts = nullptr;  // [sequences + 1]
+  int64_t queries = 0, keys = 0;      // rows of q, of k and v
+  int64_t k_pos = 0, k_head = 0, v_pos = 0, v_head = 0;
+  int heads_per_kv = 1;
 };
+
+// A context's or sequence's part of a call for one head: queries q0 .. q0 + nq - 1, keys 0 .. nk - 1 of k / v, rows
+// k_bytes / v_bytes apart; query i sees keys [0, i + before].
+struct PfSpan {
+  int64_t q0;
+  int nq, nk, before;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint32_t k_bytes, v_bytes;
+};
+
+template <int D, bool kPacked>
+__device__ __forceinline__ PfSpan pf_span(const PrefillArgs& a, int h, int b) {
+  PfSpan p;
+  if constexpr (kPacked) {
+    p.q0 = clamp64(a.starts[b], 0, a.queries);
+    const int64_t k0 = clamp64(a.k_starts[b], 0, a.keys), nq = clamp64(a.starts[b + 1], p.q0, a.queries) - p.q0;
+    p.nk = (int)(clamp64(a.k_starts[b + 1], k0, a.keys) - k0);
+    p.before = p.nk - (int)nq;
+    p.nq = (int)(nq < a.width ? nq : a.width);
+    const int kv = h / a.heads_per_kv;
+    p.k = a.k + k0 * a.k_pos + kv * a.k_head;
+    p.v = a.v + k0 * a.v_pos + kv * a.v_head;
+    p.k_bytes = (uint32_t)a.k_pos * 2;
+    p.v_bytes = (uint32_t)a.v_pos * 2;
+  } else {
+    const int64_t slot = clamp64(a.slots[b], 0, a.cache_rows - 1);
+    p.q0 = (int64_t)b * a.width;
+    p.nq = p.nk = a.width;
+    p.before = 0;
+    p.k = a.k + slot * a.s_row + h * a.s_head;
+    p.v = a.v + slot * a.s_row + h * a.s_head;
+    p.k_bytes = p.v_bytes = D * 2;
+  }
+  return p;
+}
+
+// Zeros in rows [q0, q1) of one head: queries that see no key.
+template <int D>
+__device__ __forceinline__ void pf_zeros(const PrefillArgs& a, int64_t q0, int64_t q1, int h) {
+  for (int64_t i = threadIdx.x; i < (q1 - q0) * (D / 8); i += blockDim.x)
+    *reinterpret_cast<u32x4_t*>(a.out + ((q0 + i / (D / 8)) * a.H + h) * D + i % (D / 8) * 8) = u32x4_t{0u, 0u, 0u, 0u};
+}
 
 // Workgroup -> (query block j counted from the longest, head h, context b).  The dispatcher hands consecutive
 // workgroups to the 8 XCDs in turn; when heads x contexts is a multiple of 8, XCD x gets units (head, context)
@@ -45,6 +98,32 @@ __device__ __forceinline__ PfBlock pf_block(int nqb, int H, int B) {
   return PfBlock{k % nqb, unit % H, unit / H};
 }
 
+// The same for packed prompts: XCD x's heads are x * H / 8 .., so that heads of one kv head stay in one L2.
+__device__ __forceinline__ PfBlock pf_packed_block(int nqb, int H, int B) {
+  if (H % 8 != 0) return pf_block(nqb, H, B);
+  const int L = (int)blockIdx.x + nqb * ((int)blockIdx.y + H * (int)blockIdx.z);
+  const int k = L / 8, unit = k / nqb;
+  return PfBlock{k % nqb, L % 8 * (H / 8) + unit % (H / 8), unit / (H / 8)};
+}
+
+// On tiles with keys that some query does not see, their probability is 0, but 0 times an infinity or NaN of V would
+// reach the query's output.  V operands of such a tile are looked at; where one holds such a value the products run
+// without it, and pf_add_nonfinite adds it for the queries that see it.
+__device__ __forceinline__ bool pf_nonfinite(u32x4_t w) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+__device__ __forceinline__ u32x4_t pf_finite(u32x4_t w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
+  }
+  return w;
+}
+
 // Head dim 256: one workgroup of kPwWaves waves per (query block, head, context).  The block's
 // NG = kPwSub * M groups of 16 queries (M = kPwWaves / (D/128)): group gi holds queries qb + 16 gi .. + 15.  Wave w
 // holds the 128-dimension slice sl = w % (D/128) of q and O for the groups m + M u (m = w / (D/128), u < kPwSub).
@@ -60,6 +139,7 @@ __device__ __forceinline__ PfBlock pf_block(int nqb, int H, int B) {
 constexpr int kPwWaves = 8;
 constexpr int kPwSub = 3;  // 16-query groups per wave
 
+template <bool kPacked>
 __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill_attn_wide_kernel(
     PrefillArgs a) {
   constexpr int D = 256;
@@ -77,27 +157,32 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
   __shared__ int rflag[NG];                 // the group's reference max moved on this tile
   __shared__ float lsum[NG][16];            // probability sum of each query, at the end
   const int nqb = (a.width + QW - 1) / QW;
-  const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
+  const PfBlock blk = kPacked ? pf_packed_block(nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
   const int qb = (nqb - 1 - blk.j) * QW;  // the longest blocks first
   const int h = blk.h, b = blk.b;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int sl = w % NSL, m = w / NSL;
-  const int64_t slot = clamp64(a.slots[b], 0, a.cache_rows - 1);
-  const uint16_t* kbase = a.k + slot * a.s_row + h * a.s_head;
-  const uint16_t* vbase = a.v + slot * a.s_row + h * a.s_head;
-  const int kend = min(qb + QW, a.width);
+  const PfSpan sp = pf_span<D, kPacked>(a, h, b);
+  const uint16_t* kbase = sp.k;
+  const uint16_t* vbase = sp.v;
+  const int64_t k_pos = kPacked ? a.k_pos : D, v_pos = kPacked ? a.v_pos : D;
+  const int kend = min(qb + QW, sp.nq) + sp.before;
+  if constexpr (kPacked) {
+    if (qb >= sp.nq) return;
+    if (kend <= 0) return pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + QW, sp.nq), h);
+  }
   const int nt = (kend + 31) / 32;
 
   // Global -> LDS through one set of staging registers: thread tid moves 16-byte chunks tid, tid + 64 kPwWaves, ...
   // of a tile's K or V rows.  Rows past the context read its last key (finite: masked by the causal limit).
   u32x4_t stage[kChunks];
-  auto fetch = [&](int t, const uint16_t* base) {
+  auto fetch = [&](int t, const uint16_t* base, int64_t pos) {
 #pragma unroll
     for (int e = 0; e < kChunks; ++e) {
       const int ci = tid + e * 64 * kPwWaves, r = ci / kRowChunks, col = ci % kRowChunks;
-      const int key = min(t * 32 + r, a.width - 1);
-      stage[e] = *reinterpret_cast<const u32x4_t*>(base + (int64_t)key * D + col * 8);
+      const int key = min(t * 32 + r, sp.nk - 1);
+      stage[e] = *reinterpret_cast<const u32x4_t*>(base + (int64_t)key * pos + col * 8);
     }
   };
   auto put = [&](char* dst) {
@@ -108,15 +193,15 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
     }
   };
   // Whether group gi sees the tile starting at key0: a live group whose last query reaches the tile's first key.
-  auto sees = [&](int gi, int key0) { return qb + 16 * gi < a.width && key0 <= qb + 16 * gi + 15; };
+  auto sees = [&](int gi, int key0) { return qb + 16 * gi < sp.nq && key0 <= qb + 16 * gi + 15 + sp.before; };
 
   u32x4_t qop[kPwSub][4];  // lane (c, g): q[qb + 16 gi + c][128 sl + 32 s2 + 8g .. +7] (0 past the end)
   f32x4_t o[kPwSub][8];    // output column c of block e: dimension 128 sl + 16 e + c
 #pragma unroll
   for (int u = 0; u < kPwSub; ++u) {
     const int row = qb + 16 * (m + M * u) + c;
-    const bool live = row < a.width;
-    const uint16_t* qrow = a.q + ((int64_t)(b * a.width + (live ? row : 0)) * a.H + h) * D + 128 * sl + g * 8;
+    const bool live = row < sp.nq;
+    const uint16_t* qrow = a.q + ((sp.q0 + (live ? row : 0)) * a.H + h) * D + 128 * sl + g * 8;
 #pragma unroll
     for (int s2 = 0; s2 < 4; ++s2)
       qop[u][s2] = live ? *reinterpret_cast<const u32x4_t*>(qrow + s2 * 32) : u32x4_t{0u, 0u, 0u, 0u};
@@ -127,11 +212,11 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
   for (int r = 0; r < OWN; ++r) st[r] = SoftmaxState{-INFINITY, -INFINITY, 0.f};
 
-  fetch(0, kbase);
+  fetch(0, kbase, k_pos);
   put(kl);
-  fetch(0, vbase);
+  fetch(0, vbase, v_pos);
   put(vl[0]);
-  if (nt > 1) fetch(1, kbase);
+  if (nt > 1) fetch(1, kbase, k_pos);
   lds_barrier();
   for (int t = 0; t < nt; ++t) {
     const int key0 = t * 32;
@@ -163,7 +248,7 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
     lds_barrier();
     if (t + 1 < nt) {
       put(kl);             // every wave has read this tile's K
-      fetch(t + 1, vbase);  // the next V, in flight during steps 2 and 3
+      fetch(t + 1, vbase, v_pos);  // the next V, in flight during steps 2 and 3
     }
     // 2. the softmax of this wave's own groups
 #pragma unroll
@@ -181,8 +266,8 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
       float sv[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) sv[j] = sum[j >> 2][j & 3];
-      const int lim = q0 + c + 1;
-      if (!(key0 + 31 <= q0)) {  // not every query of the group sees the whole tile
+      const int lim = q0 + c + 1 + sp.before;
+      if (!(key0 + 31 <= q0 + sp.before)) {  // not every query of the group sees the whole tile
 #pragma unroll
         for (int j = 0; j < 8; ++j) sv[j] = key0 + 8 * g + j < lim ? sv[j] : -INFINITY;
       }
@@ -237,6 +322,35 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
       }
       // V operands by transpose reads from this wave's slice of the rows: within 16 lanes, lane 4r + q points at key r,
       // dimensions 4q .. + 3, and lane c receives dimension c of the four keys.
+      bool bad = false;
+      if (kPacked && key0 + 31 > qb + 16 * m + sp.before) {  // not every query of the wave's groups sees every key
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          bad |= pf_nonfinite(
+              *reinterpret_cast<const u32x4_t*>(&vl[t & 1][(4 * i + (lane >> 4)) * kRowB + 256 * sl + (lane & 15) * 16]));
+        bad = __any(bad);
+      }
+      if (kPacked && bad) {
+        for (int key = 0; key < 32 && key0 + key < sp.nk; ++key) {
+          const uint16_t* row = reinterpret_cast<const uint16_t*>(&vl[t & 1][key * kRowB + 256 * sl]);
+#pragma unroll
+          for (int u = 0; u < kPwSub; ++u) {
+            const int gi = m + M * u;
+            if (!sees(gi, key0)) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = bf16_to_f32(
+                  reinterpret_cast<const uint16_t*>(&pex[gi][4 * g + i + 16 * (key >> 3)])[key & 7]);
+              const bool seen = key0 + key <= qb + 16 * gi + 4 * g + i + sp.before;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t bits = row[16 * e + c];
+                if ((bits & 0x7f80u) == 0x7f80u && seen) o[u][e][i] += p * bf16_to_f32(bits);
+              }
+            }
+          }
+        }
+      }
       const int rr = c >> 2, q4 = c & 3;
       const lds_char* vls = (const lds_char*)vl[t & 1];  // vl lives in LDS
 #pragma unroll
@@ -249,6 +363,7 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
         bop[1] = (uint32_t)(uint16_t)lo[2] | ((uint32_t)(uint16_t)lo[3] << 16);
         bop[2] = (uint32_t)(uint16_t)hi[0] | ((uint32_t)(uint16_t)hi[1] << 16);
         bop[3] = (uint32_t)(uint16_t)hi[2] | ((uint32_t)(uint16_t)hi[3] << 16);
+        if (kPacked && bad) bop = pf_finite(bop);
 #pragma unroll
         for (int u = 0; u < kPwSub; ++u) {
           if (!sees(m + M * u, key0)) continue;
@@ -259,7 +374,7 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
     }
     if (t + 1 < nt) {
       put(vl[(t + 1) & 1]);  // read last by tile t - 1's P V, before this tile's first barrier
-      if (t + 2 < nt) fetch(t + 2, kbase);
+      if (t + 2 < nt) fetch(t + 2, kbase, k_pos);
     }
   }
 
@@ -279,10 +394,10 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int qq = qb + 16 * gi + 4 * g + i;
-      if (qq >= a.width) continue;
+      if (qq >= sp.nq) continue;
       const float li = lsum[gi][4 * g + i];
       const float div = li > 0.f ? li : 1.f;
-      uint16_t* orow = a.out + ((int64_t)(b * a.width + qq) * a.H + h) * D + 128 * sl;
+      uint16_t* orow = a.out + ((sp.q0 + qq) * a.H + h) * D + 128 * sl;
 #pragma unroll
       for (int e = 0; e < 8; ++e) orow[16 * e + c] = (uint16_t)pack_bf16x2(o[u][e][i] / div, 0.f);
     }
@@ -327,6 +442,34 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
+}
+
+// What pf_finite left out of O^T += V^T P^T for one tile of 64 keys from ``key0``: O [query half u][e], register 4q + i of
+// lane half g in row 8q + 4g + i, dimension dim(e, row); P [u][16-key step][lane] as the score waves write it.
+template <typename Dim>
+__device__ void pf_add_nonfinite(f32x16_t (&o)[2][4], const u32x4_t (*ps)[4][64], const uint16_t* v, uint32_t v_bytes,
+                                 int key0, int nk, int query0, int before, int x, int g, Dim dim) {
+  for (int key = 0; key < 64 && key0 + key < nk; ++key) {
+    const int r = key & 31, i16 = 4 * (r >> 3) + (r & 3), from = x + 32 * ((r >> 2) & 1);
+    const uint16_t* row = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v) +
+                                                            (int64_t)(key0 + key) * v_bytes);
+    float p[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint16_t* word = reinterpret_cast<const uint16_t*>(&ps[u][2 * (key >> 5) + (i16 >> 3)][from]);
+      p[u] = bf16_to_f32(word[i16 & 7]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        const uint32_t bits = row[dim(e, 8 * (n >> 2) + 4 * g + (n & 3))];
+        if ((bits & 0x7f80u) != 0x7f80u) continue;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (key0 + key <= query0 + 32 * u + x + before) o[u][e][n] += p[u] * bf16_to_f32(bits);
+      }
+  }
 }
 
 // A wave-uniform pointer in scalar registers.
@@ -399,13 +542,13 @@ inline int ws_group(int nqb, int units8) {
 struct WsBlock {
   int round, qb, h, b;
 };
-struct WsTile {  // key tile t of a block
+struct WsTile {  // key tile t of a block, the last its ``last``
   WsBlock blk;
-  int t;
+  int t, last, nk;
   const char *kbase, *vbase;
 };
 
-template <bool kChain>
+template <bool kChain, bool kPacked>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill_attn_ws_kernel(PrefillArgs a) {
   constexpr int D = kWsD;
   __shared__ __attribute__((aligned(16))) char kls[2][kWsK * kWsRow];
@@ -433,7 +576,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (kChain) {
       place(blk, 0);
     } else {
-      const PfBlock one = pf_block(nqb, a.H, (int)gridDim.z);
+      const PfBlock one = kPacked ? pf_packed_block(nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
       blk = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, one.b};  // the longest blocks first
     }
     return blk;
@@ -442,6 +585,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (kChain) return place(blk, blk.round + 1);
     return false;
   };
+  auto span = [&](const WsBlock& blk) { return pf_span<D, kPacked>(a, blk.h, blk.b); };
+  // The block's last tile: the one of its last query's last key.
+  auto last_tile = [&](const WsBlock& blk, const PfSpan& sp) {
+    return kPacked ? (min(blk.qb + kWsQ, sp.nq) - 1 + sp.before) / kWsK : blk.qb / kWsK;
+  };
+  if constexpr (kPacked) {
+    const WsBlock blk = first();
+    const PfSpan sp = span(blk);
+    if (blk.qb >= sp.nq) return;
+    const int end = min(blk.qb + kWsQ, sp.nq);
+    if (end + sp.before <= 0) return pf_zeros<D>(a, sp.q0 + blk.qb, sp.q0 + end, blk.h);
+  }
 
   if (w < 4) {  // ------------------------------------------------------------------------------ scores
     const int qh = w & 1, kh = w >> 1;
@@ -453,10 +608,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     WsBlock blk = first();
     int t = 0;  // counted over the workgroup's blocks, as is all LDS
     for (int odd = 0;; odd ^= 1) {
-      const int qb = blk.qb, query = qb + 32 * qh + x, t_last = t + qb / kWsK;  // the last tile holds the diagonal
+      const PfSpan sp = span(blk);
+      const int qb = blk.qb, query = qb + 32 * qh + x, t_first = t;
+      const int t_last = t + last_tile(blk, sp);  // the last tile holds the diagonal
       u32x4_t q[D / 16];  // q[query][16s + 8g .. + 7] (past the end the last query's: its results are not stored)
       {
-        const uint16_t* qrow = a.q + ((int64_t)(blk.b * a.width + min(query, a.width - 1)) * a.H + blk.h) * D + g * 8;
+        const uint16_t* qrow = a.q + ((sp.q0 + min(query, sp.nq - 1)) * a.H + blk.h) * D + g * 8;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4_t*>(qrow + s * 16);
       }
@@ -483,8 +640,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         float sv[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) sv[i] = s0[i] + s1[i];
-        if (t == t_last) {
-          const int rel = 32 * qh + x - (32 * kh + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
+        const int whole = kPacked ? qb + sp.before - (t - t_first) * kWsK : 0;  // of the tile's keys, seen by every query
+        if (kPacked ? whole < kWsK - 1 : t == t_last) {
+          const int rel = whole + 32 * qh + x - (32 * kh + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
 #pragma unroll
           for (int i = 0; i < 16; ++i) sv[i] = 8 * (i >> 2) + (i & 3) <= rel ? sv[i] : -INFINITY;
         }
@@ -552,31 +710,44 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // K rows 16 vw .. + 15 of tile t to LDS, one row (64 lanes x 16 bytes) per load; rows past the context read its last
   // key (finite: masked).
   auto bring_k = [&](const WsTile& c, int n) {  // as tile n of the workgroup
-    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(c.kbase), 0, -1, 0x00020000);
+    const uint32_t row_bytes = kPacked ? (uint32_t)a.k_pos * 2 : D * 2;
+    const int t0 = kPacked ? c.t * kWsK : 0;  // packed rows may be far apart: their offsets within the tile
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(c.kbase + (int64_t)t0 * row_bytes), 0, -1, 0x00020000);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int key = min(c.t * kWsK + 16 * vw + r, a.width - 1);
+      const int key = min(c.t * kWsK + 16 * vw + r, (kPacked ? c.nk : a.width) - 1) - t0;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           kr, (__attribute__((address_space(3))) void*)&kls[n & 1][(16 * vw + r) * kWsRow], 16, lane * 16,
-          (int)((uint32_t)key * (D * 2)), 0,
+          (int)((uint32_t)key * row_bytes), 0,
           0);
     }
   };
   // V of 16-key step s of tile t: lane (c = x % 16, u = x / 16, g) loads keys 16s + 8u + 4g + j, dimensions 128 vw + 8c
   // .. + 7, j < 4.  A buffer resource per step, its size what is left of the context's rows: scalar work only, and rows
   // past the end read 0.
-  const uint32_t vlane = (uint32_t)((8 * (x >> 4) + 4 * g) * D + 128 * vw + 8 * (x & 15)) * 2;
+  const uint32_t v_bytes = kPacked ? (uint32_t)a.v_pos * 2 : D * 2;
+  const uint32_t vlane = (uint32_t)(8 * (x >> 4) + 4 * g) * v_bytes + (uint32_t)(128 * vw + 8 * (x & 15)) * 2;
   const uint32_t vbytes = (uint32_t)a.width * (D * 2);
   u32x4_t v[4][4];
   auto load_v = [&](const WsTile& c, int s) {
-    const uint32_t off = (uint32_t)(c.t * kWsK + 16 * s) * (D * 2);
-    uint32_t used = min(off, vbytes);
-    asm("" : "+s"(used));  // kept scalar (the saturating subtraction it would become is a vector instruction)
-    const __amdgpu_buffer_rsrc_t vr =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(c.vbase) + off, 0, vbytes - used, 0x00020000);
+    const char* from;
+    uint32_t room;  // bytes from there that are the context's
+    if constexpr (kPacked) {
+      const int at = c.t * kWsK + 16 * s, rows = min(c.nk - at, 16);
+      from = c.vbase + (int64_t)at * v_bytes;
+      room = rows > 0 ? (uint32_t)(rows - 1) * v_bytes + D * 2 : 0;
+    } else {
+      const uint32_t off = (uint32_t)(c.t * kWsK + 16 * s) * (D * 2);
+      uint32_t used = min(off, vbytes);
+      asm("" : "+s"(used));  // kept scalar (the saturating subtraction it would become is a vector instruction)
+      from = c.vbase + off;
+      room = vbytes - used;
+    }
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(from), 0, room, 0x00020000);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      v[s][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, vlane + j * D * 2, 0, 0));
+      v[s][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, vlane + j * v_bytes, 0, 0));
   };
   u32x4_t p[2][2];  // steps s, s + 1 of tile t
   auto read_p = [&](int t, int s) {
@@ -585,8 +756,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   // O^T += V^T P^T for the workgroup's tile t; ``ahead``: the next tile's V loads as its registers fall free.  Step
   // s + 1's operands are built beside step s's products; the scheduler keeps each step's loads behind the permutes that read their registers.
-  auto attend_v = [&](int t, const WsTile* ahead) {
+  auto attend_v = [&](int t, const WsTile& cur, const WsTile* ahead) {
     u32x4_t vop[2][4];
+    if constexpr (kPacked) {
+      const PfSpan sp = span(cur.blk);
+      if (cur.t * kWsK + kWsK - 1 > cur.blk.qb + sp.before) {  // not every query sees every key
+        bool bad = false;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) bad |= pf_nonfinite(v[s][j]);
+        if (__any(bad)) {
+          pf_add_nonfinite(o, ps[t & 1], sp.v + 128 * vw, v_bytes, cur.t * kWsK, sp.nk, cur.blk.qb, sp.before, x, g,
+                           [](int e, int row) { return 8 * (row & 15) + 4 * (row >> 4) + e; });
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[s][j] = pf_finite(v[s][j]);
+        }
+      }
+    }
     auto operands = [&](int s) {
       // The lanes of a pair (u = 0, 1) hold 8 dimensions of 4 keys each; swapped, 4 dimensions (8c + 4u ..) of 8 keys:
       // lo[j] of key 16s + 4g + j, hi[j] of key 16s + 8 + 4g + j.
@@ -646,17 +835,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   };
   auto output = [&](const WsBlock& blk, int odd) {  // O of a finished block; then O is 0 again
+    const PfSpan sp = span(blk);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int query = blk.qb + 32 * u + x;
       const float l = (lsum[odd][0][0][32 * u + x] + lsum[odd][0][1][32 * u + x]) +
                       (lsum[odd][1][0][32 * u + x] + lsum[odd][1][1][32 * u + x]);
       const float inv = l > 0.f ? 1.f / l : 1.f;
-      uint16_t* orow = a.out + ((int64_t)(blk.b * a.width + query) * a.H + blk.h) * D + 128 * vw + 32 * g;
+      uint16_t* orow = a.out + ((sp.q0 + query) * a.H + blk.h) * D + 128 * vw + 32 * g;
       auto pair = [&](float lo, float hi) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
       };
-      if (query < a.width) {
+      if (query < sp.nq) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -678,13 +868,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   };
   auto open = [&](WsTile& c) {  // the block's first tile
-    const int64_t slot = clamp64(a.slots[c.blk.b], 0, a.cache_rows - 1);
-    c.kbase = scalar_pointer(a.k + slot * a.s_row + c.blk.h * a.s_head);
-    c.vbase = scalar_pointer(a.v + slot * a.s_row + c.blk.h * a.s_head);
+    const PfSpan sp = span(c.blk);
+    c.kbase = scalar_pointer(sp.k);
+    c.vbase = scalar_pointer(sp.v);
+    c.nk = sp.nk;
+    c.last = last_tile(c.blk, sp);
     c.t = 0;
   };
   auto advance = [&](WsTile& c) {  // false (and c as it was): no more tiles
-    if (c.t < c.blk.qb / kWsK) {
+    if (c.t < c.last) {
       ++c.t;
       return true;
     }
@@ -706,11 +898,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   take_p(0);
   int n = 1, odd = 0;
   while (more) {  // tile n's scores, tile n - 1's values
-    const WsBlock was = at.blk;
+    const WsTile was = at;
     at = ahead;
     more = advance(ahead);
     bring_k(ahead, n + 1);  // unconditional (past the last tile: that tile again, not used): no wait joins a branch
-    attend_v(n - 1, &at);
+    attend_v(n - 1, was, &at);
     // vmcnt(16): tile n + 1's K rows are in LDS, tile n's 16 V loads, issued after them, stay in flight (lds_barrier
     // would wait for those too).  This wave's LDS reads of the tile are in registers by now.
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -718,13 +910,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     if (kChain && at.t == 0) {
-      output(was, odd);
+      output(was.blk, odd);
       odd ^= 1;
     }
     take_p(n);
     ++n;
   }
-  attend_v(n - 1, nullptr);
+  attend_v(n - 1, at, nullptr);
   lds_barrier();
   output(at.blk, odd);
 }
@@ -755,6 +947,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+template <bool kPacked>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill_attn_pairs_kernel(
     PrefillArgs a) {
   constexpr int D = 128;
@@ -765,39 +958,50 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ int moved[4][4];
   __shared__ float lsum[4][2][64];        // [pair][lane half]
   const int nqb = (a.width + kPairQ - 1) / kPairQ;
-  const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
+  const PfBlock blk = kPacked ? pf_packed_block(nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
   const int qb = (nqb - 1 - blk.j) * kPairQ;  // the longest blocks first
   const int h = blk.h, b = blk.b;
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), pr = w & 3;
-  const int64_t slot = clamp64(a.slots[b], 0, a.cache_rows - 1);
-  const char* kbase = scalar_pointer(a.k + slot * a.s_row + h * a.s_head);
-  const char* vbase = scalar_pointer(a.v + slot * a.s_row + h * a.s_head);
-  const int nt = (min(qb + kPairQ, a.width) + kPairK - 1) / kPairK;
+  const PfSpan sp = pf_span<D, kPacked>(a, h, b);
+  const char* kbase = scalar_pointer(sp.k);
+  const char* vbase = scalar_pointer(sp.v);
+  const int keys = min(qb + kPairQ, sp.nq) + sp.before;  // what the block's last query sees
+  if constexpr (kPacked) {
+    if (qb >= sp.nq) return;
+    if (keys <= 0) return pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + kPairQ, sp.nq), h);
+  }
+  const int nt = (keys + kPairK - 1) / kPairK;
   const int qp = qb + 64 * pr;
-  const int dq = qp < a.width ? qp / kPairK : -1;  // the pair's last tile, which holds its diagonal (-1: no queries)
+  // The pair's last tile, which holds its diagonal (-1: no queries, or they see no key).
+  const int lastk = kPacked ? min(qp + 64, sp.nq) - 1 + sp.before : qp;
+  const int dq = qp < sp.nq && lastk >= 0 ? lastk / kPairK : -1;
+  const int whole = qp + sp.before;  // every query of the pair sees keys [0, whole]
 
   // Rows 16 pr .. + 15 of tile t to LDS; rows past the context read its last key (finite: masked).  ``swap``: the chunk
   // permutation of key row r of a 16-row group.
-  auto bring = [&](const __amdgpu_buffer_rsrc_t rsrc, char* dst, int t, auto swap) {
+  auto bring = [&](const char* base, uint32_t row_bytes, char* dst, int t, auto swap) {
+    // Packed rows may be far apart: a resource per tile, its rows' offsets within it.
+    const int t0 = kPacked ? t * kPairK : 0;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(base + (int64_t)t0 * row_bytes), 0, -1, 0x00020000);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = 4 * j + (lane >> 4);
-      const int key = min(t * kPairK + 16 * pr + r, a.width - 1);
-      const uint32_t from = (uint32_t)key * (D * 2) + (uint32_t)((lane & 15) ^ swap(r)) * 16;
+      const int key = min(t * kPairK + 16 * pr + r, sp.nk - 1) - t0;
+      const uint32_t from = (uint32_t)key * row_bytes + (uint32_t)((lane & 15) ^ swap(r)) * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rsrc, (__attribute__((address_space(3))) void*)(dst + (16 * pr + 4 * j) * (D * 2)), 16, from, 0, 0, 0);
     }
   };
 
   if (w < 4) {  // ------------------------------------------------------------------------------ scores
-    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vbase), 0, -1, 0x00020000);
-    auto bring_v = [&](int t) { bring(vr, vls[t & 1], t, [](int r) { return 4 * (r & 3); }); };
+    auto bring_v = [&](int t) { bring(vbase, sp.v_bytes, vls[t & 1], t, [](int r) { return 4 * (r & 3); }); };
     u32x4_t q[2][D / 16];  // q[query][16s + 8g .. + 7], query qp + 32u + x
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint16_t* qrow =
-          a.q + ((int64_t)(b * a.width + min(qp + 32 * u + x, a.width - 1)) * a.H + h) * D + g * 8;
+          a.q + ((sp.q0 + min(qp + 32 * u + x, sp.nq - 1)) * a.H + h) * D + g * 8;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) q[u][s] = *reinterpret_cast<const u32x4_t*>(qrow + s * 16);
     }
@@ -826,12 +1030,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     auto refer = [&](Scores& sc, int t) {
       // max3's operands come from the matrix unit: every product has written its result after 24 wait states.
       asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sc[0][0]), "+v"(sc[0][1]), "+v"(sc[1][0]), "+v"(sc[1][1]));
-      if (t == dq) {
+      if (kPacked ? t * kPairK + kPairK - 1 > whole : t == dq) {
+        const int off = kPacked ? whole - t * kPairK : 0;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int rel = 32 * u + x - (32 * m + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
+            const int rel = off + 32 * u + x - (32 * m + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[m][u][i] = 8 * (i >> 2) + (i & 3) <= rel ? sc[m][u][i] : -INFINITY;
           }
@@ -919,8 +1124,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 
   // ---------------------------------------------------------------------------------------------- values
-  const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kbase), 0, -1, 0x00020000);
-  auto bring_k = [&](int t) { bring(kr, kls[t & 1], t, [](int r) { return r; }); };
+  auto bring_k = [&](int t) { bring(kbase, sp.k_bytes, kls[t & 1], t, [](int r) { return r; }); };
   f32x16_t o[2][4];  // [query half][e]: row 16k + 4q + i is dimension 32e + 8q + 4k + i, column x query x of the half
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -951,6 +1155,19 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
     const lds_char* vt = (const lds_char*)vls[t & 1];
+    bool bad = false;
+    if (kPacked && t * kPairK + kPairK - 1 > whole) {  // wave-uniform: not every query sees every key
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        // The whole tile: row 4i + lane / 16, 16 bytes a lane.
+        bad |= pf_nonfinite(*reinterpret_cast<const u32x4_t*>(&vls[t & 1][(4 * i + (lane >> 4)) * (D * 2) + (lane & 15) * 16]));
+      }
+      bad = __any(bad);
+      if (bad) {
+        pf_add_nonfinite(o, ps[pr][t & 1], sp.v, sp.v_bytes, t * kPairK, sp.nk, qp, sp.before, x, g,
+                         [](int e, int row) { return 32 * e + 8 * ((row >> 2) & 3) + 4 * (row >> 4) + (row & 3); });
+      }
+    }
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -958,7 +1175,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + vlane[e] + s * 16 * D * 2));
         const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + vlane[e] + (s * 16 + 8) * D * 2));
         const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
-        const u32x4_t vop = {l2[0], l2[1], h2[0], h2[1]};
+        u32x4_t vop = {l2[0], l2[1], h2[0], h2[1]};
+        if (kPacked && bad) vop = pf_finite(vop);
 #pragma unroll
         for (int u = 0; u < 2; ++u) o[u][e] = mfma32(vop, p[u][s], o[u][e]);
       }
@@ -973,10 +1191,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int query = qp + 32 * u + x;
-    if (query >= a.width) continue;
-    const float l = lsum[pr][0][32 * u + x] + lsum[pr][1][32 * u + x];
+    if (query >= sp.nq) continue;
+    const float l = kPacked && dq < 0 ? 0.f : lsum[pr][0][32 * u + x] + lsum[pr][1][32 * u + x];
     const float inv = l > 0.f ? 1.f / l : 1.f;
-    uint16_t* orow = a.out + ((int64_t)(b * a.width + query) * a.H + h) * D + 8 * g;
+    uint16_t* orow = a.out + ((sp.q0 + query) * a.H + h) * D + 8 * g;
     auto pair = [&](float lo, float hi) {
       return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
     };
@@ -1255,7 +1473,7 @@ extern "C" int omni_prefill_attention(const void* q, const void* k_cache, const 
       omni::prefill_attn_kernel<<<grid, omni::kPfThreads, 0, s>>>(a);
     } else {
       dim3 grid((width + omni::kPairQ - 1) / omni::kPairQ, heads, contexts);
-      omni::prefill_attn_pairs_kernel<<<grid, 512, 0, s>>>(a);
+      omni::prefill_attn_pairs_kernel<false><<<grid, 512, 0, s>>>(a);
     }
   } else if (head_dim == 512) {
     const int nqb = (width + omni::kWsQ - 1) / omni::kWsQ, units = heads * contexts;
@@ -1263,14 +1481,68 @@ extern "C" int omni_prefill_attention(const void* q, const void* k_cache, const 
     a.units8 = units / 8;
     a.group = units % 8 == 0 ? omni::ws_group(nqb, a.units8) : 0;
     if (a.group) {
-      omni::prefill_attn_ws_kernel<true><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);
+      omni::prefill_attn_ws_kernel<true, false><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);
     } else {
-      omni::prefill_attn_ws_kernel<false><<<grid, 512, 0, s>>>(a);
+      omni::prefill_attn_ws_kernel<false, false><<<grid, 512, 0, s>>>(a);
     }
   } else {
     const int qw = 16 * omni::kPwSub * (omni::kPwWaves / 2);  // queries per workgroup
     dim3 grid((width + qw - 1) / qw, heads, contexts);
-    omni::prefill_attn_wide_kernel<<<grid, 64 * omni::kPwWaves, 0, s>>>(a);
+    omni::prefill_attn_wide_kernel<false><<<grid, 64 * omni::kPwWaves, 0, s>>>(a);
+  }
+  return omni_launch_status();
+}
+
+extern "C" int omni_packed_attention(const void* q, const void* k, const void* v, int64_t k_stride_pos,
+                                     int64_t k_stride_head, int64_t v_stride_pos, int64_t v_stride_head,
+                                     const int64_t* starts, const int64_t* k_starts, int32_t sequences,
+                                     int64_t queries, int64_t keys, int32_t longest, int32_t heads, int32_t kv_heads,
+                                     int32_t head_dim, float scale, void* out, int32_t dtype, void* stream) {
+  if (dtype != OMNI_BF16) return OMNI_ERR_DTYPE;
+  if (sequences < 0 || queries < 0 || keys < 0 || longest < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads)
+    return OMNI_ERR_INVALID;
+  if (head_dim != 128 && head_dim != 256 && head_dim != 512) return OMNI_ERR_SHAPE;
+  if (!(scale > 0.f) || scale == INFINITY) return OMNI_ERR_INVALID;
+  if (sequences == 0 || queries == 0 || longest == 0) return OMNI_OK;
+  if (!q || !starts || !k_starts || !out || (keys > 0 && (!k || !v))) return OMNI_ERR_INVALID;
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v) & 15u) return OMNI_ERR_INVALID;
+  if ((k_stride_pos | k_stride_head | v_stride_pos | v_stride_head) & 7) return OMNI_ERR_INVALID;
+  if (k_stride_pos < 0 || k_stride_head < 0 || v_stride_pos < 0 || v_stride_head < 0) return OMNI_ERR_INVALID;
+  if (sequences > 65535 || heads > 65535) return OMNI_ERR_SHAPE;
+  // A tile's 64 rows are addressed by 32-bit byte offsets; a sequence's keys are counted in 31 bits.
+  if (k_stride_pos >= (1 << 24) || v_stride_pos >= (1 << 24) || keys > 0x7fffff00LL || queries > 0x7fffff00LL)
+    return OMNI_ERR_SHAPE;
+  omni::PrefillArgs a;
+  a.q = (const uint16_t*)q;
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.slots = nullptr;
+  a.s_row = a.s_head = a.cache_rows = 0;
+  a.width = longest;
+  a.H = heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = (uint16_t*)out;
+  a.units8 = a.group = 0;
+  a.starts = starts;
+  a.k_starts = k_starts;
+  a.queries = queries;
+  a.keys = keys;
+  a.k_pos = k_stride_pos;
+  a.k_head = k_stride_head;
+  a.v_pos = v_stride_pos;
+  a.v_head = v_stride_head;
+  a.heads_per_kv = heads / kv_heads;
+  const hipStream_t s = (hipStream_t)stream;
+  if (head_dim == 128) {
+    const dim3 grid((longest + omni::kPairQ - 1) / omni::kPairQ, heads, sequences);
+    omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
+  } else if (head_dim == 512) {
+    const dim3 grid((longest + omni::kWsQ - 1) / omni::kWsQ, heads, sequences);
+    omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
+  } else {
+    const int qw = 16 * omni::kPwSub * (omni::kPwWaves / 2);  // queries per workgroup
+    const dim3 grid((longest + qw - 1) / qw, heads, sequences);
+    omni::prefill_attn_wide_kernel<true><<<grid, 64 * omni::kPwWaves, 0, s>>>(a);
   }
   return omni_launch_status();
 }
