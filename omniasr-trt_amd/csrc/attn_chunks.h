@@ -18,48 +18,29 @@ struct KvChunk {
   u32x4_t r[kF8 ? 4 : 8];
 };
 
-// K: bf16 row mb at r[4 mb + s], dimensions 32s + 8g ..; e4m3 at r[2 mb + p], dimensions 64p + 16g ...
-template <bool kF8>
-__device__ __forceinline__ void load_k_chunk(KvChunk<kF8>& t, const char* row0, const char* row1, int ch, int g) {
-  if constexpr (kF8) {
+// K: bf16 row mb at r[4 mb + s], dimensions 32s + 8g ..; e4m3 at r[2 mb + p], dimensions 64p + 16g ...  ``row``: row
+// c % 4 of the lane's 8 keys, 16g bytes on; rows are kRowB bytes apart.
+template <bool kF8, int kRowB>
+__device__ __forceinline__ void load_k_chunk(KvChunk<kF8>& t, const char* row, int ch) {
+  constexpr int kSteps = kF8 ? 2 : 4;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      t.r[p] = ld16(row0 + ch * 128 + 64 * p + g * 16);
-      t.r[2 + p] = ld16(row1 + ch * 128 + 64 * p + g * 16);
-    }
-  } else {
+  for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      t.r[s] = ld16(row0 + ch * 256 + 64 * s + g * 16);
-      t.r[4 + s] = ld16(row1 + ch * 256 + 64 * s + g * 16);
-    }
-  }
+    for (int s = 0; s < kSteps; ++s) t.r[kSteps * mb + s] = ld16(row + 4 * mb * kRowB + ch * 64 * kSteps + 64 * s);
 }
 
-// V row j: dimensions 8c .. + 7 of the chunk; rows past ``last`` (of the 8) as row ``last``.  ``row_bytes``: between rows.
-template <bool kF8>
-__device__ __forceinline__ void load_v_chunk(KvChunk<kF8>& t, const char* rows, int64_t row_bytes, int last, int ch,
-                                             int c) {
+// V row j: dimensions 8c .. + 7 of the chunk.  ``row``: the first of the lane's 8 keys, at its dimensions.
+template <bool kF8, int kRowB>
+__device__ __forceinline__ void load_v_chunk(KvChunk<kF8>& t, const char* row, int ch) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const char* row = rows + (j < last ? j : last) * row_bytes;
     if constexpr (kF8) {
-      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(row + ch * 128 + c * 8);
+      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(row + j * kRowB + ch * 128);
       t.r[j >> 1][2 * (j & 1)] = w[0];
       t.r[j >> 1][2 * (j & 1) + 1] = w[1];
     } else {
-      t.r[j] = ld16(row + ch * 256 + c * 16);
+      t.r[j] = ld16(row + j * kRowB + ch * 256);
     }
-  }
-}
-
-// Query operands of a row of D elements for the scores of the chunks: in the dimensions' order of load_k_chunk.
-template <int D, bool kF8>
-__device__ __forceinline__ void load_q(u32x4_t (&q)[D / 32], const uint16_t* row, bool live, int g) {
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const int at = kF8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
-    q[i] = live ? *reinterpret_cast<const u32x4_t*>(row + at) : u32x4_t{0u, 0u, 0u, 0u};
   }
 }
 
@@ -83,16 +64,16 @@ __device__ __forceinline__ void chunk_scores(const KvChunk<kF8>& t, const u32x4_
     }
 }
 
-// The softmax step of a tile: lane (c, g) holds query c's raw scores of keys key0 + j (key0 this lane's), seen below
-// ``lim``; probabilities relative to the lazy reference maximum (see attend_scored).
+// The softmax step of a tile: lane (c, g) holds query c's raw scores of its 8 keys, of which it sees the first ``seen``;
+// probabilities relative to the lazy reference maximum (see attend_scored).
 template <int NB>
 __device__ __forceinline__ void tile_softmax(const f32x4_t (&acc)[2], float c_scale, SoftmaxState& st, f32x4_t (&o)[NB],
-                                             int g, int64_t key0, int64_t lim, float (&p)[8]) {
+                                             int g, int seen, float (&p)[8]) {
   float sv[8];
   bool over = false;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    sv[j] = key0 + j < lim ? acc[j >> 2][j & 3] : -INFINITY;
+    sv[j] = j < seen ? acc[j >> 2][j & 3] : -INFINITY;
     over |= sv[j] > st.thr;
   }
   if (__any(over)) {
@@ -114,19 +95,34 @@ __device__ __forceinline__ void tile_softmax(const f32x4_t (&acc)[2], float c_sc
   }
 }
 
-__device__ __forceinline__ bool has_nonfinite(u32x4_t w) {
-  bool bad = false;
+// A chunk of V on a tile with keys that some query does not see: their probability is 0, but 0 times an infinity or NaN of
+// V would reach the query's output, so the products run without those.  True where the lane's part held any: the caller
+// adds them to the queries that see them, whose output they make infinite or NaN whatever their weight.
+template <bool kF8>
+__device__ __forceinline__ bool only_finite(KvChunk<kF8>& t) {
+  // An exponent of ones (e4m3: exponent and mantissa) carries into the sign's place.
+  constexpr uint32_t kField = kF8 ? 0x7f7f7f7fu : 0x7f807f80u, kOne = kF8 ? 0x01010101u : 0x00800080u;
+  constexpr uint32_t kTop = kF8 ? 0x80808080u : 0x80008000u;
+  uint32_t any = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
-  return bad;
+  for (int i = 0; i < (kF8 ? 4 : 8); ++i)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) any |= (t.r[i][w] & kField) + kOne;
+  if (!__any((any & kTop) != 0)) return false;
+#pragma unroll
+  for (int i = 0; i < (kF8 ? 4 : 8); ++i)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t top = ((t.r[i][w] & kField) + kOne) & kTop;
+      t.r[i][w] &= ~((top << 1) - (top >> (kF8 ? 7 : 15)));  // every bit of such an element
+    }
+  return true;
 }
 
-// O += P V for a chunk: ``o`` [8], block e column c is dimension 8c + e.  ``edge`` (wave-uniform): some query does not see
-// some key of the tile.  Its probability there is 0, but 0 times an infinity or NaN would reach its output, so V rows that
-// hold one are left out of the product and added to the queries that see them one by one.
+// O += P V for a chunk: ``o`` [8], block e column c is dimension 8c + e.
 template <bool kF8>
 __device__ __forceinline__ void chunk_values(const KvChunk<kF8>& t, const float (&p)[8], const float (&scale)[8],
-                                             f32x4_t* o, bool edge, int64_t key0, int64_t lim, int c, int g) {
+                                             f32x4_t* o) {
   u32x4_t v[8], pop;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -139,29 +135,6 @@ __device__ __forceinline__ void chunk_values(const KvChunk<kF8>& t, const float 
 #pragma unroll
   for (int w = 0; w < 4; ++w)
     pop[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p[2 * w], p[2 * w + 1]}), bf16x2_t));
-  if (edge) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint64_t bad = __ballot(has_nonfinite(v[j]));
-      if (!bad) continue;
-      const u32x4_t zero = {0u, 0u, 0u, 0u}, row = v[j];
-      for (int gk = 0; gk < 4; ++gk) {  // key 8 gk + j of the tile, in lanes 16 gk ..
-        if (!((bad >> (16 * gk)) & 0xffffu)) continue;
-        if (g == gk) v[j] = zero;
-        u32x4_t all;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) all[i] = (uint32_t)__shfl((int)row[i], 16 * gk + c, kWave);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int from = 16 * gk + 4 * g + i;  // the lane of query 4g + i and this key
-          const bool seen = __shfl((int)(key0 + j < lim), from, kWave);
-          const float w = round_through_bf16(__shfl(p[j], from, kWave));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e][i] += seen ? w * bf16x8_elem(all, e) : 0.f;
-        }
-      }
-    }
-  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     u32x4_t b;
