@@ -21,33 +21,33 @@ struct KvChunk {
 // K: bf16 row mb at r[4 mb + s], dimensions 32s + 8g ..; e4m3 at r[2 mb + p], dimensions 64p + 16g ...  ``row``: row
 // c % 4 of the lane's 8 keys, 16g bytes on; rows are kRowB bytes apart.
 template <bool kF8, int kRowB>
-__device__ __forceinline__ void load_k_chunk(KvChunk<kF8>& t, const char* row, int ch) {
+__device__ __forceinline__ void load_k_chunk(KvChunk<kF8>& t, const char* row) {
   constexpr int kSteps = kF8 ? 2 : 4;
 #pragma unroll
   for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) t.r[kSteps * mb + s] = ld16(row + 4 * mb * kRowB + ch * 64 * kSteps + 64 * s);
+    for (int s = 0; s < kSteps; ++s) t.r[kSteps * mb + s] = ld16(row + 4 * mb * kRowB + 64 * s);
 }
 
 // V row j: dimensions 8c .. + 7 of the chunk.  ``row``: the first of the lane's 8 keys, at its dimensions.
 template <bool kF8, int kRowB>
-__device__ __forceinline__ void load_v_chunk(KvChunk<kF8>& t, const char* row, int ch) {
+__device__ __forceinline__ void load_v_chunk(KvChunk<kF8>& t, const char* row) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if constexpr (kF8) {
-      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(row + j * kRowB + ch * 128);
+      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(row + j * kRowB);
       t.r[j >> 1][2 * (j & 1)] = w[0];
       t.r[j >> 1][2 * (j & 1) + 1] = w[1];
     } else {
-      t.r[j] = ld16(row + j * kRowB + ch * 256);
+      t.r[j] = ld16(row + j * kRowB);
     }
   }
 }
 
-// S^T += K_ch Q_ch^T (``scale``: of rows mb = 0, 1; e4m3 only).
-template <bool kF8>
-__device__ __forceinline__ void chunk_scores(const KvChunk<kF8>& t, const u32x4_t* q, const float (&scale)[2],
-                                             f32x4_t (&acc)[2]) {
+// S^T = K Q^T over a chunk for NB blocks of 16 queries (``scale``: of rows mb = 0, 1; e4m3 only).
+template <bool kF8, int NB>
+__device__ __forceinline__ void chunk_scores(const KvChunk<kF8>& t, const u32x4_t (&q)[NB][4], const float (&scale)[2],
+                                             f32x4_t (&acc)[NB][2]) {
 #pragma unroll
   for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -59,16 +59,19 @@ __device__ __forceinline__ void chunk_scores(const KvChunk<kF8>& t, const u32x4_
       } else {
         k = t.r[4 * mb + s];
       }
-      acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k),
-                                                        __builtin_bit_cast(bf16x8_t, q[s]), acc[mb], 0, 0, 0);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+        acc[nb][mb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, q[nb][s]),
+            s == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc[nb][mb], 0, 0, 0);
     }
 }
 
 // The softmax step of a tile: lane (c, g) holds query c's raw scores of its 8 keys, of which it sees the first ``seen``;
-// probabilities relative to the lazy reference maximum (see attend_scored).
+// returns their probabilities relative to the lazy reference maximum (see attend_scored) as the P operand.
 template <int NB>
-__device__ __forceinline__ void tile_softmax(const f32x4_t (&acc)[2], float c_scale, SoftmaxState& st, f32x4_t (&o)[NB],
-                                             int g, int seen, float (&p)[8]) {
+__device__ __forceinline__ u32x4_t tile_softmax(const f32x4_t (&acc)[2], float c_scale, SoftmaxState& st,
+                                                f32x4_t (&o)[NB], int g, int seen) {
   float sv[8];
   bool over = false;
 #pragma unroll
@@ -88,11 +91,17 @@ __device__ __forceinline__ void tile_softmax(const f32x4_t (&acc)[2], float c_sc
     st.thr = m_new == -INFINITY ? -INFINITY : (m_new + kLazyLog2) / c_scale;
   }
   const float m_use = st.m_ref == -INFINITY ? 0.f : st.m_ref;
+  float p[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[j], c_scale, -m_use));
     st.l_run += p[j];
   }
+  u32x4_t pop;
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    pop[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p[2 * w], p[2 * w + 1]}), bf16x2_t));
+  return pop;
 }
 
 // A chunk of V on a tile with keys that some query does not see: their probability is 0, but 0 times an infinity or NaN of
@@ -119,11 +128,11 @@ __device__ __forceinline__ bool only_finite(KvChunk<kF8>& t) {
   return true;
 }
 
-// O += P V for a chunk: ``o`` [8], block e column c is dimension 8c + e.
-template <bool kF8>
-__device__ __forceinline__ void chunk_values(const KvChunk<kF8>& t, const float (&p)[8], const float (&scale)[8],
-                                             f32x4_t* o) {
-  u32x4_t v[8], pop;
+// O += P V over a chunk for NB blocks of 16 queries: block e of o, column c is dimension 8c + e.
+template <bool kF8, int NB>
+__device__ __forceinline__ void chunk_values(const KvChunk<kF8>& t, const u32x4_t (&pop)[NB], const float (&scale)[8],
+                                             f32x4_t (&o)[NB][8]) {
+  u32x4_t v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if constexpr (kF8) {
@@ -133,16 +142,15 @@ __device__ __forceinline__ void chunk_values(const KvChunk<kF8>& t, const float 
     }
   }
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
-    pop[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p[2 * w], p[2 * w + 1]}), bf16x2_t));
-#pragma unroll
   for (int e = 0; e < 8; ++e) {
     u32x4_t b;
 #pragma unroll
     for (int w = 0; w < 4; ++w)
       b[w] = __builtin_amdgcn_perm(v[2 * w + 1][e >> 1], v[2 * w][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
-    o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pop), __builtin_bit_cast(bf16x8_t, b),
-                                                   o[e], 0, 0, 0);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, pop[nb]),
+                                                         __builtin_bit_cast(bf16x8_t, b), o[nb][e], 0, 0, 0);
   }
 }
 

@@ -9,10 +9,11 @@
 // What bounds it is the HBM stream of the keys, so every CU is to stream the same share from start to end.  The 32-key
 // tiles of all units stand in one line (row after row, unit after unit), cut into equal shares, one for each workgroup of
 // four waves, whatever the rows' lengths: a share is the end of one unit, whole units, and the beginning of another.  A
-// unit's start counts as kPaStart more tiles, about what it costs.  A share's waves take a unit's tiles in turn, each with
-// the next tiles' loads in flight in registers, and join through LDS, while the loads of the share's next unit are already
-// on their way.  A unit within one share is written at once; of the others each share leaves (O, m, l) in fp32, and a second
-// launch joins them:  w_s = exp(m_s - max m), out = sum w_s O_s / sum w_s l_s.
+// unit's start counts as kPaStart more tiles, about what it costs.  A wave holds 128 dimensions, so the waves take a unit's
+// tiles in turn at head dim 128, in pairs at 256 and together at 512, where their partial scores are added through LDS;
+// each has the next tiles' loads in flight in registers.  A unit within one share is written at once; of the others each
+// share leaves (O, m, l) in fp32, and a second launch joins them:
+//   w_s = exp(m_s - max m), out = sum w_s O_s / sum w_s l_s.
 // All of it is found from the lengths on the device, so one launch shape serves every length (graphs), and results do not
 // depend on timing.
 #include <math.h>
@@ -31,16 +32,12 @@ struct PagedAttn {
   int rows, T, H, group, cols, qblocks;
   int units;  // of a row: kv heads x qblocks
   float scale_log2;
-  float* part_o;   // [2 * workgroups][16][D]: share w's unit begun before it at 2 w, its unit that goes on at 2 w + 1
-  float* part_ml;  // [2 * workgroups][16][2]
+  float* part_o;   // [2 * workgroups][16 NB][D]: share w's unit begun before it at 2 w, its unit that goes on at 2 w + 1
+  float* part_ml;  // [2 * workgroups][16 NB][2]
   uint16_t* out;   // [rows * T, H, D]
 };
 
-// Workgroups that run at once on 256 CUs: what the registers allow, a power of two.
-template <int D>
-constexpr int paged_slots_log2() {
-  return D == 512 ? 8 : 9;
-}
+constexpr int kPaSlots = 512;  // workgroups that run at once: two on each of 256 CUs
 
 // Keys that the row's first and last query see.
 struct PagedReach {
@@ -66,13 +63,17 @@ __device__ __forceinline__ int wave_scan(int v) {
 // The line: 64 rows at a time in the lanes of a wave, lane's row with ``tiles`` for each of its units, after ``before``
 // places of the rows ahead of it.
 struct PagedLine {
-  int b0, tiles, before;
+  int b0, n, tiles, before;
   __device__ int places() const { return tiles > 0 ? tiles + kPaStart : 0; }  // of a unit
   // Rows b0 .. b0 + 63, the first after ``ahead`` places; returns the places up to their end.
   __device__ int take(const PagedAttn& a, int lane, int first, int ahead) {
     b0 = first;
-    const int b = first + lane;
-    tiles = b < a.rows ? (paged_reach(a, b).last + 31) >> 5 : 0;
+    n = tiles = 0;
+    if (first + lane < a.rows) {
+      const PagedReach r = paged_reach(a, first + lane);
+      n = r.first;
+      tiles = (r.last + 31) >> 5;
+    }
     const int mine = places() * a.units, sum = wave_scan(mine);
     before = ahead + sum - mine;
     return ahead + __builtin_amdgcn_readlane(sum, kWave - 1);
@@ -86,15 +87,12 @@ __device__ __forceinline__ int paged_total(const PagedAttn& a, int lane, PagedLi
   return total;
 }
 
-// Places of a share: an even part of all for each workgroup, at least two tiles for each wave.
-template <int D>
-__device__ __forceinline__ int paged_share(int total) {
-  return max((total + (1 << paged_slots_log2<D>()) - 1) >> paged_slots_log2<D>(), 2 * kPaWaves);
-}
+// Places of a share: an even part of all for each workgroup, but not so few that its start outweighs them.
+__device__ __forceinline__ int paged_share(int total) { return max((total + kPaSlots - 1) / kPaSlots, kPaStart + 2); }
 
 // A unit, and where its tiles are in the line: [from, from + tiles).
 struct PagedUnit {
-  int b, unit, tiles, from;
+  int b, n, unit, tiles, from;
 };
 
 // The unit that holds place ``x`` (in its start or its tiles).
@@ -107,6 +105,7 @@ __device__ __forceinline__ PagedUnit paged_find(const PagedAttn& a, int lane, Pa
       const int l = __builtin_ctzll(hit);
       PagedUnit u;
       u.b = line.b0 + l;
+      u.n = __builtin_amdgcn_readlane(line.n, l);
       u.tiles = __builtin_amdgcn_readlane(line.tiles, l);
       const int start = __builtin_amdgcn_readlane(line.before, l), places = u.tiles + kPaStart;
       u.unit = (int)((uint32_t)(x - start) / (uint32_t)places);
@@ -117,16 +116,16 @@ __device__ __forceinline__ PagedUnit paged_find(const PagedAttn& a, int lane, Pa
   }
 }
 
-// Tiles ahead that a wave's loads run: what fits its registers beside the accumulators.
-template <int D, bool kF8>
+// Tiles ahead that a wave's loads run: what its registers hold beside the accumulators.
+template <bool kF8, int NB>
 constexpr int paged_ahead() {
-  return D == 128 ? 2 : 1;
+  return NB <= (kF8 ? 2 : 1) ? 2 : 1;
 }
 
-// What a lane holds of a tile: K, V and, e4m3, exponent bytes (V's for its 8 keys).
-template <int D, bool kF8>
+// What a lane holds of a tile's 128 dimensions: K, V and, e4m3, exponent bytes (V's for its 8 keys).
+template <bool kF8>
 struct PagedTile {
-  KvChunk<kF8> k[D / 128], v[D / 128];
+  KvChunk<kF8> k, v;
   uint32_t ks[2];
   u32x2_t vs;
 };
@@ -138,50 +137,49 @@ __device__ __forceinline__ int afresh(int v) {
   return v;
 }
 
-// A share's part of a unit: tiles t0 .. t1 - 1, of which this wave takes first, first + kPaWaves, ...
+// A share's part of a unit: tiles t0 .. t1 - 1, of which this wave takes ``mine``: first, first + step, ...
 struct PagedPiece {
   PagedUnit u;
-  PagedReach reach;
+  int last;  // keys that the row's last query sees (u.n: its first)
   int t0, t1, head, qblk, first, mine;
   const int32_t* table;
-  __device__ int nth(int i) const { return first + kPaWaves * min(i, mine - 1); }
 };
 
-template <int D, bool kF8>
-__global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(D == 512 ? 1 : 2))) void
-paged_attn_kernel(PagedAttn a) {
-  constexpr int kChunks = D / 128, kRowB = D * (kF8 ? 1 : 2), kAhead = paged_ahead<D, kF8>();
+// NB: blocks of 16 query columns that share a read of the keys.
+template <int D, bool kF8, int NB>
+__global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2))) void paged_attn_kernel(PagedAttn a) {
+  constexpr int kRowB = D * (kF8 ? 1 : 2), kAhead = paged_ahead<kF8, NB>();
+  constexpr int kSlices = D / 128, kStep = kPaWaves / kSlices;  // waves to a tile, tiles at a time
   constexpr int kQRow = D * 2 + 16;  // LDS bytes of a query, padded against bank conflicts
-  constexpr int kQPieces = 16 * (D / 8) / (64 * kPaWaves);  // of 16 bytes, of the block's queries, for a thread
-  __shared__ __attribute__((aligned(16))) char qs[16 * kQRow];
-  __shared__ __attribute__((aligned(16))) float os[kPaWaves][16][D];
-  __shared__ float mls[kPaWaves][16][2];
+  constexpr int kQPieces = 16 * NB * (D / 8) / (64 * kPaWaves);  // of 16 bytes, of the blocks' queries, for a thread
+  __shared__ __attribute__((aligned(16))) char qs[16 * NB * kQRow];
+  __shared__ f32x4_t parts[kSlices > 1 ? 2 : 1][kSlices > 1 ? kPaWaves : 1][NB][2][64];  // scores by tile parity and wave
+  __shared__ __attribute__((aligned(16))) float os[kStep > 1 ? kStep : 1][kStep > 1 ? 16 : 1][D];
+  __shared__ float mls[kPaWaves][16 * NB][2];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), sl = w % kSlices, stream = w / kSlices;
 
   PagedLine line;
-  const int total = paged_total(a, lane, line), share = paged_share<D>(total);
+  const int total = paged_total(a, lane, line), share = paged_share(total);
   int x = blockIdx.x * share;
   if (x >= total) return;
   const int x_end = min(x + share, total);
 
   // The next piece from place x on, false if there is none.
   auto next = [&](PagedPiece& p) {
-    while (x < x_end) {
-      p.u = paged_find(a, lane, line, x);
-      p.t0 = max(x - p.u.from, 0);
-      p.t1 = min(x_end - p.u.from, p.u.tiles);
-      x = p.u.from + p.u.tiles;
-      if (p.t1 <= p.t0) return false;  // only the start of a unit whose tiles are the next share's
-      p.head = p.u.unit / a.qblocks;
-      p.qblk = p.u.unit - p.head * a.qblocks;
-      p.reach = paged_reach(a, p.u.b);
-      p.table = a.cache.table + p.u.b * a.cache.table_stride;
-      p.first = p.t0 + w;
-      p.mine = p.first < p.t1 ? (p.t1 - p.first + kPaWaves - 1) / kPaWaves : 0;
-      return true;
-    }
-    return false;
+    if (x >= x_end) return false;
+    p.u = paged_find(a, lane, line, x);
+    p.t0 = max(x - p.u.from, 0);
+    p.t1 = min(x_end - p.u.from, p.u.tiles);
+    x = p.u.from + p.u.tiles;
+    if (p.t1 <= p.t0) return false;  // only the start of a unit whose tiles are the next share's
+    p.head = (int)((uint32_t)p.u.unit / (uint32_t)a.qblocks);
+    p.qblk = p.u.unit - p.head * a.qblocks;
+    p.last = (int)min((int64_t)p.u.n + a.T - 1, a.cache.positions);
+    p.table = a.cache.table + p.u.b * a.cache.table_stride;
+    p.first = p.t0 + stream;
+    p.mine = p.first < p.t1 ? (p.t1 - p.first + kStep - 1) / kStep : 0;
+    return true;
   };
   // 8 keys in a row are on one page.  Groups of 8 past the one with the last key are read as it; keys behind the last one
   // are read where they share its group, and masked like those a query does not see.  A page number out of the pool is
@@ -189,207 +187,249 @@ paged_attn_kernel(PagedAttn a) {
   struct Pages {
     int k, v;
   };
-  auto group_of = [&](const PagedPiece& p, int t, int eighth) { return min(t * 4 + eighth, (p.reach.last - 1) >> 3); };
+  auto group_of = [&](const PagedPiece& p, int i, int eighth) {
+    return min((p.first + kStep * i) * 4 + eighth, (p.last - 1) >> 3);
+  };
   auto page_of = [&](const PagedPiece& p, int group) { return p.table[(group * 8) >> a.cache.page_log2]; };
   auto cell = [&](const PagedPiece& p, int group, int page) {
     const int64_t held = min(max(page, 0), a.cache.pages - 1);
     return ((held * a.cache.kv + p.head) << a.cache.page_log2) + ((group * 8) & ((1 << a.cache.page_log2) - 1));
   };
   auto look = [&](const PagedPiece& p, int i) {
-    const int t = p.nth(i);
-    return Pages{page_of(p, group_of(p, t, c >> 2)), page_of(p, group_of(p, t, g))};
+    return Pages{page_of(p, group_of(p, i, c >> 2)), page_of(p, group_of(p, i, g))};
   };
-  PagedTile<D, kF8> tile[kAhead];
+  PagedTile<kF8> tile[kAhead];
   Pages pages;  // of the next tile to be loaded
-  // Loads of the wave's tile i: K with its exponents at once, V's chunks one by one from ``vrow``.  Loads past the wave's
-  // last tile are made all the same, of one line for all lanes, and not used: without a branch around them no wait has to
-  // cover the case that they were not made.
-  auto load_k = [&](PagedTile<D, kF8>& t, const PagedPiece& p, int i, Pages at, const char*& vrow, u32x2_t& vs) {
-    const int n = p.nth(i);
-    const int64_t kc = cell(p, group_of(p, n, c >> 2), at.k) + (c & 3), vc = cell(p, group_of(p, n, g), at.v);
+  // Loads of the wave's tile i: K with its exponents at once, V from ``vrow``.  Loads past the wave's last tile are made all
+  // the same, of one line for all lanes, and not used: without a branch around them no wait has to cover the case that they
+  // were not made.
+  auto load_k = [&](PagedTile<kF8>& t, const PagedPiece& p, int i, Pages at, const char*& vrow, u32x2_t& vs) {
+    const int64_t kc = cell(p, group_of(p, i, c >> 2), at.k) + (c & 3), vc = cell(p, group_of(p, i, g), at.v);
     if constexpr (kF8) {
       t.ks[0] = a.cache.k_scale[kc];
       t.ks[1] = a.cache.k_scale[kc + 4];
       vs = *reinterpret_cast<const u32x2_t*>(a.cache.v_scale + vc);
     }
-    vrow = i < p.mine ? a.cache.v + vc * kRowB + c * (kF8 ? 8 : 16) : a.cache.v;
-    const char* krow = i < p.mine ? a.cache.k + kc * kRowB + g * 16 : a.cache.k;
-#pragma unroll
-    for (int ch = 0; ch < kChunks; ++ch) load_k_chunk<kF8, kRowB>(t.k[ch], krow, ch);
-  };
-  // A piece's queries (0 past the last column) and first tiles on their way; the queries to LDS when they have come.
-  u32x4_t qv[kQPieces];
-  auto begin = [&](const PagedPiece& p) {
-    const int t = afresh(tid);
-#pragma unroll
-    for (int k = 0; k < kQPieces; ++k) {
-      const int i = t + k * 64 * kPaWaves, cc = 16 * p.qblk + i / (D / 8), e = i % (D / 8) * 8;
-      const int held = min(cc, a.cols - 1);
-      qv[k] = *reinterpret_cast<const u32x4_t*>(
-          a.q + (((int64_t)p.u.b * a.T + held / a.group) * a.H + p.head * a.group + held % a.group) * D + e);
-      if (cc != held) qv[k] = u32x4_t{0u, 0u, 0u, 0u};
-    }
-    if (p.mine == 0) return;
-    Pages at[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) at[i] = look(p, i);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const char* vrow;
-      load_k(tile[i], p, i, at[i], vrow, tile[i].vs);
-#pragma unroll
-      for (int ch = 0; ch < kChunks; ++ch) load_v_chunk<kF8, kRowB>(tile[i].v[ch], vrow, ch);
-    }
-    pages = look(p, kAhead);
+    constexpr int kSliceB = 128 * (kF8 ? 1 : 2);
+    vrow = i < p.mine ? a.cache.v + vc * kRowB + sl * kSliceB + c * (kF8 ? 8 : 16) : a.cache.v;
+    load_k_chunk<kF8, kRowB>(t.k, i < p.mine ? a.cache.k + kc * kRowB + sl * kSliceB + g * 16 : a.cache.k);
   };
 
   PagedPiece p;
   while (next(p)) {
-    begin(p);
-    const int tq = afresh(tid);
+    // The blocks' queries (0 past the last column) and the first tiles on their way; the queries to LDS.
+    {
+      const int t = afresh(tid);
+      u32x4_t qv[kQPieces];
 #pragma unroll
-    for (int k = 0; k < kQPieces; ++k) {
-      const int i = tq + k * 64 * kPaWaves;
-      *reinterpret_cast<u32x4_t*>(&qs[i / (D / 8) * kQRow + i % (D / 8) * 16]) = qv[k];
+      for (int k = 0; k < kQPieces; ++k) {
+        const int i = t + k * 64 * kPaWaves, col = 16 * NB * p.qblk + i / (D / 8), e = i % (D / 8) * 8;
+        const int held = min(col, a.cols - 1), token = (int)((uint32_t)held / (uint32_t)a.group);
+        qv[k] = *reinterpret_cast<const u32x4_t*>(
+            a.q + (((int64_t)p.u.b * a.T + token) * a.H + p.head * a.group + held - token * a.group) * D + e);
+        if (col != held) qv[k] = u32x4_t{0u, 0u, 0u, 0u};
+      }
+      Pages at[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) at[i] = look(p, i);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const char* vrow;
+        load_k(tile[i], p, i, at[i], vrow, tile[i].vs);
+        load_v_chunk<kF8, kRowB>(tile[i].v, vrow);
+      }
+      pages = look(p, kAhead);
+#pragma unroll
+      for (int k = 0; k < kQPieces; ++k) {
+        const int i = t + k * 64 * kPaWaves;
+        *reinterpret_cast<u32x4_t*>(&qs[i / (D / 8) * kQRow + i % (D / 8) * 16]) = qv[k];
+      }
     }
     lds_barrier();
-    const int col = 16 * p.qblk + c;
-    const int lim = col < a.cols ? min(p.reach.first + col / a.group, p.reach.last) : 0;
-    f32x4_t o[D / 16];
+    int lim[NB];  // keys that the lane's query columns see
+    f32x4_t o[NB][8];
+    SoftmaxState st[NB];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    SoftmaxState st{-INFINITY, -INFINITY, 0.f};
+    for (int nb = 0; nb < NB; ++nb) {
+      const int col = 16 * (NB * p.qblk + nb) + c;
+      lim[nb] = col < a.cols ? min(p.u.n + (int)((uint32_t)col / (uint32_t)a.group), p.last) : 0;
+      st[nb] = SoftmaxState{-INFINITY, -INFINITY, 0.f};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[nb][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
     bool bad = false;
     // The wave's tile i, and the loads of tile i + kAhead into its registers as they fall free.
-    auto attend = [&](PagedTile<D, kF8>& t, int i) __attribute__((always_inline)) {
-      float kscale[2] = {1.f, 1.f}, vscale[8];
-      if constexpr (kF8) {
-        kscale[0] = scale_of(t.ks[0]);
-        kscale[1] = scale_of(t.ks[1]);
+    auto attend = [&](PagedTile<kF8>& t, int i) __attribute__((always_inline)) {
+      f32x4_t acc[NB][2];
+      {
+        const float kscale[2] = {scale_of(t.ks[0]), scale_of(t.ks[1])};
+        u32x4_t q[NB][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vscale[j] = scale_of((t.vs[j >> 2] >> (8 * (j & 3))) & 0xffu);
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            q[nb][s] = *reinterpret_cast<const u32x4_t*>(
+                &qs[(16 * nb + c) * kQRow + sl * 256 + (kF8 ? 128 * (s >> 1) + 32 * g + 16 * (s & 1) : 64 * s + 16 * g)]);
+        chunk_scores<kF8, NB>(t.k, q, kscale, acc);
       }
-      f32x4_t acc[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-      for (int ch = 0; ch < kChunks; ++ch) {
-        u32x4_t q[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          q[s] = *reinterpret_cast<const u32x4_t*>(
-              &qs[c * kQRow + ch * 256 + (kF8 ? 128 * (s >> 1) + 32 * g + 16 * (s & 1) : 64 * s + 16 * g)]);
-        chunk_scores<kF8>(t.k[ch], q, kscale, acc);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      __builtin_amdgcn_sched_barrier(0);
       const char* vrow;
       u32x2_t vs;
       load_k(t, p, i + kAhead, pages, vrow, vs);
       pages = look(p, i + kAhead + 1);
       __builtin_amdgcn_sched_barrier(0);
-      float pr[8];
-      const int at = p.nth(i) * 32;
-      tile_softmax<D / 16>(acc, a.scale_log2, st, o, g, lim - at - 8 * g, pr);
-      // Only the wave's last tile of the unit can hold keys that a query does not see: T <= 16 such keys and the end of a
-      // tile lie within two tiles, of two waves.  (Columns that are no query's see none.)
-      if (at + 31 >= p.reach.first) {
+      if constexpr (kSlices > 1) {
 #pragma unroll
-        for (int ch = 0; ch < kChunks; ++ch) bad |= only_finite<kF8>(t.v[ch]);
-      }
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int ch = 0; ch < kChunks; ++ch) {
-        chunk_values<kF8>(t.v[ch], pr, vscale, o + 8 * ch);
-        load_v_chunk<kF8, kRowB>(t.v[ch], vrow, ch);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int mb = 0; mb < 2; ++mb) parts[i & 1][w][nb][mb][lane] = acc[nb][mb];
+        lds_barrier();
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb) {
+            acc[nb][mb] = parts[i & 1][w - sl][nb][mb][lane];  // the slices in one order in every wave
+#pragma unroll
+            for (int s = 1; s < kSlices; ++s) acc[nb][mb] += parts[i & 1][w - sl + s][nb][mb][lane];
+          }
       }
+      if (i < p.mine) {
+        const int at = (p.first + kStep * i) * 32;
+        float vscale[8];
+        u32x4_t pop[NB];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vscale[j] = scale_of((t.vs[j >> 2] >> (8 * (j & 3))) & 0xffu);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          pop[nb] = tile_softmax<8>(acc[nb], a.scale_log2, st[nb], o[nb], g, lim[nb] - at - 8 * g);
+        // Only the wave's last tile of the unit can hold keys that a query does not see where the waves' tiles are kStep
+        // apart, its last two otherwise: such keys are the last T - 1 <= 15 and the end of the last tile.
+        if (at + 31 >= p.u.n) bad |= only_finite<kF8>(t.v);
+        chunk_values<kF8, NB>(t.v, pop, vscale, o);
+      }
+      load_v_chunk<kF8, kRowB>(t.v, vrow);
       t.vs = vs;
+      __builtin_amdgcn_sched_barrier(0);
     };
-    if (p.mine > 0) {
+    // The waves of a tile, and those beside them, meet at its barrier: as many rounds for all.
+    const int rounds = kSlices > 1 ? (p.t1 - p.t0 + kStep - 1) / kStep : p.mine;
+    if (rounds > 0) {
       for (int i = 0;;) {
         attend(tile[0], i);
-        if (++i == p.mine) break;
+        if (++i == rounds) break;
         if constexpr (kAhead == 2) {
           attend(tile[1], i);
-          if (++i == p.mine) break;
+          if (++i == rounds) break;
         }
       }
     }
-    // ---- the four waves' parts, joined through LDS
+    if (__any(bad)) {  // infinities and NaN of V that the products of the last tiles left out
+      for (int i = max(p.mine - 2, 0); i < p.mine; ++i) {
+        const int at = (p.first + kStep * i) * 32;
+        if (at + 31 < p.u.n) continue;
+        for (int key = at; key < min(at + 32, p.last); ++key) {
+          const int64_t row = (cell(p, key >> 3, page_of(p, key >> 3)) + (key & 7)) * D + 128 * sl + 8 * c;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = kF8 ? ((a.cache.v[row + e] & 0x7f) == 0x7f ? NAN : 0.f)
+                                : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.cache.v)[row + e]);
+            if (v - v == 0.f) continue;  // finite
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int col = 16 * (NB * p.qblk + nb) + 4 * g + r;
+                if (col < a.cols && key < p.u.n + col / a.group) o[nb][e][r] += v;
+              }
+          }
+        }
+      }
+    }
+
+    // ---- the waves' parts: those of one slice joined through LDS
     const int tj = afresh(tid), cj = tj & 15, gj = (tj & 63) >> 4;
-    const float l = column_sum(st.l_run);
-    if (gj == 0) {
-      mls[w][cj][0] = st.m_ref;
-      mls[w][cj][1] = l;
-    }
-    const int live = min(a.cols - 16 * p.qblk, 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (4 * gj + i >= live) continue;
-#pragma unroll
-      for (int ch = 0; ch < kChunks; ++ch)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<f32x4_t*>(&os[w][4 * gj + i][128 * ch + 8 * cj + 4 * h]) = f32x4_t{
-              o[8 * ch + 4 * h][i], o[8 * ch + 4 * h + 1][i], o[8 * ch + 4 * h + 2][i], o[8 * ch + 4 * h + 3][i]};
-    }
-    if (__any(bad)) {  // infinities and NaN of V that the product of the wave's last tile left out
-      const int at = p.nth(p.mine - 1) * 32;
-      for (int key = at; key < min(at + 32, p.reach.last); ++key) {
-        const int64_t row = (cell(p, key >> 3, page_of(p, key >> 3)) + (key & 7)) * D;
-        for (int e = tj & 63; e < D; e += kWave) {
-          const float v = kF8 ? ((a.cache.v[row + e] & 0x7f) == 0x7f ? NAN : 0.f)
-                              : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.cache.v)[row + e]);
-          if (v - v == 0.f) continue;  // finite
-          for (int r = 0; r < live; ++r)
-            if (key < p.reach.first + (16 * p.qblk + r) / a.group) os[w][r][e] += v;
-        }
-      }
-    }
-    lds_barrier();
     const bool whole = p.t0 == 0 && p.t1 == p.u.tiles;
-    const int64_t slot = (2 * (int64_t)blockIdx.x + (p.t0 == 0 ? 1 : 0)) * 16;
-    for (int i = tj; i < live * (D / 8); i += 64 * kPaWaves) {
-      const int r = i / (D / 8), e = i % (D / 8) * 8;
-      float m = -INFINITY, ls = 0.f;
-      f32x4_t sum[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-      for (int s = 0; s < kPaWaves; ++s) m = fmaxf(m, mls[s][r][0]);
-#pragma unroll
-      for (int s = 0; s < kPaWaves; ++s) {
-        const float ms = mls[s][r][0];
-        const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-        ls += f * mls[s][r][1];
-        sum[0] += f * *reinterpret_cast<const f32x4_t*>(&os[s][r][e]);
-        sum[1] += f * *reinterpret_cast<const f32x4_t*>(&os[s][r][e + 4]);
-      }
+    const int64_t slot = (2 * (int64_t)blockIdx.x + (p.t0 == 0 ? 1 : 0)) * 16 * NB;
+    // 8 dimensions from ``e`` of the piece's column ``r`` (relative to m, weights' sum l), out or left for the second launch.
+    auto keep = [&](int r, int e, f32x4_t lo, f32x4_t hi, float m, float l) {
+      const int col = 16 * NB * p.qblk + r;
       if (whole) {
-        const int cc = 16 * p.qblk + r;
-        const float div = ls == 0.f ? 1.f : ls;
-        u32x4_t v;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = pack_bf16x2(sum[k >> 1][2 * (k & 1)] / div, sum[k >> 1][2 * (k & 1) + 1] / div);
+        const float div = l == 0.f ? 1.f : l;
+        const u32x4_t v = {pack_bf16x2(lo[0] / div, lo[1] / div), pack_bf16x2(lo[2] / div, lo[3] / div),
+                           pack_bf16x2(hi[0] / div, hi[1] / div), pack_bf16x2(hi[2] / div, hi[3] / div)};
+        const int token = (int)((uint32_t)col / (uint32_t)a.group);
         *reinterpret_cast<u32x4_t*>(
-            a.out + (((int64_t)p.u.b * a.T + cc / a.group) * a.H + p.head * a.group + cc % a.group) * D + e) = v;
+            a.out + (((int64_t)p.u.b * a.T + token) * a.H + p.head * a.group + col - token * a.group) * D + e) = v;
       } else {
         float* po = a.part_o + (slot + r) * D + e;
-        *reinterpret_cast<f32x4_t*>(po) = sum[0];
-        *reinterpret_cast<f32x4_t*>(po + 4) = sum[1];
+        *reinterpret_cast<f32x4_t*>(po) = lo;
+        *reinterpret_cast<f32x4_t*>(po + 4) = hi;
         if (e == 0) {
           a.part_ml[(slot + r) * 2] = m;
-          a.part_ml[(slot + r) * 2 + 1] = ls;
+          a.part_ml[(slot + r) * 2 + 1] = l;
+        }
+      }
+    };
+    const int live = min(a.cols - 16 * NB * p.qblk, 16 * NB);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float l = column_sum(st[nb].l_run);
+      if (16 * nb >= live) break;
+      if constexpr (kStep == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * gj + i;
+          const float mr = __shfl(st[nb].m_ref, r, kWave), lr = __shfl(l, r, kWave);
+          if (16 * nb + r >= live) continue;
+          keep(16 * nb + r, 128 * sl + 8 * cj, f32x4_t{o[nb][0][i], o[nb][1][i], o[nb][2][i], o[nb][3][i]},
+               f32x4_t{o[nb][4][i], o[nb][5][i], o[nb][6][i], o[nb][7][i]}, mr, lr);
+        }
+      } else {
+        if (nb > 0) lds_barrier();  // the block before has been read
+        if (gj == 0) {
+          mls[w][16 * nb + cj][0] = st[nb].m_ref;
+          mls[w][16 * nb + cj][1] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (16 * nb + 4 * gj + i >= live) continue;
+          float* row = &os[stream][4 * gj + i][128 * sl + 8 * cj];
+          *reinterpret_cast<f32x4_t*>(row) = f32x4_t{o[nb][0][i], o[nb][1][i], o[nb][2][i], o[nb][3][i]};
+          *reinterpret_cast<f32x4_t*>(row + 4) = f32x4_t{o[nb][4][i], o[nb][5][i], o[nb][6][i], o[nb][7][i]};
+        }
+        lds_barrier();
+        for (int i = tj; i < min(live - 16 * nb, 16) * (D / 8); i += 64 * kPaWaves) {
+          const int r = i / (D / 8), e = i % (D / 8) * 8;
+          float m = -INFINITY, ls = 0.f;
+          f32x4_t sum[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int s = 0; s < kStep; ++s) m = fmaxf(m, mls[s * kSlices][16 * nb + r][0]);
+#pragma unroll
+          for (int s = 0; s < kStep; ++s) {
+            const float ms = mls[s * kSlices][16 * nb + r][0];
+            const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+            ls += f * mls[s * kSlices][16 * nb + r][1];
+            sum[0] += f * *reinterpret_cast<const f32x4_t*>(&os[s][r][e]);
+            sum[1] += f * *reinterpret_cast<const f32x4_t*>(&os[s][r][e + 4]);
+          }
+          keep(16 * nb + r, e, sum[0], sum[1], m, ls);
         }
       }
     }
+    // The next piece's queries and scores go where this one's were read, and its parts where these were summed.
+    lds_barrier();
   }
 }
 
 // One workgroup per (query, head): its unit's parts joined where more than one share holds it, zeros where it has no tile.
 // Each wave takes every fourth part, several at a time, and the waves join through LDS.
-template <int D>
+template <int D, int NB>
 __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAttn a) {
   constexpr int kPer = D / 64, kBatch = 4;  // dimensions of a lane, parts in flight
   __shared__ float os[kPaWaves][D], ls[kPaWaves], ms[kPaWaves];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x, b = row / a.T, h = blockIdx.y;
-  const int col = (row - b * a.T) * a.group + h % a.group, unit = h / a.group * a.qblocks + col / 16;
+  const int col = (row - b * a.T) * a.group + h % a.group, unit = h / a.group * a.qblocks + col / (16 * NB);
   PagedLine line;
   int total = 0, tiles = 0, before = 0;
   for (int b0 = 0; b0 < a.rows; b0 += kWave) {
@@ -404,10 +444,10 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
     for (int e = threadIdx.x; e < D; e += 64 * kPaWaves) out[e] = 0;
     return;
   }
-  const uint32_t from = before + unit * (tiles + kPaStart) + kPaStart, share = paged_share<D>(total);
+  const uint32_t from = before + unit * (tiles + kPaStart) + kPaStart, share = paged_share(total);
   const int w0 = from / share, w1 = (from + tiles - 1) / share;
   if (w0 == w1) return;
-  auto slot = [&](int part) { return (2 * (int64_t)part + (part == w0 ? 1 : 0)) * 16 + col % 16; };
+  auto slot = [&](int part) { return (2 * (int64_t)part + (part == w0 ? 1 : 0)) * 16 * NB + col % (16 * NB); };
   float m = -INFINITY, l = 0.f, o[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) o[e] = 0.f;
@@ -467,26 +507,31 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
 }
 
 // Workgroups of a call: what runs at once, but none that a full table would leave without a share.
-inline int paged_workgroups(int64_t units, int64_t positions, int head_dim) {
-  const int64_t most = 1 << (head_dim == 512 ? paged_slots_log2<512>() : paged_slots_log2<128>());
-  const int64_t places = units * ((positions + 31) / 32 + kPaStart), want = (places + 2 * kPaWaves - 1) / (2 * kPaWaves);
-  return (int)(want < most ? want : most);
+inline int paged_workgroups(int64_t units, int64_t positions) {
+  const int64_t places = units * ((positions + 31) / 32 + kPaStart), want = (places + kPaStart + 1) / (kPaStart + 2);
+  return (int)(want < kPaSlots ? want : kPaSlots);
+}
+
+// Blocks of 16 columns that share a read of the keys, as far as the registers go.
+inline int paged_blocks(int cols) { return cols <= 16 ? 1 : 2; }
+
+template <int D, int NB>
+inline void paged_launch(const PagedAttn& a, bool f8, int workgroups, hipStream_t s) {
+  if (f8) paged_attn_kernel<D, true, NB><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
+  else paged_attn_kernel<D, false, NB><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
+  paged_attn_merge_kernel<D, NB><<<dim3((unsigned)(a.rows * a.T), a.H), 64 * kPaWaves, 0, s>>>(a);
 }
 
 }  // namespace omni
 
 using namespace omni;
 
-static int64_t paged_attn_units(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads) {
-  const int64_t cols = (int64_t)tokens * (heads / kv_heads);
-  return rows * kv_heads * ((cols + 15) / 16);
-}
-
 extern "C" size_t omni_paged_attention_workspace(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
                                                  int32_t head_dim, int32_t page, int32_t width) {
   if (rows <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-  const int64_t units = paged_attn_units(rows, tokens, heads, kv_heads);
-  return (size_t)(2LL * paged_workgroups(units, (int64_t)width * page, head_dim) * 16 * (head_dim + 2) * 4);
+  const int cols = tokens * (heads / kv_heads), wide = 16 * paged_blocks(cols);
+  const int64_t units = rows * kv_heads * ((cols + wide - 1) / wide);
+  return (size_t)(2LL * paged_workgroups(units, (int64_t)width * page) * wide * (head_dim + 2) * 4);
 }
 
 extern "C" int omni_paged_attention(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
@@ -518,33 +563,30 @@ extern "C" int omni_paged_attention(const void* q, const void* k_pages, const vo
   a.rows = rows;
   a.group = heads / kv_heads;
   a.cols = tokens * a.group;
-  a.qblocks = (a.cols + 15) / 16;
+  const int blocks = paged_blocks(a.cols), wide = 16 * blocks;
+  a.qblocks = (a.cols + wide - 1) / wide;
   a.units = kv_heads * a.qblocks;
   const int64_t units = (int64_t)rows * a.units;
   // Places of the line, keys and groups are counted in 31 bits.
   if (a.cache.positions > 0x7fffff00LL || units > 0x7fffff00LL ||
       units * ((a.cache.positions + 31) / 32 + kPaStart) > 0x7fffff00LL)
     return OMNI_ERR_SHAPE;
-  const int workgroups = paged_workgroups(units, a.cache.positions, head_dim);
+  const int workgroups = paged_workgroups(units, a.cache.positions);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + 2LL * workgroups * 16 * head_dim;
+  a.part_ml = a.part_o + 2LL * workgroups * wide * head_dim;
   a.out = (uint16_t*)out;
   const hipStream_t s = (hipStream_t)stream;
-  const dim3 merge((unsigned)(rows * tokens), heads);
   const bool f8 = cache_dtype == OMNI_E4M3;
   if (head_dim == 128) {
-    if (f8) paged_attn_kernel<128, true><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
-    else paged_attn_kernel<128, false><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
-    paged_attn_merge_kernel<128><<<merge, 64 * kPaWaves, 0, s>>>(a);
+    if (blocks == 1) paged_launch<128, 1>(a, f8, workgroups, s);
+    else paged_launch<128, 2>(a, f8, workgroups, s);
   } else if (head_dim == 256) {
-    if (f8) paged_attn_kernel<256, true><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
-    else paged_attn_kernel<256, false><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
-    paged_attn_merge_kernel<256><<<merge, 64 * kPaWaves, 0, s>>>(a);
+    if (blocks == 1) paged_launch<256, 1>(a, f8, workgroups, s);
+    else paged_launch<256, 2>(a, f8, workgroups, s);
   } else {
-    if (f8) paged_attn_kernel<512, true><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
-    else paged_attn_kernel<512, false><<<workgroups, 64 * kPaWaves, 0, s>>>(a);
-    paged_attn_merge_kernel<512><<<merge, 64 * kPaWaves, 0, s>>>(a);
+    if (blocks == 1) paged_launch<512, 1>(a, f8, workgroups, s);
+    else paged_launch<512, 2>(a, f8, workgroups, s);
   }
   return omni_launch_status();
 }

@@ -32,6 +32,7 @@ no other code path: on a GPU without the library these functions raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 from contextlib import nullcontext
 
 import torch
@@ -73,6 +74,10 @@ def _dtype(t: torch.Tensor) -> int:
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+# torch's current stream of a device as the integer the C entry points take (no stream object on the way).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _ptr(t: torch.Tensor | None):
@@ -618,32 +623,52 @@ def beam_select(logits: torch.Tensor, score: torch.Tensor, count: torch.Tensor, 
 
 # ---------------------------------------------------------------------------------------------- paged caches
 
-def _current(device: torch.device):
-    """The context a launch on ``device`` runs in: a stream is used with its own device current."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(device: int):
+    """The context a launch on GPU ``device`` runs in: a stream is used with its own device current."""
+    return _SAME if device == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_SAME = nullcontext()
+
+
+def _on(device: int, named: tuple) -> None:
+    """Checks that the (name, tensor) pairs are on GPU ``device``."""
+    for name, t in named:
+        if t.get_device() != device or device < 0:
+            raise ValueError(f"{name}: on the GPU, all on one device")
+
+
+def _positions(n: int, named: tuple) -> None:
+    """Checks contiguous int64 vectors of ``n``."""
+    for name, t in named:
+        if t.dtype != torch.long or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous int64 [{n}]")
 
 
 def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k_scale: torch.Tensor | None,
-           v_scale: torch.Tensor | None) -> int:
-    """Checks a paged cache; returns its element type.  ``k_pages`` / ``v_pages`` [pages, kv heads, page, D], bf16 or
-    float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8; ``table`` [rows, width] int32."""
+           v_scale: torch.Tensor | None) -> tuple[int, torch.Size, tuple]:
+    """Checks a paged cache; returns its element type, shape and tensors by name.  ``k_pages`` / ``v_pages`` [pages, kv
+    heads, page, D], bf16 or float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8; ``table``
+    [rows, width] int32."""
     shape, dtype = k_pages.shape, k_pages.dtype
-    _need(len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype and k_pages.is_contiguous()
-          and v_pages.is_contiguous(), "k_pages / v_pages: contiguous [pages, kv heads, page, D] of one dtype")
-    _need(shape[3] in (128, 256, 512) and shape[2] in (16, 32, 64, 128, 256),
-          "k_pages / v_pages: head dim 128, 256 or 512, pages of 16, 32, 64, 128 or 256 positions")
-    _need(table.dtype == torch.int32 and table.dim() == 2 and (table.stride(1) == 1 or table.size(1) <= 1),
-          "table: [rows, width] int32 with unit stride in width")
-    device = k_pages.device
-    if dtype == torch.float8_e4m3fn:
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need(t is not None and t.dtype == torch.uint8 and t.shape == shape[:3] and t.is_contiguous()
-                  and t.device == device, f"{name}: contiguous uint8 [pages, kv heads, page] for e4m3 pages")
-    else:
-        _need(dtype == torch.bfloat16, "k_pages / v_pages: bfloat16 or float8_e4m3fn")
-        _need(k_scale is None and v_scale is None, "k_scale / v_scale: for e4m3 pages only")
-    _need(v_pages.device == device and table.device == device, "pages and table: one device")
-    return _lib.BF16 if dtype == torch.bfloat16 else _lib.E4M3
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dtype or not k_pages.is_contiguous() \
+            or not v_pages.is_contiguous():
+        raise ValueError("k_pages / v_pages: contiguous [pages, kv heads, page, D] of one dtype")
+    if shape[3] not in (128, 256, 512) or shape[2] not in (16, 32, 64, 128, 256) or shape[1] < 1:
+        raise ValueError("k_pages / v_pages: head dim 128, 256 or 512, pages of 16, 32, 64, 128 or 256 positions")
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.size(1) > 1):
+        raise ValueError("table: [rows, width] int32 with unit stride in width")
+    tensors = (("k_pages", k_pages), ("v_pages", v_pages), ("table", table))
+    if dtype == torch.bfloat16:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale / v_scale: for e4m3 pages only")
+        return _lib.BF16, shape, tensors
+    if dtype != torch.float8_e4m3fn:
+        raise ValueError("k_pages / v_pages: bfloat16 or float8_e4m3fn")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is None or t.dtype != torch.uint8 or t.shape != shape[:3] or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous uint8 [pages, kv heads, page] for e4m3 pages")
+    return _lib.E4M3, shape, (*tensors, ("k_scale", k_scale), ("v_scale", v_scale))
 
 
 def _row_stride(table: torch.Tensor) -> int:
@@ -664,27 +689,25 @@ def rope_kv_paged(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     Pages are bf16, or float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8: a vector x is kept as
     the e4m3 nearest to x * 2^-e, and the byte e + 127, e the least integer with max |x| <= 448 * 2^e."""
     lib = _lib.load()
-    cache = _paged(k_pages, v_pages, table, k_scale, v_scale)
-    pages, kv, page, dim = k_pages.shape
-    _need(qkv.dim() == 2 and heads >= 1 and qkv.size(1) == (heads + 2 * kv) * dim and qkv.stride(1) == 1,
-          "qkv: [N, (heads + 2 * kv heads) * D] with unit stride in the last dimension")
-    n, device = qkv.size(0), qkv.device
-    _need(qkv.dtype == torch.bfloat16, "qkv: bfloat16")
-    _need(cs.dtype == torch.float32 and cs.is_contiguous() and cs.dim() == 3 and cs.size(1) * 2 == dim
-          and cs.size(2) == 2, "cs: contiguous [P, D/2, 2] fp32")
-    for name, t in (("pos", pos), ("slots", slots), ("cache_pos", cache_pos)):
-        if t is not None:
-            _index(t, name)
-            _need(t.numel() == n and t.device == device, f"{name}: [N] on qkv's device")
-    _need(k_pages.device == device and cs.device == device, "qkv, cs and the cache: one device")
-    q = torch.empty(n, heads, dim, device=device, dtype=qkv.dtype)
-    k = torch.empty(n, kv, dim, device=device, dtype=qkv.dtype) if rotated else None
-    with _current(device):
+    cache, (pages, kv, page, dim), held = _paged(k_pages, v_pages, table, k_scale, v_scale)
+    if qkv.dim() != 2 or heads < 1 or qkv.size(1) != (heads + 2 * kv) * dim or qkv.stride(1) != 1:
+        raise ValueError("qkv: [N, (heads + 2 * kv heads) * D] with unit stride in the last dimension")
+    if qkv.dtype != torch.bfloat16:
+        raise ValueError("qkv: bfloat16")
+    if cs.dtype != torch.float32 or cs.dim() != 3 or cs.size(1) * 2 != dim or cs.size(2) != 2 or not cs.is_contiguous():
+        raise ValueError("cs: contiguous [P, D/2, 2] fp32")
+    n, device = qkv.size(0), qkv.get_device()
+    at = [("pos", pos), *((name, t) for name, t in (("slots", slots), ("cache_pos", cache_pos)) if t is not None)]
+    _positions(n, at)
+    _on(device, (("qkv", qkv), ("cs", cs), *at, *held))
+    q = torch.empty((n, heads, dim), device=qkv.device, dtype=torch.bfloat16)
+    k = torch.empty((n, kv, dim), device=qkv.device, dtype=torch.bfloat16) if rotated else None
+    with _launch(device):
         status = lib.omni_rope_kv_paged(
             qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.size(1), cs.data_ptr(), cs.size(0), pos.data_ptr(),
             _ptr(slots), _ptr(cache_pos), q.data_ptr(), _ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
             _ptr(v_scale), pages, page, table.data_ptr(), _row_stride(table), table.size(0), table.size(1), n, heads,
-            kv, dim, cache, _lib.BF16, _stream(qkv))
+            kv, dim, cache, _lib.BF16, _raw_stream(device))
     _lib.check(status, "rope_kv_paged")
     return (q, k) if rotated else q
 
@@ -696,22 +719,25 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     its power of two is a bf16 number), zeros where the row, position or page is outside the cache.  What a prompt that
     goes on behind cached positions attends to (:func:`packed_attention`).  The cache as for :func:`rope_kv_paged`."""
     lib = _lib.load()
-    cache = _paged(k_pages, v_pages, table, k_scale, v_scale)
-    pages, kv, page, dim = k_pages.shape
-    device = k_pages.device
-    for name, t in (("slots", slots), ("pos", pos)):
-        _index(t, name)
-        _need(t.numel() == slots.numel() and t.device == device, f"{name}: [N] on the cache's device")
-    n = slots.numel()
-    k = torch.empty(n, kv, dim, device=device, dtype=torch.bfloat16)
-    v = torch.empty(n, kv, dim, device=device, dtype=torch.bfloat16)
-    with _current(device):
+    cache, (pages, kv, page, dim), held = _paged(k_pages, v_pages, table, k_scale, v_scale)
+    n, device = slots.numel(), k_pages.get_device()
+    at = (("slots", slots), ("pos", pos))
+    _positions(n, at)
+    _on(device, (*at, *held))
+    kv_out = torch.empty((2, n, kv, dim), device=k_pages.device, dtype=torch.bfloat16)
+    k, v = kv_out.unbind()
+    with _launch(device):
         status = lib.omni_paged_read(
             k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), pages, page, table.data_ptr(),
             _row_stride(table), table.size(0), table.size(1), slots.data_ptr(), pos.data_ptr(), n, kv, dim, cache,
-            k.data_ptr(), v.data_ptr(), _stream(k))
+            k.data_ptr(), v.data_ptr(), _raw_stream(device))
     _lib.check(status, "paged_read")
     return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(*shape: int) -> int:
+    return max(_lib.load().omni_paged_attention_workspace(*shape), 256)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -722,26 +748,26 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     No key gives zeros.  Returns [B*T, H, D].  Calls may overlap: each has its own workspace.  The cache as for
     :func:`rope_kv_paged`."""
     lib = _lib.load()
-    cache = _paged(k_pages, v_pages, table, k_scale, v_scale)
-    pages, kv, page, dim = k_pages.shape
-    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.is_contiguous() and q.size(2) == dim
-          and q.size(1) % kv == 0 and q.size(1) >= kv, "q: contiguous bf16 [B*T, H, D], H a multiple of the kv heads")
-    _need(1 <= tokens <= 16 and q.size(0) % tokens == 0, "tokens: 1..16, q: [B*T, H, D]")
-    device, heads, rows = q.device, q.size(1), q.size(0) // tokens
-    _need(table.size(0) >= rows, "table: at least B rows")
-    _need(pages > 0 and table.size(1) > 0, "the cache: at least one page and one table entry")
-    _index(lengths, "lengths")
-    _need(lengths.numel() >= rows, "lengths: [B]")
-    _need(lengths.device == device and k_pages.device == device, "q, lengths and the cache: one device")
+    cache, (pages, kv, page, dim), held = _paged(k_pages, v_pages, table, k_scale, v_scale)
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.size(2) != dim or q.size(1) < kv or q.size(1) % kv \
+            or not q.is_contiguous():
+        raise ValueError("q: contiguous bf16 [B*T, H, D], H a multiple of the kv heads")
+    if not 1 <= tokens <= 16 or q.size(0) % tokens:
+        raise ValueError("tokens: 1..16, q: [B*T, H, D]")
+    heads, rows, width, device = q.size(1), q.size(0) // tokens, table.size(1), q.get_device()
+    if table.size(0) < rows or pages == 0 or width == 0:
+        raise ValueError("table: at least B rows, one entry and one page")
+    if lengths.dtype != torch.long or lengths.numel() < rows or not lengths.is_contiguous():
+        raise ValueError("lengths: contiguous int64 [B]")
+    _on(device, (("q", q), ("lengths", lengths), *held))
     out = torch.empty_like(q)
-    width = table.size(1)
-    with _current(device):
-        ws = lib.omni_paged_attention_workspace(rows, tokens, heads, kv, dim, page, width)
-        workspace = torch.empty(max(ws, 256), device=device, dtype=torch.uint8)
+    workspace = torch.empty(_paged_workspace(rows, tokens, heads, kv, dim, page, width), device=q.device,
+                            dtype=torch.uint8)
+    with _launch(device):
         status = lib.omni_paged_attention(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), pages, page,
             table.data_ptr(), _row_stride(table), width, lengths.data_ptr(), rows, tokens, heads, kv, dim, scale,
-            out.data_ptr(), workspace.data_ptr(), workspace.numel(), cache, _lib.BF16, _stream(q))
+            out.data_ptr(), workspace.data_ptr(), workspace.numel(), cache, _lib.BF16, _raw_stream(device))
     _lib.check(status, "paged attention")
     return out
 
@@ -756,30 +782,32 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     goes on behind earlier positions (:func:`paged_read`).  No key gives zeros.  ``longest``: at least the queries of the
     longest sequence.  Returns ``out`` [N, H, D] (new by default); rows in no sequence are left as they are in it."""
     lib = _lib.load()
-    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.is_contiguous() and q.size(2) in (128, 256, 512),
-          "q: contiguous bf16 [N, H, D], D = 128, 256 or 512")
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.size(2) not in (128, 256, 512) or not q.is_contiguous():
+        raise ValueError("q: contiguous bf16 [N, H, D], D = 128, 256 or 512")
     n, heads, dim = q.shape
-    _need(k.dim() == 3 and k.shape == v.shape and k.size(2) == dim and k.dtype == q.dtype == v.dtype,
-          "k / v: bf16 [M, kv heads, D]")
+    if k.dim() != 3 or k.shape != v.shape or k.size(2) != dim or k.dtype != torch.bfloat16 or v.dtype != k.dtype:
+        raise ValueError("k / v: bf16 [M, kv heads, D]")
     m, kv = k.size(0), k.size(1)
-    _need(kv >= 1 and heads % kv == 0 and heads >= kv, "q: a multiple of k's heads")
-    _need(k.stride(2) == 1 and v.stride(2) == 1, "k / v: unit stride in D")
+    if kv < 1 or heads < kv or heads % kv:
+        raise ValueError("q: a multiple of k's heads")
+    if k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("k / v: unit stride in D")
+    if starts.numel() < 1 or longest < 0:
+        raise ValueError("starts: [S + 1], longest: at least the longest sequence's queries")
     k_starts = starts if k_starts is None else k_starts
-    device = q.device
-    for name, t in (("starts", starts), ("k_starts", k_starts)):
-        _index(t, name)
-        _need(t.numel() == starts.numel() >= 1 and t.device == device, f"{name}: [S + 1] on q's device")
-    _need(k.device == device and v.device == device, "q, k and v: one device")
-    _need(longest >= 0, "longest: at least the longest sequence's queries")
+    device = q.get_device()
+    at = (("starts", starts), ("k_starts", k_starts))
+    _positions(starts.numel(), at)
+    _on(device, (("q", q), ("k", k), ("v", v), *at))
     if out is None:
         out = torch.empty_like(q)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == device,
-          "out: contiguous, q's shape, dtype and device")
-    with _current(device):
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous():
+        raise ValueError("out: contiguous, q's shape, dtype and device")
+    with _launch(device):
         status = lib.omni_packed_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             starts.data_ptr(), k_starts.data_ptr(), starts.numel() - 1, n, m, min(longest, n), heads, kv, dim, scale,
-            out.data_ptr(), _lib.BF16, _stream(q))
+            out.data_ptr(), _lib.BF16, _raw_stream(device))
     _lib.check(status, "packed attention")
     return out
 
