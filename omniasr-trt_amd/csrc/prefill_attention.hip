@@ -10,7 +10,7 @@
 
 #include <algorithm>
 
-#include "attn_tiles.h"
+#include "attn_chunks.h"
 #include "common.h"
 
 namespace omni {
@@ -37,6 +37,7 @@ struct PrefillArgs {
   int64_t queries = 0, keys = 0;      // rows of q, of k and v
   int64_t k_pos = 0, k_head = 0, v_pos = 0, v_head = 0;
   int heads_per_kv = 1;
+  int together = 1;  // head dim 128: heads of a kv head in one block (1, 2 or 4)
 };
 
 // A context's or sequence's part of a call for one head: queries q0 .. q0 + nq - 1, keys 0 .. nk - 1 of k / v, rows
@@ -98,30 +99,111 @@ __device__ __forceinline__ PfBlock pf_block(int nqb, int H, int B) {
   return PfBlock{k % nqb, unit % H, unit / H};
 }
 
-// The same for packed prompts: XCD x's heads are x * H / 8 .., so that heads of one kv head stay in one L2.
-__device__ __forceinline__ PfBlock pf_packed_block(int nqb, int H, int B) {
-  if (H % 8 != 0) return pf_block(nqb, H, B);
-  const int L = (int)blockIdx.x + nqb * ((int)blockIdx.y + H * (int)blockIdx.z);
-  const int k = L / 8, unit = k / nqb;
-  return PfBlock{k % nqb, L % 8 * (H / 8) + unit % (H / 8), unit / (H / 8)};
+// The sequence of rank r by work (queries x keys, less what causality hides), the most first: so the last blocks of a
+// launch, whose CUs wait for each other, are the short ones.  Past 64 sequences, the order of the call.
+__device__ __forceinline__ int pf_ranked(const PrefillArgs& a, int sequences, int r) {
+  if (sequences > kWave) return r;
+  const int lane = lane_id(), s = min(lane, sequences - 1);
+  const float nq = (float)(a.starts[s + 1] - a.starts[s]), nk = (float)(a.k_starts[s + 1] - a.k_starts[s]);
+  const float work = lane < sequences ? nq * (2.f * nk - nq) : -INFINITY;
+  int rank = 0;
+  for (int t = 0; t < sequences; ++t) {
+    const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(work), t));
+    rank += other > work || (other == work && t < lane) ? 1 : 0;
+  }
+  const uint64_t hit = __ballot(lane < sequences && rank == r);
+  return hit ? __builtin_ctzll(hit) : r;  // (always one, but for starts that are no counts)
 }
 
-// On tiles with keys that some query does not see, their probability is 0, but 0 times an infinity or NaN of V would
-// reach the query's output.  V operands of such a tile are looked at; where one holds such a value the products run
-// without it, and pf_add_nonfinite adds it for the queries that see it.
-__device__ __forceinline__ bool pf_nonfinite(u32x4_t w) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
-  return bad;
+// The same for packed prompts, with ``heads`` blocks of heads: XCD x's are x * heads / 8 .., so that heads of one kv head
+// stay in one L2.
+__device__ __forceinline__ PfBlock pf_packed_block(const PrefillArgs& a, int nqb, int heads, int sequences) {
+  PfBlock p;
+  if (heads % 8 != 0) {
+    p = pf_block(nqb, heads, sequences);
+  } else {
+    const int L = (int)blockIdx.x + nqb * ((int)blockIdx.y + heads * (int)blockIdx.z);
+    const int k = L / 8, unit = k / nqb;
+    p = PfBlock{k % nqb, L % 8 * (heads / 8) + unit % (heads / 8), unit / (heads / 8)};
+  }
+  p.b = pf_ranked(a, sequences, p.b);
+  return p;
 }
-__device__ __forceinline__ u32x4_t pf_finite(u32x4_t w) {
+
+// On a tile with keys that some query does not see, their probability is 0, but 0 times an infinity or NaN of V would
+// reach the query's output.  Looking for such values tile by tile costs the kernels registers that they do not have, so
+// the outputs are looked at instead: a wave with one that is not finite works its queries out again, 16 at a time and 128
+// dimensions of the result (``out`` and ``v`` point at them), leaving what is not finite out of the products of those tiles
+// and adding it to the queries that see it -- whose output it makes infinite or NaN whatever its weight.  Rare, and slow.
+// ``q`` / ``out``: the first of the ``n`` <= 16 queries, rows q_pos apart; the first sees keys [0, whole] of nk.
+template <int D>
+__device__ __noinline__ void pf_again_16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out,
+                                         int64_t q_pos, int64_t k_pos, int64_t v_pos, int n, int whole, int nk,
+                                         float scale_log2) {
+  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const int end = whole + n, query = min(c, n - 1), lim = whole + query + 1;
+  const uint16_t* qrow = q + query * q_pos + 8 * g;
+  f32x4_t o[1][8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[0][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  SoftmaxState st{-INFINITY, -INFINITY, 0.f};
+  for (int t = 0; t < end; t += 32) {
+    f32x4_t acc[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+    for (int s = 0; s < D; s += 32) {
+      const u32x4_t qs = *reinterpret_cast<const u32x4_t*>(qrow + s);
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+        const int key = min(t + 8 * (c >> 2) + 4 * mb + (c & 3), nk - 1);
+        const u32x4_t ks = *reinterpret_cast<const u32x4_t*>(k + key * k_pos + s + 8 * g);
+        acc[mb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ks), __builtin_bit_cast(bf16x8_t, qs),
+                                                          acc[mb], 0, 0, 0);
+      }
+    }
+    const u32x4_t pop[1] = {tile_softmax<8>(acc, scale_log2, st, o[0], g, lim - t - 8 * g)};
+    KvChunk<false> vt;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      vt.r[j] = ld16(reinterpret_cast<const char*>(v + min(t + 8 * g + j, nk - 1) * v_pos + 8 * c));
+    if (t + 31 > whole && __any(only_finite<false>(vt))) {
+      for (int key = t; key < min(t + 32, end); ++key)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float value = bf16_to_f32(v[key * v_pos + 8 * c + e]);
+          const float extra = value - value == 0.f ? 0.f : value;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[0][e][i] += key <= whole + 4 * g + i ? extra : 0.f;
+        }
+    }
+    const float one[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+    chunk_values<false, 1>(vt, pop, one, o);
+  }
+  const float l = column_sum(st.l_run);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
-    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
+    const float li = __shfl(l, 4 * g + i, kWave), div = li == 0.f ? 1.f : li;
+    if (4 * g + i >= n) continue;
+    u32x4_t w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(o[0][2 * e][i] / div, o[0][2 * e + 1][i] / div);
+    *reinterpret_cast<u32x4_t*>(out + (4 * g + i) * q_pos + 8 * c) = w;
   }
-  return w;
+}
+
+// Queries q_first .. q_first + 16 groups - 1 of a head again, dimensions slice .. + 127.
+template <int D>
+__device__ __forceinline__ void pf_again(const PrefillArgs& a, const PfSpan& sp, int h, int q_first, int groups, int slice) {
+  for (int i = 0; i < groups; ++i) {
+    const int q0 = q_first + 16 * i, n = min(sp.nq - q0, 16);
+    if (n <= 0) return;
+    const int64_t row = ((sp.q0 + q0) * a.H + h) * D;
+    pf_again_16<D>(a.q + row, sp.k, sp.v + slice, a.out + row + slice, (int64_t)a.H * D, a.k_pos, a.v_pos, n,
+                   q0 + sp.before, sp.nk, a.scale_log2);
+  }
+}
+
+// Whether a word of two bf16 holds an infinity or NaN: an exponent of ones carries into the sign's place.
+__device__ __forceinline__ bool pf_nonfinite(uint32_t w) {
+  return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
 }
 
 // Head dim 256: one workgroup of kPwWaves waves per (query block, head, context).  The block's
@@ -157,7 +239,7 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
   __shared__ int rflag[NG];                 // the group's reference max moved on this tile
   __shared__ float lsum[NG][16];            // probability sum of each query, at the end
   const int nqb = (a.width + QW - 1) / QW;
-  const PfBlock blk = kPacked ? pf_packed_block(nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
+  const PfBlock blk = kPacked ? pf_packed_block(a, nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
   const int qb = (nqb - 1 - blk.j) * QW;  // the longest blocks first
   const int h = blk.h, b = blk.b;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
@@ -322,35 +404,6 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
       }
       // V operands by transpose reads from this wave's slice of the rows: within 16 lanes, lane 4r + q points at key r,
       // dimensions 4q .. + 3, and lane c receives dimension c of the four keys.
-      bool bad = false;
-      if (kPacked && key0 + 31 > qb + 16 * m + sp.before) {  // not every query of the wave's groups sees every key
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          bad |= pf_nonfinite(
-              *reinterpret_cast<const u32x4_t*>(&vl[t & 1][(4 * i + (lane >> 4)) * kRowB + 256 * sl + (lane & 15) * 16]));
-        bad = __any(bad);
-      }
-      if (kPacked && bad) {
-        for (int key = 0; key < 32 && key0 + key < sp.nk; ++key) {
-          const uint16_t* row = reinterpret_cast<const uint16_t*>(&vl[t & 1][key * kRowB + 256 * sl]);
-#pragma unroll
-          for (int u = 0; u < kPwSub; ++u) {
-            const int gi = m + M * u;
-            if (!sees(gi, key0)) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float p = bf16_to_f32(
-                  reinterpret_cast<const uint16_t*>(&pex[gi][4 * g + i + 16 * (key >> 3)])[key & 7]);
-              const bool seen = key0 + key <= qb + 16 * gi + 4 * g + i + sp.before;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const uint32_t bits = row[16 * e + c];
-                if ((bits & 0x7f80u) == 0x7f80u && seen) o[u][e][i] += p * bf16_to_f32(bits);
-              }
-            }
-          }
-        }
-      }
       const int rr = c >> 2, q4 = c & 3;
       const lds_char* vls = (const lds_char*)vl[t & 1];  // vl lives in LDS
 #pragma unroll
@@ -363,7 +416,6 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
         bop[1] = (uint32_t)(uint16_t)lo[2] | ((uint32_t)(uint16_t)lo[3] << 16);
         bop[2] = (uint32_t)(uint16_t)hi[0] | ((uint32_t)(uint16_t)hi[1] << 16);
         bop[3] = (uint32_t)(uint16_t)hi[2] | ((uint32_t)(uint16_t)hi[3] << 16);
-        if (kPacked && bad) bop = pf_finite(bop);
 #pragma unroll
         for (int u = 0; u < kPwSub; ++u) {
           if (!sees(m + M * u, key0)) continue;
@@ -391,6 +443,7 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
   for (int u = 0; u < kPwSub; ++u) {
     const int gi = m + M * u;
+    bool again = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int qq = qb + 16 * gi + 4 * g + i;
@@ -399,8 +452,13 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
       const float div = li > 0.f ? li : 1.f;
       uint16_t* orow = a.out + ((sp.q0 + qq) * a.H + h) * D + 128 * sl;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) orow[16 * e + c] = (uint16_t)pack_bf16x2(o[u][e][i] / div, 0.f);
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t w = pack_bf16x2(o[u][e][i] / div, 0.f);
+        orow[16 * e + c] = (uint16_t)w;
+        if constexpr (kPacked) again |= pf_nonfinite(w);
+      }
     }
+    if (kPacked && __any(again)) pf_again<D>(a, sp, h, qb + 16 * gi, 1, 128 * sl);
   }
 }
 
@@ -437,39 +495,10 @@ constexpr int kWsRow = kWsD * 2 + 16;  // LDS bytes per K row
 constexpr int kWsAhead = 4;
 constexpr float kWsGuard = 16.0f;
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
-}
-
-// What pf_finite left out of O^T += V^T P^T for one tile of 64 keys from ``key0``: O [query half u][e], register 4q + i of
-// lane half g in row 8q + 4g + i, dimension dim(e, row); P [u][16-key step][lane] as the score waves write it.
-template <typename Dim>
-__device__ void pf_add_nonfinite(f32x16_t (&o)[2][4], const u32x4_t (*ps)[4][64], const uint16_t* v, uint32_t v_bytes,
-                                 int key0, int nk, int query0, int before, int x, int g, Dim dim) {
-  for (int key = 0; key < 64 && key0 + key < nk; ++key) {
-    const int r = key & 31, i16 = 4 * (r >> 3) + (r & 3), from = x + 32 * ((r >> 2) & 1);
-    const uint16_t* row = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v) +
-                                                            (int64_t)(key0 + key) * v_bytes);
-    float p[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint16_t* word = reinterpret_cast<const uint16_t*>(&ps[u][2 * (key >> 5) + (i16 >> 3)][from]);
-      p[u] = bf16_to_f32(word[i16 & 7]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        const uint32_t bits = row[dim(e, 8 * (n >> 2) + 4 * g + (n & 3))];
-        if ((bits & 0x7f80u) != 0x7f80u) continue;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (key0 + key <= query0 + 32 * u + x + before) o[u][e][n] += p[u] * bf16_to_f32(bits);
-      }
-  }
 }
 
 // A wave-uniform pointer in scalar registers.
@@ -576,7 +605,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (kChain) {
       place(blk, 0);
     } else {
-      const PfBlock one = kPacked ? pf_packed_block(nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
+      const PfBlock one =
+          kPacked ? pf_packed_block(a, nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
       blk = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, one.b};  // the longest blocks first
     }
     return blk;
@@ -756,26 +786,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   // O^T += V^T P^T for the workgroup's tile t; ``ahead``: the next tile's V loads as its registers fall free.  Step
   // s + 1's operands are built beside step s's products; the scheduler keeps each step's loads behind the permutes that read their registers.
-  auto attend_v = [&](int t, const WsTile& cur, const WsTile* ahead) {
+  auto attend_v = [&](int t, const WsTile* ahead) {
     u32x4_t vop[2][4];
-    if constexpr (kPacked) {
-      const PfSpan sp = span(cur.blk);
-      if (cur.t * kWsK + kWsK - 1 > cur.blk.qb + sp.before) {  // not every query sees every key
-        bool bad = false;
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) bad |= pf_nonfinite(v[s][j]);
-        if (__any(bad)) {
-          pf_add_nonfinite(o, ps[t & 1], sp.v + 128 * vw, v_bytes, cur.t * kWsK, sp.nk, cur.blk.qb, sp.before, x, g,
-                           [](int e, int row) { return 8 * (row & 15) + 4 * (row >> 4) + e; });
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[s][j] = pf_finite(v[s][j]);
-        }
-      }
-    }
     auto operands = [&](int s) {
       // The lanes of a pair (u = 0, 1) hold 8 dimensions of 4 keys each; swapped, 4 dimensions (8c + 4u ..) of 8 keys:
       // lo[j] of key 16s + 4g + j, hi[j] of key 16s + 8 + 4g + j.
@@ -836,6 +848,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   auto output = [&](const WsBlock& blk, int odd) {  // O of a finished block; then O is 0 again
     const PfSpan sp = span(blk);
+    bool again = false;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int query = blk.qb + 32 * u + x;
@@ -859,6 +872,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
               out[2 * k + 1] = pair(o[u][2][at], o[u][3][at]);
             }
             *reinterpret_cast<u32x4_t*>(orow + 64 * r + 8 * i) = out;
+            if constexpr (kPacked) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) again |= pf_nonfinite(out[k]);
+            }
           }
       }
 #pragma unroll
@@ -866,6 +883,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
     }
+    if (kPacked && __any(again)) pf_again<D>(a, sp, blk.h, blk.qb, 4, 128 * vw);
   };
   auto open = [&](WsTile& c) {  // the block's first tile
     const PfSpan sp = span(c.blk);
@@ -898,11 +916,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   take_p(0);
   int n = 1, odd = 0;
   while (more) {  // tile n's scores, tile n - 1's values
-    const WsTile was = at;
+    const WsBlock was = at.blk;
     at = ahead;
     more = advance(ahead);
     bring_k(ahead, n + 1);  // unconditional (past the last tile: that tile again, not used): no wait joins a branch
-    attend_v(n - 1, was, &at);
+    attend_v(n - 1, &at);
     // vmcnt(16): tile n + 1's K rows are in LDS, tile n's 16 V loads, issued after them, stay in flight (lds_barrier
     // would wait for those too).  This wave's LDS reads of the tile are in registers by now.
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -910,13 +928,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     if (kChain && at.t == 0) {
-      output(was.blk, odd);
+      output(was, odd);
       odd ^= 1;
     }
     take_p(n);
     ++n;
   }
-  attend_v(n - 1, at, nullptr);
+  attend_v(n - 1, nullptr);
   lds_barrier();
   output(at.blk, odd);
 }
@@ -957,22 +975,29 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ float als[4][4][64];         // [pair][tile % 4]: O's factors, when the reference moved
   __shared__ int moved[4][4];
   __shared__ float lsum[4][2][64];        // [pair][lane half]
-  const int nqb = (a.width + kPairQ - 1) / kPairQ;
-  const PfBlock blk = kPacked ? pf_packed_block(nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
-  const int qb = (nqb - 1 - blk.j) * kPairQ;  // the longest blocks first
-  const int h = blk.h, b = blk.b;
+  // The pairs' 64 queries: of one head one after another, or (packed) of 2 or 4 heads that read the same keys.
+  const int together = kPacked ? a.together : 1, queries = kPairQ / together;
+  const int nqb = (a.width + queries - 1) / queries;
+  const PfBlock blk = kPacked ? pf_packed_block(a, nqb, a.H / together, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
+  const int qb = (nqb - 1 - blk.j) * queries;  // the longest blocks first
+  const int b = blk.b;
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), pr = w & 3;
+  const int h = kPacked ? blk.h * together + pr % together : blk.h;
   const PfSpan sp = pf_span<D, kPacked>(a, h, b);
   const char* kbase = scalar_pointer(sp.k);
   const char* vbase = scalar_pointer(sp.v);
-  const int keys = min(qb + kPairQ, sp.nq) + sp.before;  // what the block's last query sees
+  const int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees
   if constexpr (kPacked) {
     if (qb >= sp.nq) return;
-    if (keys <= 0) return pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + kPairQ, sp.nq), h);
+    if (keys <= 0) {
+      for (int i = 0; i < together; ++i)
+        pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), blk.h * together + i);
+      return;
+    }
   }
   const int nt = (keys + kPairK - 1) / kPairK;
-  const int qp = qb + 64 * pr;
+  const int qp = qb + 64 * (kPacked ? pr / together : pr);
   // The pair's last tile, which holds its diagonal (-1: no queries, or they see no key).
   const int lastk = kPacked ? min(qp + 64, sp.nq) - 1 + sp.before : qp;
   const int dq = qp < sp.nq && lastk >= 0 ? lastk / kPairK : -1;
@@ -1155,19 +1180,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
     const lds_char* vt = (const lds_char*)vls[t & 1];
-    bool bad = false;
-    if (kPacked && t * kPairK + kPairK - 1 > whole) {  // wave-uniform: not every query sees every key
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        // The whole tile: row 4i + lane / 16, 16 bytes a lane.
-        bad |= pf_nonfinite(*reinterpret_cast<const u32x4_t*>(&vls[t & 1][(4 * i + (lane >> 4)) * (D * 2) + (lane & 15) * 16]));
-      }
-      bad = __any(bad);
-      if (bad) {
-        pf_add_nonfinite(o, ps[pr][t & 1], sp.v, sp.v_bytes, t * kPairK, sp.nk, qp, sp.before, x, g,
-                         [](int e, int row) { return 32 * e + 8 * ((row >> 2) & 3) + 4 * (row >> 4) + (row & 3); });
-      }
-    }
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -1175,8 +1187,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + vlane[e] + s * 16 * D * 2));
         const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + vlane[e] + (s * 16 + 8) * D * 2));
         const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
-        u32x4_t vop = {l2[0], l2[1], h2[0], h2[1]};
-        if (kPacked && bad) vop = pf_finite(vop);
+        const u32x4_t vop = {l2[0], l2[1], h2[0], h2[1]};
 #pragma unroll
         for (int u = 0; u < 2; ++u) o[u][e] = mfma32(vop, p[u][s], o[u][e]);
       }
@@ -1188,6 +1199,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (t >= 2 && t - 2 <= dq) attend_v(t - 2);
     landed_barrier();
   }
+  bool again = false;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int query = qp + 32 * u + x;
@@ -1210,8 +1222,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           out[2 * k + 1] = pair(o[u][e][at + 2], o[u][e][at + 3]);
         }
         *reinterpret_cast<u32x4_t*>(orow + 32 * e + 16 * rb) = out;
+        if constexpr (kPacked) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) again |= pf_nonfinite(out[i]);
+        }
       }
   }
+  if (kPacked && __any(again)) pf_again<D>(a, sp, h, qp, 4, 0);
 }
 
 // Head dim 128 in blocks of 192 queries, for the launches of small_blocks: one workgroup of 4 waves, two workgroups per
@@ -1534,7 +1551,9 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
   a.heads_per_kv = heads / kv_heads;
   const hipStream_t s = (hipStream_t)stream;
   if (head_dim == 128) {
-    const dim3 grid((longest + omni::kPairQ - 1) / omni::kPairQ, heads, sequences);
+    a.together = a.heads_per_kv % 4 == 0 ? 4 : a.heads_per_kv % 2 == 0 ? 2 : 1;
+    const int queries = omni::kPairQ / a.together;
+    const dim3 grid((longest + queries - 1) / queries, heads / a.together, sequences);
     omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
   } else if (head_dim == 512) {
     const dim3 grid((longest + omni::kWsQ - 1) / omni::kWsQ, heads, sequences);
