@@ -53,63 +53,76 @@ struct PagedWrite {
   int heads;
 };
 
+// One workgroup per token; a thread keeps the same 8 dimensions of every vector it takes, so the token's angles are read
+// once and its cell is found once.
 template <int D, bool kF8>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite w, PagedCache a) {
   constexpr int kLanes = D / 8;  // of one vector; a vector never spans two waves
-  const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  const int vec = piece / kLanes, e0 = piece % kLanes * 8;
-  if (vec >= w.heads + 2 * a.kv) return;
+  constexpr int kBatch = 3;      // vectors in flight
+  const int stride = blockDim.x / kLanes;  // vectors at a time
+  const int e0 = threadIdx.x % kLanes * 8, vectors = w.heads + 2 * a.kv;
   const int64_t n = blockIdx.x;
-  const u32x4_t raw = *reinterpret_cast<const u32x4_t*>(w.qkv + n * w.qkv_stride + vec * D + e0);
+  const uint16_t* row = w.qkv + n * w.qkv_stride + e0;
   const int64_t p = w.pos[n];
-  float x[8];
+  const int64_t cell0 = paged_cell(a, w.slots ? w.slots[n] : n, w.cache_pos ? w.cache_pos[n] : p, 0);
+  const f32x4_t* angles = reinterpret_cast<const f32x4_t*>(w.cs + clamp64(p, 0, w.cs_rows - 1) * D + e0);
+  const f32x4_t t0 = angles[0], t1 = angles[1];
+  for (int v0 = threadIdx.x / kLanes; v0 < vectors; v0 += stride * kBatch) {
+    u32x4_t raw[kBatch];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = bf16x8_elem(raw, e);
-  if (vec < w.heads + a.kv) {
-    const f32x4_t* row = reinterpret_cast<const f32x4_t*>(w.cs + clamp64(p, 0, w.cs_rows - 1) * D + e0);
-    const f32x4_t t0 = row[0], t1 = row[1];
-    turn_pair(x[0], x[1], t0[0], t0[1]);
-    turn_pair(x[2], x[3], t0[2], t0[3]);
-    turn_pair(x[4], x[5], t1[0], t1[1]);
-    turn_pair(x[6], x[7], t1[2], t1[3]);
-  }
-  u32x4_t bf;
+    for (int k = 0; k < kBatch; ++k)
+      if (v0 + k * stride < vectors) raw[k] = *reinterpret_cast<const u32x4_t*>(row + (v0 + k * stride) * D);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bf[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-  if (vec < w.heads) {
-    *reinterpret_cast<u32x4_t*>(w.q_out + (n * w.heads + vec) * D + e0) = bf;
-    return;
-  }
-  const bool is_k = vec < w.heads + a.kv;
-  const int head = vec - w.heads - (is_k ? 0 : a.kv);
-  if (is_k && w.k_out) *reinterpret_cast<u32x4_t*>(w.k_out + (n * a.kv + head) * D + e0) = bf;
-  const int64_t cell = paged_cell(a, w.slots ? w.slots[n] : n, w.cache_pos ? w.cache_pos[n] : p, head);
-  char* pages = is_k ? a.k : a.v;
-  if constexpr (!kF8) {
-    if (cell < 0) return;
-    *reinterpret_cast<u32x4_t*>(pages + (cell * D + e0) * 2) = is_k ? bf : raw;
-  } else {
-    uint32_t top = 0;
+    for (int k = 0; k < kBatch; ++k) {
+      const int vec = v0 + k * stride;
+      if (vec >= vectors) break;
+      float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t u = __float_as_uint(x[e]) & 0x7fffffffu;
-      top = max(top, u < 0x7f800000u ? u : 0u);
+      for (int e = 0; e < 8; ++e) x[e] = bf16x8_elem(raw[k], e);
+      u32x4_t bf = raw[k];
+      if (vec < w.heads + a.kv) {
+        turn_pair(x[0], x[1], t0[0], t0[1]);
+        turn_pair(x[2], x[3], t0[2], t0[3]);
+        turn_pair(x[4], x[5], t1[0], t1[1]);
+        turn_pair(x[6], x[7], t1[2], t1[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bf[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+      }
+      if (vec < w.heads) {
+        *reinterpret_cast<u32x4_t*>(w.q_out + (n * w.heads + vec) * D + e0) = bf;
+        continue;
+      }
+      const bool is_k = vec < w.heads + a.kv;
+      const int head = vec - w.heads - (is_k ? 0 : a.kv);
+      if (is_k && w.k_out) *reinterpret_cast<u32x4_t*>(w.k_out + (n * a.kv + head) * D + e0) = bf;
+      if (cell0 < 0) continue;
+      const int64_t cell = cell0 + ((int64_t)head << a.page_log2);
+      char* pages = is_k ? a.k : a.v;
+      if constexpr (!kF8) {
+        *reinterpret_cast<u32x4_t*>(pages + (cell * D + e0) * 2) = bf;
+      } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t u = __float_as_uint(x[e]) & 0x7fffffffu;
+          top = max(top, u < 0x7f800000u ? u : 0u);
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
+        const int exponent = e4m3_exponent(top);
+        const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = to_e4m3_range(x[e], down, exponent == 120);
+        u32x2_t codes;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int half = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+          codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], half, true);
+        }
+        *reinterpret_cast<u32x2_t*>(pages + cell * D + e0) = codes;
+        if (e0 == 0) (is_k ? a.k_scale : a.v_scale)[cell] = (uint8_t)(exponent + 127);
+      }
     }
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
-    if (cell < 0) return;
-    const int exponent = e4m3_exponent(top);
-    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = to_e4m3_range(x[e], down, exponent == 120);
-    u32x2_t codes;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int half = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
-      codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], half, true);
-    }
-    *reinterpret_cast<u32x2_t*>(pages + cell * D + e0) = codes;
-    if (e0 == 0) (is_k ? a.k_scale : a.v_scale)[cell] = (uint8_t)(exponent + 127);
   }
 }
 
@@ -120,45 +133,58 @@ struct PagedRead {
   uint16_t* v;
 };
 
+// One workgroup per token, as paged_write_kernel.
 template <int D, bool kF8>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead r, PagedCache a) {
-  constexpr int kLanes = D / 8;
-  const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  const int vec = piece / kLanes, e0 = piece % kLanes * 8;
-  if (vec >= 2 * a.kv) return;
+  constexpr int kLanes = D / 8, kBatch = 4;
+  const int stride = blockDim.x / kLanes;
+  const int e0 = threadIdx.x % kLanes * 8, vectors = 2 * a.kv;
   const int64_t n = blockIdx.x;
-  const bool is_k = vec < a.kv;
-  const int head = vec - (is_k ? 0 : a.kv);
-  const int64_t cell = paged_cell(a, r.slots[n], r.pos[n], head);
-  u32x4_t out = {0u, 0u, 0u, 0u};
-  if (cell >= 0) {
-    const char* pages = is_k ? a.k : a.v;
-    if constexpr (kF8) {
-      out = e4m3x8_to_bf16(*reinterpret_cast<const u32x2_t*>(pages + cell * D + e0),
-                           scale_of((is_k ? a.k_scale : a.v_scale)[cell]));
-    } else {
-      out = *reinterpret_cast<const u32x4_t*>(pages + (cell * D + e0) * 2);
+  const int64_t cell0 = paged_cell(a, r.slots[n], r.pos[n], 0);
+  for (int v0 = threadIdx.x / kLanes; v0 < vectors; v0 += stride * kBatch) {
+    u32x4_t out[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int vec = v0 + k * stride;
+      const bool is_k = vec < a.kv;
+      const int64_t cell = cell0 + ((int64_t)(vec - (is_k ? 0 : a.kv)) << a.page_log2);
+      const char* pages = is_k ? a.k : a.v;
+      out[k] = u32x4_t{0u, 0u, 0u, 0u};
+      if (cell0 < 0 || vec >= vectors) continue;
+      if constexpr (kF8) {
+        out[k] = e4m3x8_to_bf16(*reinterpret_cast<const u32x2_t*>(pages + cell * D + e0),
+                                scale_of((is_k ? a.k_scale : a.v_scale)[cell]));
+      } else {
+        out[k] = *reinterpret_cast<const u32x4_t*>(pages + (cell * D + e0) * 2);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int vec = v0 + k * stride, head = vec - (vec < a.kv ? 0 : a.kv);
+      if (vec >= vectors) break;
+      *reinterpret_cast<u32x4_t*>((vec < a.kv ? r.k : r.v) + (n * a.kv + head) * D + e0) = out[k];
     }
   }
-  *reinterpret_cast<u32x4_t*>((is_k ? r.k : r.v) + (n * a.kv + head) * D + e0) = out;
 }
 
 }  // namespace omni
 
 using namespace omni;
 
-// The instance of ``kernel`` for a head dim and cache type.
-#define OMNI_PAGED_LAUNCH(kernel, head_dim, f8, grid, stream, ...)                                  \
+// The instance of ``kernel`` for a head dim and cache type, with whole waves for a token's ``vectors``, four at most.
+#define OMNI_PAGED_LAUNCH(kernel, head_dim, vectors, f8, grid, stream, ...)                         \
   do {                                                                                              \
+    const int64_t lanes = (int64_t)(vectors) * (head_dim / 8);                                      \
+    const int block = lanes >= 256 ? 256 : (int)((lanes + 63) / 64 * 64);                           \
     if (head_dim == 128) {                                                                          \
-      if (f8) kernel<128, true><<<grid, 256, 0, stream>>>(__VA_ARGS__);                             \
-      else kernel<128, false><<<grid, 256, 0, stream>>>(__VA_ARGS__);                               \
+      if (f8) kernel<128, true><<<grid, block, 0, stream>>>(__VA_ARGS__);                           \
+      else kernel<128, false><<<grid, block, 0, stream>>>(__VA_ARGS__);                             \
     } else if (head_dim == 256) {                                                                   \
-      if (f8) kernel<256, true><<<grid, 256, 0, stream>>>(__VA_ARGS__);                             \
-      else kernel<256, false><<<grid, 256, 0, stream>>>(__VA_ARGS__);                               \
+      if (f8) kernel<256, true><<<grid, block, 0, stream>>>(__VA_ARGS__);                           \
+      else kernel<256, false><<<grid, block, 0, stream>>>(__VA_ARGS__);                             \
     } else {                                                                                        \
-      if (f8) kernel<512, true><<<grid, 256, 0, stream>>>(__VA_ARGS__);                             \
-      else kernel<512, false><<<grid, 256, 0, stream>>>(__VA_ARGS__);                               \
+      if (f8) kernel<512, true><<<grid, block, 0, stream>>>(__VA_ARGS__);                           \
+      else kernel<512, false><<<grid, block, 0, stream>>>(__VA_ARGS__);                             \
     }                                                                                               \
   } while (0)
 
@@ -182,9 +208,8 @@ extern "C" int omni_rope_kv_paged(const void* qkv, int64_t qkv_row_stride, const
                      (uint16_t*)k_out, heads};
   const PagedCache a =
       omni_paged_cache(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, table, table_stride, rows, width);
-  const int pieces = (heads + 2 * kv_heads) * (head_dim / 8);
-  const dim3 grid((unsigned)n_tokens, (unsigned)((pieces + 255) / 256));
-  OMNI_PAGED_LAUNCH(paged_write_kernel, head_dim, cache_dtype == OMNI_E4M3, grid, (hipStream_t)stream, w, a);
+  const dim3 grid((unsigned)n_tokens);
+  OMNI_PAGED_LAUNCH(paged_write_kernel, head_dim, heads + 2 * kv_heads, cache_dtype == OMNI_E4M3, grid, (hipStream_t)stream, w, a);
   return omni_launch_status();
 }
 
@@ -203,8 +228,7 @@ extern "C" int omni_paged_read(const void* k_pages, const void* v_pages, const v
   const PagedRead r{slots, pos, (uint16_t*)k_out, (uint16_t*)v_out};
   const PagedCache a =
       omni_paged_cache(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, table, table_stride, rows, width);
-  const int pieces = 2 * kv_heads * (head_dim / 8);
-  const dim3 grid((unsigned)n_tokens, (unsigned)((pieces + 255) / 256));
-  OMNI_PAGED_LAUNCH(paged_read_kernel, head_dim, cache_dtype == OMNI_E4M3, grid, (hipStream_t)stream, r, a);
+  const dim3 grid((unsigned)n_tokens);
+  OMNI_PAGED_LAUNCH(paged_read_kernel, head_dim, 2 * kv_heads, cache_dtype == OMNI_E4M3, grid, (hipStream_t)stream, r, a);
   return omni_launch_status();
 }
