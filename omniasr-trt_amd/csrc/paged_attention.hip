@@ -23,7 +23,8 @@
 namespace omni {
 
 constexpr int kPaWaves = 4;
-constexpr int kPaStart = 6;
+constexpr int kPaStart = 3;
+constexpr int kPaLeast = 3;  // places of a share, at least
 
 struct PagedAttn {
   const uint16_t* q;  // [rows * T, H, D]
@@ -87,8 +88,12 @@ __device__ __forceinline__ int paged_total(const PagedAttn& a, int lane, PagedLi
   return total;
 }
 
-// Places of a share: an even part of all for each workgroup, but not so few that its start outweighs them.
-__device__ __forceinline__ int paged_share(int total) { return max((total + kPaSlots - 1) / kPaSlots, kPaStart + 2); }
+// Places of a share: an even part of all for each workgroup, but not so few that what the second launch has to read
+// outweighs them.  Measured, a unit's start counted as 2, 3, 4 and 6 tiles and shares of 2, 3, 4 places and more, us: 1 slot
+// x 1433 keys, 8 x 512 e4m3, shares of 2 12.5, 3 13.3, 4 14.4, 8 18.2 (a tile after the other takes 1.1 us there); 32 over 8
+// x 128 9.8, 9.3, 9.4, 12.1; 8 slots x 5 of 750-2400 keys within 26-27 whichever; 16 slots of 4000-8188 keys, 16 over 2 x
+// 256, starts of 2 30.9, 3 30.5, 4 29.8.
+__device__ __forceinline__ int paged_share(int total) { return max((total + kPaSlots - 1) / kPaSlots, kPaLeast); }
 
 // A unit, and where its tiles are in the line: [from, from + tiles).
 struct PagedUnit {
@@ -508,7 +513,7 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
 
 // Workgroups of a call: what runs at once, but none that a full table would leave without a share.
 inline int paged_workgroups(int64_t units, int64_t positions) {
-  const int64_t places = units * ((positions + 31) / 32 + kPaStart), want = (places + kPaStart + 1) / (kPaStart + 2);
+  const int64_t places = units * ((positions + 31) / 32 + kPaStart), want = (places + kPaLeast - 1) / kPaLeast;
   return (int)(want < kPaSlots ? want : kPaSlots);
 }
 

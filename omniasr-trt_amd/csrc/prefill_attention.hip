@@ -50,29 +50,44 @@ struct PfSpan {
   uint32_t k_bytes, v_bytes;
 };
 
-template <int D, bool kPacked>
+template <int D>
 __device__ __forceinline__ PfSpan pf_span(const PrefillArgs& a, int h, int b) {
+  const int64_t slot = clamp64(a.slots[b], 0, a.cache_rows - 1);
   PfSpan p;
-  if constexpr (kPacked) {
-    p.q0 = clamp64(a.starts[b], 0, a.queries);
-    const int64_t k0 = clamp64(a.k_starts[b], 0, a.keys), nq = clamp64(a.starts[b + 1], p.q0, a.queries) - p.q0;
-    p.nk = (int)(clamp64(a.k_starts[b + 1], k0, a.keys) - k0);
-    p.before = p.nk - (int)nq;
-    p.nq = (int)(nq < a.width ? nq : a.width);
-    const int kv = h / a.heads_per_kv;
-    p.k = a.k + k0 * a.k_pos + kv * a.k_head;
-    p.v = a.v + k0 * a.v_pos + kv * a.v_head;
-    p.k_bytes = (uint32_t)a.k_pos * 2;
-    p.v_bytes = (uint32_t)a.v_pos * 2;
-  } else {
-    const int64_t slot = clamp64(a.slots[b], 0, a.cache_rows - 1);
-    p.q0 = (int64_t)b * a.width;
-    p.nq = p.nk = a.width;
-    p.before = 0;
-    p.k = a.k + slot * a.s_row + h * a.s_head;
-    p.v = a.v + slot * a.s_row + h * a.s_head;
-    p.k_bytes = p.v_bytes = D * 2;
-  }
+  p.q0 = (int64_t)b * a.width;
+  p.nq = p.nk = a.width;
+  p.before = 0;
+  p.k = a.k + slot * a.s_row + h * a.s_head;
+  p.v = a.v + slot * a.s_row + h * a.s_head;
+  p.k_bytes = p.v_bytes = D * 2;
+  return p;
+}
+
+// A packed sequence: its first query and key, and how many there are, within q and k.
+struct PfSequence {
+  int64_t q0, k0;
+  int nq, nk;
+};
+__device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s) {
+  PfSequence p;
+  p.q0 = clamp64(a.starts[s], 0, a.queries);
+  p.k0 = clamp64(a.k_starts[s], 0, a.keys);
+  p.nq = (int)(clamp64(a.starts[s + 1], p.q0, a.queries) - p.q0);
+  p.nk = (int)(clamp64(a.k_starts[s + 1], p.k0, a.keys) - p.k0);
+  return p;
+}
+
+__device__ __forceinline__ PfSpan pf_packed_span(const PrefillArgs& a, int h, const PfSequence& s) {
+  const int kv = h / a.heads_per_kv;
+  PfSpan p;
+  p.q0 = s.q0;
+  p.nq = min(s.nq, a.width);
+  p.nk = s.nk;
+  p.before = s.nk - s.nq;
+  p.k = a.k + s.k0 * a.k_pos + kv * a.k_head;
+  p.v = a.v + s.k0 * a.v_pos + kv * a.v_head;
+  p.k_bytes = (uint32_t)a.k_pos * 2;
+  p.v_bytes = (uint32_t)a.v_pos * 2;
   return p;
 }
 
@@ -99,25 +114,39 @@ __device__ __forceinline__ PfBlock pf_block(int nqb, int H, int B) {
   return PfBlock{k % nqb, unit % H, unit / H};
 }
 
+__device__ __forceinline__ int64_t pf_readlane64(int64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // The sequence of rank r by work (queries x keys, less what causality hides), the most first: so the last blocks of a
 // launch, whose CUs wait for each other, are the short ones.  Past 64 sequences, the order of the call.
-__device__ __forceinline__ int pf_ranked(const PrefillArgs& a, int sequences, int r) {
-  if (sequences > kWave) return r;
-  const int lane = lane_id(), s = min(lane, sequences - 1);
-  const float nq = (float)(a.starts[s + 1] - a.starts[s]), nk = (float)(a.k_starts[s + 1] - a.k_starts[s]);
-  const float work = lane < sequences ? nq * (2.f * nk - nq) : -INFINITY;
+__device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequences, int r) {
+  if (sequences > kWave) return pf_sequence(a, r);
+  const int lane = lane_id();
+  const PfSequence mine = pf_sequence(a, min(lane, sequences - 1));
+  const float work = lane < sequences ? (float)mine.nq * (2.f * (float)mine.nk - (float)mine.nq) : -INFINITY;
   int rank = 0;
   for (int t = 0; t < sequences; ++t) {
     const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(work), t));
     rank += other > work || (other == work && t < lane) ? 1 : 0;
   }
-  const uint64_t hit = __ballot(lane < sequences && rank == r);
-  return hit ? __builtin_ctzll(hit) : r;  // (always one, but for starts that are no counts)
+  const int l = __builtin_ctzll(__ballot(lane < sequences && rank == r));
+  PfSequence p;
+  p.q0 = pf_readlane64(mine.q0, l);
+  p.k0 = pf_readlane64(mine.k0, l);
+  p.nq = __builtin_amdgcn_readlane(mine.nq, l);
+  p.nk = __builtin_amdgcn_readlane(mine.nk, l);
+  return p;
 }
 
-// The same for packed prompts, with ``heads`` blocks of heads: XCD x's are x * heads / 8 .., so that heads of one kv head
-// stay in one L2.
-__device__ __forceinline__ PfBlock pf_packed_block(const PrefillArgs& a, int nqb, int heads, int sequences) {
+// The workgroup's block for packed prompts, with ``heads`` blocks of heads: XCD x's are x * heads / 8 .., so that heads of
+// one kv head stay in one L2.
+struct PfPacked {
+  int j, h;
+  PfSequence s;
+};
+__device__ __forceinline__ PfPacked pf_packed_block(const PrefillArgs& a, int nqb, int heads, int sequences) {
   PfBlock p;
   if (heads % 8 != 0) {
     p = pf_block(nqb, heads, sequences);
@@ -126,8 +155,7 @@ __device__ __forceinline__ PfBlock pf_packed_block(const PrefillArgs& a, int nqb
     const int k = L / 8, unit = k / nqb;
     p = PfBlock{k % nqb, L % 8 * (heads / 8) + unit % (heads / 8), unit / (heads / 8)};
   }
-  p.b = pf_ranked(a, sequences, p.b);
-  return p;
+  return PfPacked{p.j, p.h, pf_ranked(a, sequences, p.b)};
 }
 
 // On a tile with keys that some query does not see, their probability is 0, but 0 times an infinity or NaN of V would
@@ -239,13 +267,23 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
   __shared__ int rflag[NG];                 // the group's reference max moved on this tile
   __shared__ float lsum[NG][16];            // probability sum of each query, at the end
   const int nqb = (a.width + QW - 1) / QW;
-  const PfBlock blk = kPacked ? pf_packed_block(a, nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
-  const int qb = (nqb - 1 - blk.j) * QW;  // the longest blocks first
-  const int h = blk.h, b = blk.b;
+  int j, h;
+  PfSpan sp;
+  if constexpr (kPacked) {
+    const PfPacked blk = pf_packed_block(a, nqb, a.H, (int)gridDim.z);
+    j = blk.j;
+    h = blk.h;
+    sp = pf_packed_span(a, h, blk.s);
+  } else {
+    const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
+    j = blk.j;
+    h = blk.h;
+    sp = pf_span<D>(a, h, blk.b);
+  }
+  const int qb = (nqb - 1 - j) * QW;  // the longest blocks first
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int sl = w % NSL, m = w / NSL;
-  const PfSpan sp = pf_span<D, kPacked>(a, h, b);
   const uint16_t* kbase = sp.k;
   const uint16_t* vbase = sp.v;
   const int64_t k_pos = kPacked ? a.k_pos : D, v_pos = kPacked ? a.v_pos : D;
@@ -600,13 +638,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     blk = WsBlock{round, (nqb - 1 - r / members) * kWsQ, unit % a.H, unit / a.H};
     return true;
   };
+  WsBlock only;  // packed: the one block of the workgroup, and its span
+  PfSpan only_span;
+  if constexpr (kPacked) {
+    const PfPacked one = pf_packed_block(a, nqb, a.H, (int)gridDim.z);
+    only = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, 0};
+    only_span = pf_packed_span(a, one.h, one.s);
+    if (only.qb >= only_span.nq) return;
+    const int end = min(only.qb + kWsQ, only_span.nq);
+    if (end + only_span.before <= 0)
+      return pf_zeros<D>(a, only_span.q0 + only.qb, only_span.q0 + end, only.h);
+  }
   auto first = [&]() {
     WsBlock blk;
-    if constexpr (kChain) {
+    if constexpr (kPacked) {
+      blk = only;
+    } else if constexpr (kChain) {
       place(blk, 0);
     } else {
-      const PfBlock one =
-          kPacked ? pf_packed_block(a, nqb, a.H, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
+      const PfBlock one = pf_block(nqb, a.H, (int)gridDim.z);
       blk = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, one.b};  // the longest blocks first
     }
     return blk;
@@ -615,18 +665,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (kChain) return place(blk, blk.round + 1);
     return false;
   };
-  auto span = [&](const WsBlock& blk) { return pf_span<D, kPacked>(a, blk.h, blk.b); };
+  auto span = [&](const WsBlock& blk) {
+    if constexpr (kPacked) return only_span;
+    return pf_span<D>(a, blk.h, blk.b);
+  };
   // The block's last tile: the one of its last query's last key.
   auto last_tile = [&](const WsBlock& blk, const PfSpan& sp) {
     return kPacked ? (min(blk.qb + kWsQ, sp.nq) - 1 + sp.before) / kWsK : blk.qb / kWsK;
   };
-  if constexpr (kPacked) {
-    const WsBlock blk = first();
-    const PfSpan sp = span(blk);
-    if (blk.qb >= sp.nq) return;
-    const int end = min(blk.qb + kWsQ, sp.nq);
-    if (end + sp.before <= 0) return pf_zeros<D>(a, sp.q0 + blk.qb, sp.q0 + end, blk.h);
-  }
 
   if (w < 4) {  // ------------------------------------------------------------------------------ scores
     const int qh = w & 1, kh = w >> 1;
@@ -906,13 +952,32 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   at.blk = first();
   open(at);
   bring_k(at, 0);
-  landed_barrier();
-  ahead = at;
-  bool more = advance(ahead);
-  bring_k(ahead, 1);
+  bool more;
+  if constexpr (kPacked) {
+    // All of the start's loads at once, then waits for the first K tile (32 loads behind it) and the second (16): what
+    // the block takes before its first tile is done is 1.2 us less than one after the other.
+    __builtin_amdgcn_sched_barrier(0);
+    ahead = at;
+    more = advance(ahead);
+    bring_k(ahead, 1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int s = 0; s < 4; ++s) load_v(at, s);
-  landed_barrier();
+    for (int s = 0; s < 4; ++s) load_v(at, s);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x8f70);  // vmcnt(32)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_waitcnt(0x4f70);  // vmcnt(16)
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  } else {
+    landed_barrier();
+    ahead = at;
+    more = advance(ahead);
+    bring_k(ahead, 1);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) load_v(at, s);
+    landed_barrier();
+  }
   take_p(0);
   int n = 1, odd = 0;
   while (more) {  // tile n's scores, tile n - 1's values
@@ -978,13 +1043,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // The pairs' 64 queries: of one head one after another, or (packed) of 2 or 4 heads that read the same keys.
   const int together = kPacked ? a.together : 1, queries = kPairQ / together;
   const int nqb = (a.width + queries - 1) / queries;
-  const PfBlock blk = kPacked ? pf_packed_block(a, nqb, a.H / together, (int)gridDim.z) : pf_block(nqb, a.H, (int)gridDim.z);
-  const int qb = (nqb - 1 - blk.j) * queries;  // the longest blocks first
-  const int b = blk.b;
+  int j, hb, b = 0;
+  PfSequence seq = {};
+  if constexpr (kPacked) {
+    const PfPacked blk = pf_packed_block(a, nqb, a.H / together, (int)gridDim.z);
+    j = blk.j;
+    hb = blk.h;
+    seq = blk.s;
+  } else {
+    const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
+    j = blk.j;
+    hb = blk.h;
+    b = blk.b;
+  }
+  const int qb = (nqb - 1 - j) * queries;  // the longest blocks first
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), pr = w & 3;
-  const int h = kPacked ? blk.h * together + pr % together : blk.h;
-  const PfSpan sp = pf_span<D, kPacked>(a, h, b);
+  const int h = kPacked ? hb * together + pr % together : hb;
+  PfSpan sp;
+  if constexpr (kPacked) sp = pf_packed_span(a, h, seq);
+  else sp = pf_span<D>(a, h, b);
   const char* kbase = scalar_pointer(sp.k);
   const char* vbase = scalar_pointer(sp.v);
   const int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees
@@ -992,7 +1070,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (qb >= sp.nq) return;
     if (keys <= 0) {
       for (int i = 0; i < together; ++i)
-        pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), blk.h * together + i);
+        pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), hb * together + i);
       return;
     }
   }
