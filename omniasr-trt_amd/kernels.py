@@ -33,7 +33,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from contextlib import nullcontext
 
 import torch
 import torch.nn.functional as F
@@ -623,56 +622,67 @@ def beam_select(logits: torch.Tensor, score: torch.Tensor, count: torch.Tensor, 
 
 # ---------------------------------------------------------------------------------------------- paged caches
 
-def _launch(device: int):
-    """The context a launch on GPU ``device`` runs in: a stream is used with its own device current."""
-    return _SAME if device == torch.cuda.current_device() else torch.cuda.device(device)
+_BF16, _E4M3, _LONG = torch.bfloat16, torch.float8_e4m3fn, torch.long
+_HEAD_DIMS, _PAGES = (128, 256, 512), (16, 32, 64, 128, 256)
+_current_device = torch._C._cuda_getDevice
 
 
-_SAME = nullcontext()
-
-
-def _on(device: int, named: tuple) -> None:
-    """Checks that the (name, tensor) pairs are on GPU ``device``."""
-    for name, t in named:
-        if t.get_device() != device or device < 0:
-            raise ValueError(f"{name}: on the GPU, all on one device")
-
-
-def _positions(n: int, named: tuple) -> None:
-    """Checks contiguous int64 vectors of ``n``."""
-    for name, t in named:
-        if t.dtype != torch.long or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous int64 [{n}]")
+def _call(device: int, what: str, entry, *args) -> None:
+    """``entry(*args, stream)`` on GPU ``device``'s current stream, the device made current where it is not."""
+    if device == _current_device():
+        status = entry(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = entry(*args, _raw_stream(device))
+    if status:
+        _lib.check(status, what)
 
 
 def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k_scale: torch.Tensor | None,
-           v_scale: torch.Tensor | None) -> tuple[int, torch.Size, tuple]:
-    """Checks a paged cache; returns its element type, shape and tensors by name.  ``k_pages`` / ``v_pages`` [pages, kv
-    heads, page, D], bf16 or float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8; ``table``
-    [rows, width] int32."""
+           v_scale: torch.Tensor | None, device: int) -> tuple:
+    """Checks a paged cache (compare :func:`_paged_refusal`); returns its shape, the pages', exponents' and table's part of
+    the C calls' arguments, its element type, and whether it is on GPU ``device``."""
     shape, dtype = k_pages.shape, k_pages.dtype
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dtype or not k_pages.is_contiguous() \
-            or not v_pages.is_contiguous():
-        raise ValueError("k_pages / v_pages: contiguous [pages, kv heads, page, D] of one dtype")
-    if shape[3] not in (128, 256, 512) or shape[2] not in (16, 32, 64, 128, 256) or shape[1] < 1:
-        raise ValueError("k_pages / v_pages: head dim 128, 256 or 512, pages of 16, 32, 64, 128 or 256 positions")
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.size(1) > 1):
-        raise ValueError("table: [rows, width] int32 with unit stride in width")
-    tensors = (("k_pages", k_pages), ("v_pages", v_pages), ("table", table))
-    if dtype == torch.bfloat16:
-        if k_scale is not None or v_scale is not None:
-            raise ValueError("k_scale / v_scale: for e4m3 pages only")
-        return _lib.BF16, shape, tensors
-    if dtype != torch.float8_e4m3fn:
-        raise ValueError("k_pages / v_pages: bfloat16 or float8_e4m3fn")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t is None or t.dtype != torch.uint8 or t.shape != shape[:3] or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous uint8 [pages, kv heads, page] for e4m3 pages")
-    return _lib.E4M3, shape, (*tensors, ("k_scale", k_scale), ("v_scale", v_scale))
+    fp8 = dtype is _E4M3
+    if not ((fp8 or dtype is _BF16) and len(shape) == 4 and shape[3] in _HEAD_DIMS and shape[2] in _PAGES and shape[1] > 0
+            and v_pages.shape == shape and v_pages.dtype is dtype and k_pages.is_contiguous() and v_pages.is_contiguous()
+            and table.dtype is torch.int32 and table.dim() == 2 and (table.size(1) < 2 or table.stride(1) == 1)):
+        _paged_refusal(k_pages, v_pages, table)
+    here = k_pages.get_device() == v_pages.get_device() == table.get_device() == device >= 0
+    ks = vs = None
+    if fp8:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is None or t.dtype is not torch.uint8 or t.shape != shape[:3] or not t.is_contiguous():
+                raise ValueError(f"{name}: contiguous uint8 [pages, kv heads, page] for e4m3 pages")
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+        here = here and k_scale.get_device() == v_scale.get_device() == device
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("k_scale / v_scale: for e4m3 pages only")
+    stride = table.stride(0) if table.size(0) > 1 else table.size(1)
+    return shape, (k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, shape[0], shape[2], table.data_ptr(), stride), \
+        _lib.E4M3 if fp8 else _lib.BF16, here
 
 
-def _row_stride(table: torch.Tensor) -> int:
-    return table.stride(0) if table.size(0) > 1 else max(table.stride(0), table.size(1))
+def _paged_refusal(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor) -> None:
+    """Raises with what of a paged cache is not as :func:`rope_kv_paged` states it."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    _need(len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype and k_pages.is_contiguous()
+          and v_pages.is_contiguous(), "k_pages / v_pages: contiguous [pages, kv heads, page, D] of one dtype")
+    _need(dtype in (_BF16, _E4M3), "k_pages / v_pages: bfloat16 or float8_e4m3fn")
+    _need(shape[3] in _HEAD_DIMS and shape[2] in _PAGES and shape[1] > 0,
+          "k_pages / v_pages: head dim 128, 256 or 512, pages of 16, 32, 64, 128 or 256 positions")
+    raise ValueError("table: [rows, width] int32 with unit stride in width")
+
+
+_ELSEWHERE = "the cache and the call's tensors: on the GPU, all on one device"
+
+
+def _positions(n: int, device: int, *named: tuple) -> None:
+    """Checks contiguous int64 vectors of ``n`` on GPU ``device``, as (name, tensor or None)."""
+    for name, t in named:
+        if t is not None and not (t.dtype is _LONG and t.numel() == n and t.is_contiguous()
+                                  and t.get_device() == device >= 0):
+            raise ValueError(f"{name}: contiguous int64 [{n}] on the GPU, where the call's other tensors are")
 
 
 def rope_kv_paged(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_pages: torch.Tensor,
@@ -689,26 +699,24 @@ def rope_kv_paged(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     Pages are bf16, or float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8: a vector x is kept as
     the e4m3 nearest to x * 2^-e, and the byte e + 127, e the least integer with max |x| <= 448 * 2^e."""
     lib = _lib.load()
-    cache, (pages, kv, page, dim), held = _paged(k_pages, v_pages, table, k_scale, v_scale)
+    device = qkv.get_device()
+    (_, kv, _, dim), pages, cache, here = _paged(k_pages, v_pages, table, k_scale, v_scale, device)
     if qkv.dim() != 2 or heads < 1 or qkv.size(1) != (heads + 2 * kv) * dim or qkv.stride(1) != 1:
         raise ValueError("qkv: [N, (heads + 2 * kv heads) * D] with unit stride in the last dimension")
-    if qkv.dtype != torch.bfloat16:
+    if qkv.dtype is not _BF16:
         raise ValueError("qkv: bfloat16")
-    if cs.dtype != torch.float32 or cs.dim() != 3 or cs.size(1) * 2 != dim or cs.size(2) != 2 or not cs.is_contiguous():
+    if cs.dtype is not torch.float32 or cs.dim() != 3 or cs.size(1) * 2 != dim or cs.size(2) != 2 \
+            or not cs.is_contiguous():
         raise ValueError("cs: contiguous [P, D/2, 2] fp32")
-    n, device = qkv.size(0), qkv.get_device()
-    at = [("pos", pos), *((name, t) for name, t in (("slots", slots), ("cache_pos", cache_pos)) if t is not None)]
-    _positions(n, at)
-    _on(device, (("qkv", qkv), ("cs", cs), *at, *held))
-    q = torch.empty((n, heads, dim), device=qkv.device, dtype=torch.bfloat16)
-    k = torch.empty((n, kv, dim), device=qkv.device, dtype=torch.bfloat16) if rotated else None
-    with _launch(device):
-        status = lib.omni_rope_kv_paged(
-            qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.size(1), cs.data_ptr(), cs.size(0), pos.data_ptr(),
-            _ptr(slots), _ptr(cache_pos), q.data_ptr(), _ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
-            _ptr(v_scale), pages, page, table.data_ptr(), _row_stride(table), table.size(0), table.size(1), n, heads,
-            kv, dim, cache, _lib.BF16, _raw_stream(device))
-    _lib.check(status, "rope_kv_paged")
+    n = qkv.size(0)
+    _positions(n, device, ("pos", pos), ("slots", slots), ("cache_pos", cache_pos))
+    if not here or cs.get_device() != device:
+        raise ValueError(_ELSEWHERE)
+    q = torch.empty((n, heads, dim), device=qkv.device, dtype=_BF16)
+    k = torch.empty((n, kv, dim), device=qkv.device, dtype=_BF16) if rotated else None
+    _call(device, "rope_kv_paged", lib.omni_rope_kv_paged, qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.size(1),
+          cs.data_ptr(), cs.size(0), pos.data_ptr(), _ptr(slots), _ptr(cache_pos), q.data_ptr(), _ptr(k), *pages,
+          table.size(0), table.size(1), n, heads, kv, dim, cache, _lib.BF16)
     return (q, k) if rotated else q
 
 
@@ -719,19 +727,16 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     its power of two is a bf16 number), zeros where the row, position or page is outside the cache.  What a prompt that
     goes on behind cached positions attends to (:func:`packed_attention`).  The cache as for :func:`rope_kv_paged`."""
     lib = _lib.load()
-    cache, (pages, kv, page, dim), held = _paged(k_pages, v_pages, table, k_scale, v_scale)
-    n, device = slots.numel(), k_pages.get_device()
-    at = (("slots", slots), ("pos", pos))
-    _positions(n, at)
-    _on(device, (*at, *held))
-    kv_out = torch.empty((2, n, kv, dim), device=k_pages.device, dtype=torch.bfloat16)
-    k, v = kv_out.unbind()
-    with _launch(device):
-        status = lib.omni_paged_read(
-            k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), pages, page, table.data_ptr(),
-            _row_stride(table), table.size(0), table.size(1), slots.data_ptr(), pos.data_ptr(), n, kv, dim, cache,
-            k.data_ptr(), v.data_ptr(), _raw_stream(device))
-    _lib.check(status, "paged_read")
+    device = k_pages.get_device()
+    (_, kv, _, dim), pages, cache, here = _paged(k_pages, v_pages, table, k_scale, v_scale, device)
+    n = slots.numel()
+    _positions(n, device, ("slots", slots), ("pos", pos))
+    if not here:
+        raise ValueError(_ELSEWHERE)
+    k = torch.empty((n, kv, dim), device=k_pages.device, dtype=_BF16)
+    v = torch.empty_like(k)
+    _call(device, "paged_read", lib.omni_paged_read, *pages, table.size(0), table.size(1), slots.data_ptr(),
+          pos.data_ptr(), n, kv, dim, cache, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -748,27 +753,26 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     No key gives zeros.  Returns [B*T, H, D].  Calls may overlap: each has its own workspace.  The cache as for
     :func:`rope_kv_paged`."""
     lib = _lib.load()
-    cache, (pages, kv, page, dim), held = _paged(k_pages, v_pages, table, k_scale, v_scale)
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.size(2) != dim or q.size(1) < kv or q.size(1) % kv \
+    device = q.get_device()
+    (pool, kv, page, dim), pages, cache, here = _paged(k_pages, v_pages, table, k_scale, v_scale, device)
+    if q.dim() != 3 or q.dtype is not _BF16 or q.size(2) != dim or q.size(1) < kv or q.size(1) % kv \
             or not q.is_contiguous():
         raise ValueError("q: contiguous bf16 [B*T, H, D], H a multiple of the kv heads")
-    if not 1 <= tokens <= 16 or q.size(0) % tokens:
+    total, heads, _ = q.shape
+    if not 1 <= tokens <= 16 or total % tokens:
         raise ValueError("tokens: 1..16, q: [B*T, H, D]")
-    heads, rows, width, device = q.size(1), q.size(0) // tokens, table.size(1), q.get_device()
-    if table.size(0) < rows or pages == 0 or width == 0:
+    rows, width = total // tokens, table.size(1)
+    if table.size(0) < rows or pool == 0 or width == 0:
         raise ValueError("table: at least B rows, one entry and one page")
-    if lengths.dtype != torch.long or lengths.numel() < rows or not lengths.is_contiguous():
+    if lengths.dtype is not _LONG or lengths.numel() < rows or not lengths.is_contiguous():
         raise ValueError("lengths: contiguous int64 [B]")
-    _on(device, (("q", q), ("lengths", lengths), *held))
+    if not here or lengths.get_device() != device:
+        raise ValueError(_ELSEWHERE)
     out = torch.empty_like(q)
-    workspace = torch.empty(_paged_workspace(rows, tokens, heads, kv, dim, page, width), device=q.device,
-                            dtype=torch.uint8)
-    with _launch(device):
-        status = lib.omni_paged_attention(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), pages, page,
-            table.data_ptr(), _row_stride(table), width, lengths.data_ptr(), rows, tokens, heads, kv, dim, scale,
-            out.data_ptr(), workspace.data_ptr(), workspace.numel(), cache, _lib.BF16, _raw_stream(device))
-    _lib.check(status, "paged attention")
+    size = _paged_workspace(rows, tokens, heads, kv, dim, page, width)
+    workspace = torch.empty(size, device=q.device, dtype=torch.uint8)
+    _call(device, "paged attention", lib.omni_paged_attention, q.data_ptr(), *pages, width, lengths.data_ptr(), rows,
+          tokens, heads, kv, dim, scale, out.data_ptr(), workspace.data_ptr(), size, cache, _lib.BF16)
     return out
 
 
@@ -782,33 +786,32 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     goes on behind earlier positions (:func:`paged_read`).  No key gives zeros.  ``longest``: at least the queries of the
     longest sequence.  Returns ``out`` [N, H, D] (new by default); rows in no sequence are left as they are in it."""
     lib = _lib.load()
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.size(2) not in (128, 256, 512) or not q.is_contiguous():
+    if q.dim() != 3 or q.dtype is not _BF16 or q.size(2) not in _HEAD_DIMS or not q.is_contiguous():
         raise ValueError("q: contiguous bf16 [N, H, D], D = 128, 256 or 512")
     n, heads, dim = q.shape
-    if k.dim() != 3 or k.shape != v.shape or k.size(2) != dim or k.dtype != torch.bfloat16 or v.dtype != k.dtype:
+    if k.dim() != 3 or k.shape != v.shape or k.size(2) != dim or k.dtype is not _BF16 or v.dtype is not _BF16:
         raise ValueError("k / v: bf16 [M, kv heads, D]")
-    m, kv = k.size(0), k.size(1)
+    m, kv, _ = k.shape
     if kv < 1 or heads < kv or heads % kv:
         raise ValueError("q: a multiple of k's heads")
-    if k.stride(2) != 1 or v.stride(2) != 1:
+    (k_pos, k_head, k_unit), (v_pos, v_head, v_unit) = k.stride(), v.stride()
+    if k_unit != 1 or v_unit != 1:
         raise ValueError("k / v: unit stride in D")
-    if starts.numel() < 1 or longest < 0:
+    bounds = starts.numel()
+    if bounds < 1 or longest < 0:
         raise ValueError("starts: [S + 1], longest: at least the longest sequence's queries")
     k_starts = starts if k_starts is None else k_starts
     device = q.get_device()
-    at = (("starts", starts), ("k_starts", k_starts))
-    _positions(starts.numel(), at)
-    _on(device, (("q", q), ("k", k), ("v", v), *at))
+    _positions(bounds, device, ("starts", starts), ("k_starts", k_starts))
+    if not k.get_device() == v.get_device() == device >= 0:
+        raise ValueError("q, k and v: on the GPU, all on one device")
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous():
+    elif out.shape != q.shape or out.dtype is not _BF16 or out.get_device() != device or not out.is_contiguous():
         raise ValueError("out: contiguous, q's shape, dtype and device")
-    with _launch(device):
-        status = lib.omni_packed_attention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            starts.data_ptr(), k_starts.data_ptr(), starts.numel() - 1, n, m, min(longest, n), heads, kv, dim, scale,
-            out.data_ptr(), _lib.BF16, _raw_stream(device))
-    _lib.check(status, "packed attention")
+    _call(device, "packed attention", lib.omni_packed_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pos, k_head,
+          v_pos, v_head, starts.data_ptr(), k_starts.data_ptr(), bounds - 1, n, m, min(longest, n), heads, kv, dim, scale,
+          out.data_ptr(), _lib.BF16)
     return out
 
 
