@@ -37,7 +37,7 @@ struct PrefillArgs {
   int64_t queries = 0, keys = 0;      // rows of q, of k and v
   int64_t k_pos = 0, k_head = 0, v_pos = 0, v_head = 0;
   int heads_per_kv = 1;
-  int together = 1;  // head dim 128: heads of a kv head in one block (1, 2 or 4)
+  int together = 1;  // head dims 128 and 256: heads of a kv head in one block (1, 2 or 4)
 };
 
 // A context's or sequence's part of a call for one head: queries q0 .. q0 + nq - 1, keys 0 .. nk - 1 of k / v, rows
@@ -249,7 +249,6 @@ __device__ __forceinline__ bool pf_nonfinite(uint32_t w) {
 constexpr int kPwWaves = 8;
 constexpr int kPwSub = 3;  // 16-query groups per wave
 
-template <bool kPacked>
 __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill_attn_wide_kernel(
     PrefillArgs a) {
   constexpr int D = 256;
@@ -267,42 +266,27 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
   __shared__ int rflag[NG];                 // the group's reference max moved on this tile
   __shared__ float lsum[NG][16];            // probability sum of each query, at the end
   const int nqb = (a.width + QW - 1) / QW;
-  int j, h;
-  PfSpan sp;
-  if constexpr (kPacked) {
-    const PfPacked blk = pf_packed_block(a, nqb, a.H, (int)gridDim.z);
-    j = blk.j;
-    h = blk.h;
-    sp = pf_packed_span(a, h, blk.s);
-  } else {
-    const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
-    j = blk.j;
-    h = blk.h;
-    sp = pf_span<D>(a, h, blk.b);
-  }
-  const int qb = (nqb - 1 - j) * QW;  // the longest blocks first
+  const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
+  const int qb = (nqb - 1 - blk.j) * QW;  // the longest blocks first
+  const int h = blk.h, b = blk.b;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int sl = w % NSL, m = w / NSL;
-  const uint16_t* kbase = sp.k;
-  const uint16_t* vbase = sp.v;
-  const int64_t k_pos = kPacked ? a.k_pos : D, v_pos = kPacked ? a.v_pos : D;
-  const int kend = min(qb + QW, sp.nq) + sp.before;
-  if constexpr (kPacked) {
-    if (qb >= sp.nq) return;
-    if (kend <= 0) return pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + QW, sp.nq), h);
-  }
+  const int64_t slot = clamp64(a.slots[b], 0, a.cache_rows - 1);
+  const uint16_t* kbase = a.k + slot * a.s_row + h * a.s_head;
+  const uint16_t* vbase = a.v + slot * a.s_row + h * a.s_head;
+  const int kend = min(qb + QW, a.width);
   const int nt = (kend + 31) / 32;
 
   // Global -> LDS through one set of staging registers: thread tid moves 16-byte chunks tid, tid + 64 kPwWaves, ...
   // of a tile's K or V rows.  Rows past the context read its last key (finite: masked by the causal limit).
   u32x4_t stage[kChunks];
-  auto fetch = [&](int t, const uint16_t* base, int64_t pos) {
+  auto fetch = [&](int t, const uint16_t* base) {
 #pragma unroll
     for (int e = 0; e < kChunks; ++e) {
       const int ci = tid + e * 64 * kPwWaves, r = ci / kRowChunks, col = ci % kRowChunks;
-      const int key = min(t * 32 + r, sp.nk - 1);
-      stage[e] = *reinterpret_cast<const u32x4_t*>(base + (int64_t)key * pos + col * 8);
+      const int key = min(t * 32 + r, a.width - 1);
+      stage[e] = *reinterpret_cast<const u32x4_t*>(base + (int64_t)key * D + col * 8);
     }
   };
   auto put = [&](char* dst) {
@@ -313,15 +297,15 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
     }
   };
   // Whether group gi sees the tile starting at key0: a live group whose last query reaches the tile's first key.
-  auto sees = [&](int gi, int key0) { return qb + 16 * gi < sp.nq && key0 <= qb + 16 * gi + 15 + sp.before; };
+  auto sees = [&](int gi, int key0) { return qb + 16 * gi < a.width && key0 <= qb + 16 * gi + 15; };
 
   u32x4_t qop[kPwSub][4];  // lane (c, g): q[qb + 16 gi + c][128 sl + 32 s2 + 8g .. +7] (0 past the end)
   f32x4_t o[kPwSub][8];    // output column c of block e: dimension 128 sl + 16 e + c
 #pragma unroll
   for (int u = 0; u < kPwSub; ++u) {
     const int row = qb + 16 * (m + M * u) + c;
-    const bool live = row < sp.nq;
-    const uint16_t* qrow = a.q + ((sp.q0 + (live ? row : 0)) * a.H + h) * D + 128 * sl + g * 8;
+    const bool live = row < a.width;
+    const uint16_t* qrow = a.q + ((int64_t)(b * a.width + (live ? row : 0)) * a.H + h) * D + 128 * sl + g * 8;
 #pragma unroll
     for (int s2 = 0; s2 < 4; ++s2)
       qop[u][s2] = live ? *reinterpret_cast<const u32x4_t*>(qrow + s2 * 32) : u32x4_t{0u, 0u, 0u, 0u};
@@ -332,11 +316,11 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
   for (int r = 0; r < OWN; ++r) st[r] = SoftmaxState{-INFINITY, -INFINITY, 0.f};
 
-  fetch(0, kbase, k_pos);
+  fetch(0, kbase);
   put(kl);
-  fetch(0, vbase, v_pos);
+  fetch(0, vbase);
   put(vl[0]);
-  if (nt > 1) fetch(1, kbase, k_pos);
+  if (nt > 1) fetch(1, kbase);
   lds_barrier();
   for (int t = 0; t < nt; ++t) {
     const int key0 = t * 32;
@@ -368,7 +352,7 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
     lds_barrier();
     if (t + 1 < nt) {
       put(kl);             // every wave has read this tile's K
-      fetch(t + 1, vbase, v_pos);  // the next V, in flight during steps 2 and 3
+      fetch(t + 1, vbase);  // the next V, in flight during steps 2 and 3
     }
     // 2. the softmax of this wave's own groups
 #pragma unroll
@@ -386,8 +370,8 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
       float sv[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) sv[j] = sum[j >> 2][j & 3];
-      const int lim = q0 + c + 1 + sp.before;
-      if (!(key0 + 31 <= q0 + sp.before)) {  // not every query of the group sees the whole tile
+      const int lim = q0 + c + 1;
+      if (!(key0 + 31 <= q0)) {  // not every query of the group sees the whole tile
 #pragma unroll
         for (int j = 0; j < 8; ++j) sv[j] = key0 + 8 * g + j < lim ? sv[j] : -INFINITY;
       }
@@ -464,7 +448,7 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
     }
     if (t + 1 < nt) {
       put(vl[(t + 1) & 1]);  // read last by tile t - 1's P V, before this tile's first barrier
-      if (t + 2 < nt) fetch(t + 2, kbase, k_pos);
+      if (t + 2 < nt) fetch(t + 2, kbase);
     }
   }
 
@@ -481,22 +465,16 @@ __global__ __launch_bounds__(64 * kPwWaves) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
   for (int u = 0; u < kPwSub; ++u) {
     const int gi = m + M * u;
-    bool again = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int qq = qb + 16 * gi + 4 * g + i;
-      if (qq >= sp.nq) continue;
+      if (qq >= a.width) continue;
       const float li = lsum[gi][4 * g + i];
       const float div = li > 0.f ? li : 1.f;
-      uint16_t* orow = a.out + ((sp.q0 + qq) * a.H + h) * D + 128 * sl;
+      uint16_t* orow = a.out + ((int64_t)(b * a.width + qq) * a.H + h) * D + 128 * sl;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t w = pack_bf16x2(o[u][e][i] / div, 0.f);
-        orow[16 * e + c] = (uint16_t)w;
-        if constexpr (kPacked) again |= pf_nonfinite(w);
-      }
+      for (int e = 0; e < 8; ++e) orow[16 * e + c] = (uint16_t)pack_bf16x2(o[u][e][i] / div, 0.f);
     }
-    if (kPacked && __any(again)) pf_again<D>(a, sp, h, qb + 16 * gi, 1, 128 * sl);
   }
 }
 
@@ -954,8 +932,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   bring_k(at, 0);
   bool more;
   if constexpr (kPacked) {
-    // All of the start's loads at once, then waits for the first K tile (32 loads behind it) and the second (16): what
-    // the block takes before its first tile is done is 1.2 us less than one after the other.
+    // All of the start's loads at once, then waits for the first K tile (32 loads behind it) and the second (16).
     __builtin_amdgcn_sched_barrier(0);
     ahead = at;
     more = advance(ahead);
@@ -1309,6 +1286,300 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   if (kPacked && __any(again)) pf_again<D>(a, sp, h, qp, 4, 0);
 }
 
+// Packed prompts at head dim 256: 128 queries and 64-key tiles per workgroup of 8 waves, in two groups of 64 queries, of one
+// head or (grouped heads) of two that read the same keys.  Score wave w (0..3) has 32 queries, all 256 dimensions in
+// registers, and as in prefill_attn_pairs_kernel multiplies tile t beside the softmax of tile t - 1 with a reference of its
+// own; value wave w has 128 dimensions of a group's O and as in prefill_attn_ws_kernel takes V straight from memory a tile
+// ahead, two tiles behind the scores.  K goes to LDS by direct loads, two rows each, 16-byte chunk c of row r at position
+// c ^ (r % 16).  One barrier per tile.
+// What bounds a tile is what bounds prefill_attn_ws_kernel's: as many products for 3/4 of its bytes.  Measured, 16 heads
+// over 2: 8 prompts of 750-2400 186 us (729 TFLOP/s), 16 of up to 500 behind up to 900 keys 79 us; the form of
+// prefill_attn_wide_kernel (192 queries, partial scores added through LDS) 346 and 135 us.
+constexpr int kPmQ = 128, kPmK = 64, kPmD = 256;
+
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void packed_attn_mid_kernel(PrefillArgs a) {
+  constexpr int D = kPmD;
+  __shared__ __attribute__((aligned(16))) char kls[2][kPmK * D * 2];
+  __shared__ u32x4_t ps[2][4][4][64];  // [tile parity][score wave][16-key step][lane]
+  __shared__ float als[4][4][32];      // [score wave][tile % 4]: O's factors, when the reference moved
+  __shared__ int moved[4][4];
+  __shared__ float lsum[4][2][32];     // [score wave][lane half]
+  const int together = a.together, queries = kPmQ / together;
+  const int nqb = (a.width + queries - 1) / queries;
+  const PfPacked blk = pf_packed_block(a, nqb, a.H / together, (int)gridDim.z);
+  const int qb = (nqb - 1 - blk.j) * queries;  // the longest blocks first
+  const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = (w & 3) >> 1, h = blk.h * together + group % together;
+  const PfSpan sp = pf_packed_span(a, h, blk.s);
+  if (qb >= sp.nq) return;
+  const int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees
+  if (keys <= 0) {
+    for (int i = 0; i < together; ++i)
+      pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), blk.h * together + i);
+    return;
+  }
+  const int nt = (keys + kPmK - 1) / kPmK;
+  const int qp = qb + 64 * (group / together);  // the group's first query
+  // The group's last tile (-1: no queries, or they see no key).
+  const int lastk = min(qp + 64, sp.nq) - 1 + sp.before;
+  const int dq = qp < sp.nq && lastk >= 0 ? lastk / kPmK : -1;
+
+  if (w < 4) {  // ------------------------------------------------------------------------------ scores
+    const int query = qp + 32 * (w & 1) + x, whole = qp + 32 * (w & 1) + sp.before;  // all 32 see keys [0, whole]
+    u32x4_t q[D / 16];  // q[query][16s + 8g .. + 7]
+    {
+      const uint16_t* qrow = a.q + ((sp.q0 + min(query, sp.nq - 1)) * a.H + h) * D + g * 8;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4_t*>(qrow + s * 16);
+    }
+    float m_ref = -INFINITY, thr = -INFINITY, l_run = 0.f;
+    const int klane = x * (D * 2) + ((g ^ (x & 15)) * 16);
+    auto k_at = [&](int t, int m, int s) {
+      return *reinterpret_cast<const u32x4_t*>(&kls[t & 1][32 * m * (D * 2) + (klane ^ (32 * s))]);
+    };
+    typedef f32x16_t Scores[2];  // [key half m]
+    f32x16_t zero;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+    // One 16-key step's probabilities: keys 16 (2m + hf) .., as the value wave's operand.
+    auto put_p = [&](const Scores& sc, int t, int m, int hf, float mu) {
+      u32x4_t pop;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][8 * hf + 2 * e], a.scale_log2, -mu));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][8 * hf + 2 * e + 1], a.scale_log2, -mu));
+        l_run += p0 + p1;
+        pop[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
+      }
+      ps[t & 1][w][2 * m + hf][lane] = pop;
+    };
+    // The reference of tile t's scores (masked where not every query sees every key).
+    auto refer = [&](Scores& sc, int t) {
+      // max3's operands come from the matrix unit: every product has written its result after 24 wait states.
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sc[0]), "+v"(sc[1]));
+      if (t * kPmK + kPmK - 1 > whole) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const int rel = whole - t * kPmK + x - (32 * m + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[m][i] = 8 * (i >> 2) + (i & 3) <= rel ? sc[m][i] : -INFINITY;
+        }
+      }
+      float mx = max3(sc[0][0], sc[1][0], sc[0][1]);
+      mx = max3(mx, sc[1][1], sc[1][1]);
+#pragma unroll
+      for (int i = 2; i < 16; ++i) mx = max3(mx, sc[0][i], sc[1][i]);
+      const bool move = __any(mx > thr);
+      if (lane == 0) moved[w][t & 3] = move ? 1 : 0;
+      if (move) {
+        const float top = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        const float m_new = fmaxf(m_ref, top * a.scale_log2);
+        const float alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -INFINITY ? 0.f : m_new));  // m_ref = -inf: 0
+        if (g == 0) als[w][t & 3][x] = alpha;
+        l_run *= alpha;
+        m_ref = m_new;
+        thr = m_new == -INFINITY ? -INFINITY : (m_new + kWsGuard) / a.scale_log2;
+      }
+    };
+    // Step t: tile t's products into ``to``, the softmax of tile t - 1's scores ``from`` beside them.
+    auto step = [&](const Scores& from, Scores& to, int t, bool soft) {
+      u32x4_t kf[2] = {k_at(t, 0, 0), k_at(t, 1, 0)};
+      const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) to[m] = mfma32(kf[m], q[s], s == 0 ? zero : to[m]);
+        if (s + 1 < D / 16) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) kf[m] = k_at(t, m, s + 1);
+        }
+        if (soft && (s & 3) == 3) put_p(from, t - 1, s >> 3, (s >> 2) & 1, mu);
+      }
+      refer(to, t);
+    };
+    auto finish = [&](const Scores& from, int t) {  // the group's last tile
+      const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) put_p(from, t, s >> 1, s & 1, mu);
+      lsum[w][g][x] = l_run;
+    };
+    Scores sa, sb;
+    lds_barrier();  // the first K tile
+    if (dq >= 0) step(sb, sa, 0, false);
+    lds_barrier();
+    int t = 1;
+    for (; t + 1 <= dq; t += 2) {
+      step(sa, sb, t, true);
+      lds_barrier();
+      step(sb, sa, t + 1, true);
+      lds_barrier();
+    }
+    if (t <= dq) {  // one more, then its scores are in sb
+      step(sa, sb, t, true);
+      lds_barrier();
+      finish(sb, t);
+      lds_barrier();
+      t += 2;
+    } else if (dq >= 0) {
+      finish(sa, t - 1);
+      lds_barrier();
+      t += 1;
+    }
+    for (; t <= nt + 1; ++t) lds_barrier();
+    return;
+  }
+
+  // ---------------------------------------------------------------------------------------------- values
+  const int vw = w - 4, slice = 128 * (vw & 1);
+  const char* kbase = scalar_pointer(sp.k);
+  const char* vbase = scalar_pointer(sp.v);
+  f32x16_t o[2][4];  // as prefill_attn_ws_kernel's, of queries qp + 32u + x and dimensions slice ..
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
+  // K rows 16 vw .. + 15 of tile t to LDS (past the last tile: that tile again, not used); rows past the sequence read its
+  // last key (finite or masked).
+  auto bring_k = [&](int t) {
+    const int at = min(t, nt - 1), t0 = at * kPmK;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(kbase + (int64_t)t0 * sp.k_bytes), 0, -1, 0x00020000);
+#pragma unroll
+    for (int r2 = 0; r2 < 8; ++r2) {
+      const int r = 16 * vw + 2 * r2 + g;
+      const int key = min(t0 + r, sp.nk - 1) - t0;
+      const uint32_t from = (uint32_t)key * sp.k_bytes + (uint32_t)(x ^ (r & 15)) * 16;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          kr, (__attribute__((address_space(3))) void*)&kls[t & 1][(16 * vw + 2 * r2) * (D * 2)], 16, from, 0, 0, 0);
+    }
+  };
+  const uint32_t vlane = (uint32_t)(8 * (x >> 4) + 4 * g) * sp.v_bytes + (uint32_t)(slice + 8 * (x & 15)) * 2;
+  u32x4_t v[4][4];
+  auto load_v = [&](int t, int s) {  // 16-key step s of tile t; rows past the sequence read 0
+    const int at = t * kPmK + 16 * s, rows = min(sp.nk - at, 16);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(vbase + (int64_t)at * sp.v_bytes), 0, rows > 0 ? (uint32_t)(rows - 1) * sp.v_bytes + D * 2 : 0,
+        0x00020000);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[s][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, vlane + j * sp.v_bytes, 0, 0));
+  };
+  // O^T += V^T P^T for tile t, and the loads of tile ``ahead`` as its registers fall free.
+  auto attend_v = [&](int t, int ahead) {
+    u32x4_t p[2][2], vop[2][4];
+    auto read_p = [&](int s) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) p[u][s & 1] = ps[t & 1][2 * group + u][s][lane];
+    };
+    read_p(0);
+    read_p(1);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (moved[2 * group + u][t & 3]) {  // wave-uniform
+        const float al = als[2 * group + u][t & 3][x];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[u][e][i] *= al;
+      }
+    auto operands = [&](int s) {  // as prefill_attn_ws_kernel's
+      u32x2_t lo[4], hi[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const auto r = __builtin_amdgcn_permlane16_swap(v[s][j][d], v[s][j][2 + d], false, false);
+          lo[j][d] = r[0];
+          hi[j][d] = r[1];
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int q2 = 0; q2 < 2; ++q2) {
+          vop[s & 1][e][q2] = __builtin_amdgcn_perm(lo[2 * q2 + 1][e >> 1], lo[2 * q2][e >> 1], sel);
+          vop[s & 1][e][2 + q2] = __builtin_amdgcn_perm(hi[2 * q2 + 1][e >> 1], hi[2 * q2][e >> 1], sel);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(vop[s & 1][e]));  // built here, not where first used
+    };
+    operands(0);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(ahead, s);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) o[u][e] = mfma32(vop[s & 1][e], p[u][s & 1], o[u][e]);
+      if (s < 2) read_p(s + 2);
+      if (s < 3) operands(s + 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step's end: its K tile is in LDS, the 16 V loads issued after it may be on their way.
+  auto k_landed = [&]() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x4f70);  // vmcnt(16)
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  };
+  bring_k(0);
+  landed_barrier();
+  bring_k(1);
+  landed_barrier();  // step 0
+  int t = 1;
+  if (dq >= 0) {
+    bring_k(2);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) load_v(0, s);
+    k_landed();  // step 1
+    for (t = 2; t <= dq + 2; ++t) {
+      bring_k(t + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      attend_v(t - 2, min(t - 1, dq));
+      k_landed();
+    }
+  }
+  for (; t <= nt + 1; ++t) {
+    bring_k(t + 1);
+    landed_barrier();
+  }
+  bool again = false;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int query = qp + 32 * u + x;
+    if (query >= sp.nq) continue;
+    const float l = dq < 0 ? 0.f : lsum[2 * group + u][0][x] + lsum[2 * group + u][1][x];
+    const float inv = l > 0.f ? 1.f / l : 1.f;
+    uint16_t* orow = a.out + ((sp.q0 + query) * a.H + h) * D + slice + 32 * g;
+    auto pair = [&](float lo, float hi) {
+      return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
+    };
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // dimensions 64r + 32g + 8i + 4k + e, k = 0, 1
+        u32x4_t out;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = 4 * (r + 2 * k) + i;
+          out[2 * k] = pair(o[u][0][at], o[u][1][at]);
+          out[2 * k + 1] = pair(o[u][2][at], o[u][3][at]);
+        }
+        *reinterpret_cast<u32x4_t*>(orow + 64 * r + 8 * i) = out;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) again |= pf_nonfinite(out[k]);
+      }
+  }
+  if (__any(again)) pf_again<D>(a, sp, h, qp, 4, slice);
+}
+
 // Head dim 128 in blocks of 192 queries, for the launches of small_blocks: one workgroup of 4 waves, two workgroups per
 // CU.  The block's 32-key tiles go through LDS once for all of its waves (double-buffered: tile t + 1's global loads are
 // in flight during tile t's math).  Each wave holds kPfSub groups of 16 queries: per tile it reads the K fragments and,
@@ -1583,7 +1854,7 @@ extern "C" int omni_prefill_attention(const void* q, const void* k_cache, const 
   } else {
     const int qw = 16 * omni::kPwSub * (omni::kPwWaves / 2);  // queries per workgroup
     dim3 grid((width + qw - 1) / qw, heads, contexts);
-    omni::prefill_attn_wide_kernel<false><<<grid, 64 * omni::kPwWaves, 0, s>>>(a);
+    omni::prefill_attn_wide_kernel<<<grid, 64 * omni::kPwWaves, 0, s>>>(a);
   }
   return omni_launch_status();
 }
@@ -1637,9 +1908,10 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
     const dim3 grid((longest + omni::kWsQ - 1) / omni::kWsQ, heads, sequences);
     omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
   } else {
-    const int qw = 16 * omni::kPwSub * (omni::kPwWaves / 2);  // queries per workgroup
-    const dim3 grid((longest + qw - 1) / qw, heads, sequences);
-    omni::prefill_attn_wide_kernel<true><<<grid, 64 * omni::kPwWaves, 0, s>>>(a);
+    a.together = a.heads_per_kv % 2 == 0 ? 2 : 1;
+    const int queries = omni::kPmQ / a.together;
+    const dim3 grid((longest + queries - 1) / queries, heads / a.together, sequences);
+    omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
   }
   return omni_launch_status();
 }
