@@ -413,6 +413,7 @@ int omni_silu_mul(const void *gate_inner, int64_t gate_inner_stride, void *out, 
  * page table[r, p / page].  head_dim: 128, 256 or 512.  ``cache_dtype`` OMNI_BF16, or OMNI_E4M3 with ``k_scale`` /
  * ``v_scale`` [pages, kv_heads, page] bytes: a vector's values are code * 2^(byte - 127) (bytes are 1..254).
  * Two rows may share pages (a common beginning); pages and entries behind a row's positions in use are never read.
+ * A call takes up to 2^24 - 1 tokens (omni_paged_attention: queries, rows * tokens) and 4096 heads.
  */
 
 /*
@@ -420,7 +421,7 @@ int omni_silu_mul(const void *gate_inner, int64_t gate_inner_stride, void *out, 
  * head_dim] bf16 (q | k | v).  The rotated q goes to ``q_out`` [n_tokens, heads, head_dim]; the rotated k and the v of
  * token n to position cache_pos[n] (NULL: pos[n]) of cache row slots[n] (NULL: n).  Tokens whose row, position or page is
  * outside the cache are not written.  A call's (row, position) pairs are distinct: of two equal ones either token's values
- * may stay, in part.  ``k_out`` [n_tokens, kv_heads, head_dim], if not NULL, gets the rotated k in bf16 as well, for
+ * may stay, in part.  K and V have pages and exponents of their own.  ``k_out`` [n_tokens, kv_heads, head_dim], if not NULL, gets the rotated k in bf16 as well, for
  * omni_packed_attention over the same prompts.
  * OMNI_E4M3: exponent e of a vector x is the least integer with max |x| <= 448 * 2^e, over the finite x and at least -126
  * (0 for a vector of zeros); the code is x * 2^-e to the nearest e4m3, ties to even, from the rotated fp32 k (at e = 120, where
@@ -468,7 +469,8 @@ int omni_paged_attention(const void *q, const void *k_pages, const void *v_pages
  * in head_dim).  Query i of the sequence's nq sees its keys [0, i + nk - nq] of nk -- with nk > nq the prompt goes on
  * behind nk - nq earlier keys -- and none gives zeros.  ``starts`` / ``k_starts`` [sequences + 1], not decreasing; held
  * within q and k.  ``longest``: at least the longest sequence's queries (it sizes the grid; queries past it are not
- * computed).  Rows of ``out`` [queries, heads, head_dim] in no sequence are left as they are.  bf16, fp32 accumulation,
+ * computed).  Rows of ``out`` [queries, heads, head_dim] in no sequence are left as they are; ``out`` shares no memory with
+ * q, k and v.  bf16, fp32 accumulation,
  * head_dim 128, 256 or 512; heads a multiple of kv_heads; scale > 0.  No workspace.
  */
 int omni_packed_attention(const void *q, const void *k, const void *v, int64_t k_stride_pos,

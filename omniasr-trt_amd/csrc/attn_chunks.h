@@ -105,26 +105,37 @@ __device__ __forceinline__ u32x4_t tile_softmax(const f32x4_t (&acc)[2], float c
 }
 
 // A chunk of V on a tile with keys that some query does not see: their probability is 0, but 0 times an infinity or NaN of
-// V would reach the query's output, so the products run without those.  True where the lane's part held any: the caller
-// adds them to the queries that see them, whose output they make infinite or NaN whatever their weight.
+// V would reach the query's output, so the products run without those.  True where there was any: the caller adds them to
+// the queries that see them, whose output they make infinite or NaN whatever their weight.  ``vs``: e4m3, the exponent bytes
+// of the 8 keys.  A code of e4m3 is a NaN at 0x7f; with an exponent byte b above 246 it is infinite in bf16 from 2^(255-b) on,
+// the code 8 * (262 - b); with 255 (never written, but a place not written yet may hold it) all are, 0 too.
 template <bool kF8>
-__device__ __forceinline__ bool only_finite(KvChunk<kF8>& t) {
-  // An exponent of ones (e4m3: exponent and mantissa) carries into the sign's place.
-  constexpr uint32_t kField = kF8 ? 0x7f7f7f7fu : 0x7f807f80u, kOne = kF8 ? 0x01010101u : 0x00800080u;
-  constexpr uint32_t kTop = kF8 ? 0x80808080u : 0x80008000u;
+__device__ __forceinline__ bool only_finite(KvChunk<kF8>& t, u32x2_t& vs) {
+  // What, added to a magnitude that is not finite, carries into the sign's place.
+  constexpr uint32_t kField = kF8 ? 0x7f7f7f7fu : 0x7f807f80u, kTop = kF8 ? 0x80808080u : 0x80008000u;
+  auto carry = [&](int i, int w) {
+    if constexpr (!kF8) return 0x00800080u;
+    const int j = 2 * i + (w >> 1), b = (vs[j >> 2] >> (8 * (j & 3))) & 0xff;
+    return 0x01010101u * (uint32_t)(b == 255 ? 0x80 : max(8 * (b - 246), 1));
+  };
   uint32_t any = 0;
 #pragma unroll
   for (int i = 0; i < (kF8 ? 4 : 8); ++i)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) any |= (t.r[i][w] & kField) + kOne;
+    for (int w = 0; w < 4; ++w) any |= (t.r[i][w] & kField) + carry(i, w);
   if (!__any((any & kTop) != 0)) return false;
 #pragma unroll
   for (int i = 0; i < (kF8 ? 4 : 8); ++i)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const uint32_t top = ((t.r[i][w] & kField) + kOne) & kTop;
+      const uint32_t top = ((t.r[i][w] & kField) + carry(i, w)) & kTop;
       t.r[i][w] &= ~((top << 1) - (top >> (kF8 ? 7 : 15)));  // every bit of such an element
     }
+  if constexpr (kF8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (((vs[j >> 2] >> (8 * (j & 3))) & 0xff) == 0xff) vs[j >> 2] -= 0x80u << (8 * (j & 3));
+  }
   return true;
 }
 

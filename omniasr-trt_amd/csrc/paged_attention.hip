@@ -117,6 +117,8 @@ __device__ __forceinline__ PagedUnit paged_find(const PagedAttn& a, int lane, Pa
       u.from = start + u.unit * places + kPaStart;
       return u;
     }
+    // (Past the last row only where another stream changed the lengths meanwhile: no unit, so that the search ends.)
+    if (line.b0 + kWave >= a.rows) return PagedUnit{0, 0, 0, 0, x};
     ahead = line.take(a, lane, line.b0 + kWave, ahead);
   }
 }
@@ -303,13 +305,13 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
         float vscale[8];
         u32x4_t pop[NB];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vscale[j] = scale_of((t.vs[j >> 2] >> (8 * (j & 3))) & 0xffu);
-#pragma unroll
         for (int nb = 0; nb < NB; ++nb)
           pop[nb] = tile_softmax<8>(acc[nb], a.scale_log2, st[nb], o[nb], g, lim[nb] - at - 8 * g);
         // Only the wave's last tile of the unit can hold keys that a query does not see where the waves' tiles are kStep
         // apart, its last two otherwise: such keys are the last T - 1 <= 15 and the end of the last tile.
-        if (at + 31 >= p.u.n) bad |= only_finite<kF8>(t.v);
+        if (at + 31 >= p.u.n) bad |= only_finite<kF8>(t.v, t.vs);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vscale[j] = scale_of((t.vs[j >> 2] >> (8 * (j & 3))) & 0xffu);
         chunk_values<kF8, NB>(t.v, pop, vscale, o);
       }
       load_v_chunk<kF8, kRowB>(t.v, vrow);
@@ -328,16 +330,20 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
         }
       }
     }
-    if (__any(bad)) {  // infinities and NaN of V that the products of the last tiles left out
+    if (__any(bad)) {  // infinities and NaN of V that the products of the last tiles left out (the ballot keeps it one branch)
       for (int i = max(p.mine - 2, 0); i < p.mine; ++i) {
         const int at = (p.first + kStep * i) * 32;
         if (at + 31 < p.u.n) continue;
         for (int key = at; key < min(at + 32, p.last); ++key) {
-          const int64_t row = (cell(p, key >> 3, page_of(p, key >> 3)) + (key & 7)) * D + 128 * sl + 8 * c;
+          const int64_t at_cell = cell(p, key >> 3, page_of(p, key >> 3)) + (key & 7), row = at_cell * D + 128 * sl + 8 * c;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float v = kF8 ? ((a.cache.v[row + e] & 0x7f) == 0x7f ? NAN : 0.f)
-                                : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.cache.v)[row + e]);
+            float v;
+            if constexpr (kF8) {
+              v = __builtin_amdgcn_cvt_f32_fp8((uint8_t)a.cache.v[row + e], 0) * scale_of(a.cache.v_scale[at_cell]);
+            } else {
+              v = bf16_to_f32(reinterpret_cast<const uint16_t*>(a.cache.v)[row + e]);
+            }
             if (v - v == 0.f) continue;  // finite
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -555,7 +561,7 @@ extern "C" int omni_paged_attention(const void* q, const void* k_pages, const vo
   if (status != OMNI_OK) return status;
   if (pages == 0 || width == 0) return OMNI_ERR_INVALID;
   if (!q || !lengths || !out || (((uintptr_t)q | (uintptr_t)out) & 15u)) return OMNI_ERR_INVALID;
-  if (rows > 65535) return OMNI_ERR_SHAPE;
+  if ((int64_t)rows * tokens > 0xffffff) return OMNI_ERR_SHAPE;  // the second launch's threads along x: 256 to a query
   if (!workspace || ((uintptr_t)workspace & 255u) ||
       workspace_bytes < omni_paged_attention_workspace(rows, tokens, heads, kv_heads, head_dim, page, width))
     return OMNI_ERR_WORKSPACE;

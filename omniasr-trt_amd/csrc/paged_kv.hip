@@ -171,6 +171,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead r, PagedCache
 
 using namespace omni;
 
+constexpr int64_t kPagedTokens = 0xffffff;  // a launch's threads, 256 to a token at most, are counted in 32 bits
+
 // The instance of ``kernel`` for a head dim and cache type, with whole waves for a token's ``vectors``, four at most.
 #define OMNI_PAGED_LAUNCH(kernel, head_dim, vectors, f8, grid, stream, ...)                         \
   do {                                                                                              \
@@ -195,12 +197,13 @@ extern "C" int omni_rope_kv_paged(const void* qkv, int64_t qkv_row_stride, const
                                   int64_t rows, int32_t width, int64_t n_tokens, int32_t heads, int32_t kv_heads,
                                   int32_t head_dim, int32_t cache_dtype, int32_t dtype, void* stream) {
   if (dtype != OMNI_BF16) return OMNI_ERR_DTYPE;
-  if (n_tokens < 0 || n_tokens > 0x7fffffffLL || heads <= 0 || kv_heads <= 0) return OMNI_ERR_INVALID;
+  if (n_tokens < 0 || heads <= 0 || kv_heads <= 0) return OMNI_ERR_INVALID;
   if (n_tokens == 0) return OMNI_OK;
   const int status = omni_check_pages(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, head_dim, table,
                                       table_stride, rows, width, cache_dtype);
   if (status != OMNI_OK) return status;
-  if (heads > 4096 || kv_heads > 4096) return OMNI_ERR_SHAPE;
+  if (heads > 4096 || kv_heads > 4096 || n_tokens > kPagedTokens) return OMNI_ERR_SHAPE;
+  if (k_pages == v_pages || (k_scale && k_scale == v_scale)) return OMNI_ERR_INVALID;  // two vectors for one place
   if (!qkv || !cs || !pos || !q_out || cs_rows <= 0) return OMNI_ERR_INVALID;
   if (((uintptr_t)qkv | (uintptr_t)cs | (uintptr_t)q_out | (uintptr_t)k_out) & 15u) return OMNI_ERR_INVALID;
   if (qkv_row_stride % 8 || qkv_row_stride < (heads + 2LL * kv_heads) * head_dim) return OMNI_ERR_INVALID;
@@ -218,12 +221,12 @@ extern "C" int omni_paged_read(const void* k_pages, const void* v_pages, const v
                                int32_t width, const int64_t* slots, const int64_t* pos, int64_t n_tokens,
                                int32_t kv_heads, int32_t head_dim, int32_t cache_dtype, void* k_out, void* v_out,
                                void* stream) {
-  if (n_tokens < 0 || n_tokens > 0x7fffffffLL || kv_heads <= 0) return OMNI_ERR_INVALID;
+  if (n_tokens < 0 || kv_heads <= 0) return OMNI_ERR_INVALID;
   if (n_tokens == 0) return OMNI_OK;
   const int status = omni_check_pages(k_pages, v_pages, k_scale, v_scale, pages, page, kv_heads, head_dim, table,
                                       table_stride, rows, width, cache_dtype);
   if (status != OMNI_OK) return status;
-  if (kv_heads > 4096) return OMNI_ERR_SHAPE;
+  if (kv_heads > 4096 || n_tokens > kPagedTokens) return OMNI_ERR_SHAPE;
   if (!slots || !pos || !k_out || !v_out || (((uintptr_t)k_out | (uintptr_t)v_out) & 15u)) return OMNI_ERR_INVALID;
   const PagedRead r{slots, pos, (uint16_t*)k_out, (uint16_t*)v_out};
   const PagedCache a =

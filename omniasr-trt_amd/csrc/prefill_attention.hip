@@ -192,7 +192,8 @@ __device__ __noinline__ void pf_again_16(const uint16_t* q, const uint16_t* k, c
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       vt.r[j] = ld16(reinterpret_cast<const char*>(v + min(t + 8 * g + j, nk - 1) * v_pos + 8 * c));
-    if (t + 31 > whole && __any(only_finite<false>(vt))) {
+    u32x2_t none = {0u, 0u};
+    if (t + 31 > whole && only_finite<false>(vt, none)) {
       for (int key = t; key < min(t + 32, end); ++key)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -1898,20 +1899,16 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
   a.v_pos = v_stride_pos;
   a.v_head = v_stride_head;
   a.heads_per_kv = heads / kv_heads;
+  a.together = 1;
+  if (head_dim == 128) a.together = a.heads_per_kv % 4 == 0 ? 4 : a.heads_per_kv % 2 == 0 ? 2 : 1;
+  if (head_dim == 256) a.together = a.heads_per_kv % 2 == 0 ? 2 : 1;
+  const int rows = (head_dim == 128 ? omni::kPairQ : head_dim == 256 ? omni::kPmQ : omni::kWsQ) / a.together;
+  const dim3 grid((longest + rows - 1) / rows, heads / a.together, sequences);
+  // The blocks are counted in 31 bits, a launch's threads along x, 512 to a block, in 32.
+  if (grid.x >= (1u << 23) || (int64_t)grid.x * grid.y * grid.z > 0x7fffffffLL) return OMNI_ERR_SHAPE;
   const hipStream_t s = (hipStream_t)stream;
-  if (head_dim == 128) {
-    a.together = a.heads_per_kv % 4 == 0 ? 4 : a.heads_per_kv % 2 == 0 ? 2 : 1;
-    const int queries = omni::kPairQ / a.together;
-    const dim3 grid((longest + queries - 1) / queries, heads / a.together, sequences);
-    omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
-  } else if (head_dim == 512) {
-    const dim3 grid((longest + omni::kWsQ - 1) / omni::kWsQ, heads, sequences);
-    omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
-  } else {
-    a.together = a.heads_per_kv % 2 == 0 ? 2 : 1;
-    const int queries = omni::kPmQ / a.together;
-    const dim3 grid((longest + queries - 1) / queries, heads / a.together, sequences);
-    omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
-  }
+  if (head_dim == 128) omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
+  else if (head_dim == 256) omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
+  else omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
   return omni_launch_status();
 }

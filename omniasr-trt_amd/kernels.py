@@ -694,7 +694,8 @@ def rope_kv_paged(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     that is to page ``table[slots[n], position // page]`` of ``k_pages`` / ``v_pages`` [pages, kv heads, page, D].  Tokens
     whose row, position or page is outside the cache (a negative row marks padding) are not written; the (row, position)
     pairs of a call are distinct.  Returns the rotated q [N, heads, D]; with ``rotated`` also the rotated k
-    [N, kv heads, D], which :func:`packed_attention` takes beside the v in ``qkv``.
+    [N, kv heads, D], which :func:`packed_attention` takes beside the v in ``qkv``.  K and V have
+    pages (and exponents) of their own.
 
     Pages are bf16, or float8_e4m3fn with ``k_scale`` / ``v_scale`` [pages, kv heads, page] uint8: a vector x is kept as
     the e4m3 nearest to x * 2^-e, and the byte e + 127, e the least integer with max |x| <= 448 * 2^e."""
@@ -776,6 +777,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory between the first and last elements of two tensors overlaps."""
+    if not a.numel() or not b.numel():
+        return False
+    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
+    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, longest: int,
                      scale: float, *, k_starts: torch.Tensor | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:
@@ -784,7 +793,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     is queries ``starts[s]`` .. ``starts[s + 1] - 1`` and keys ``k_starts[s]`` .. (default: ``starts``), both [S + 1]
     int64, not decreasing.  Query i of its nq sees keys [0, i + nk - nq] of its nk: with more keys than queries the prompt
     goes on behind earlier positions (:func:`paged_read`).  No key gives zeros.  ``longest``: at least the queries of the
-    longest sequence.  Returns ``out`` [N, H, D] (new by default); rows in no sequence are left as they are in it."""
+    longest sequence.  Returns ``out`` [N, H, D] (new by default, memory of its own otherwise); rows in no sequence are
+    left as they are in it."""
     lib = _lib.load()
     if q.dim() != 3 or q.dtype is not _BF16 or q.size(2) not in _HEAD_DIMS or not q.is_contiguous():
         raise ValueError("q: contiguous bf16 [N, H, D], D = 128, 256 or 512")
@@ -809,6 +819,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not _BF16 or out.get_device() != device or not out.is_contiguous():
         raise ValueError("out: contiguous, q's shape, dtype and device")
+    elif any(_share_memory(out, t) for t in (q, k, v)):
+        raise ValueError("out: memory of its own, not q's, k's or v's")
     _call(device, "packed attention", lib.omni_packed_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pos, k_head,
           v_pos, v_head, starts.data_ptr(), k_starts.data_ptr(), bounds - 1, n, m, min(longest, n), heads, kv, dim, scale,
           out.data_ptr(), _lib.BF16)

@@ -107,9 +107,18 @@ def test_call_refusals():
     _refused(kernels.packed_attention, "on the GPU", q, kk, kk, starts, 3, 0.1)
 
 
+def test_shared_memory_of_tensors():
+    x = torch.zeros(6, 4, 8)
+    assert kernels._share_memory(x, x) and kernels._share_memory(x[2:4], x[3:]) and kernels._share_memory(x[3:], x[:, :1])
+    assert not kernels._share_memory(x[:3], x[3:]) and not kernels._share_memory(x[3:], x[:3])
+    assert not kernels._share_memory(x[0, :2], x[0, 2:]) and not kernels._share_memory(x, x[:0])
+    assert not kernels._share_memory(x, torch.zeros_like(x))
+
+
 def test_c_abi_refusals_before_launch():
     lib = _lib.load()
-    pages = [FAKE, FAKE, FAKE, FAKE, 64, 16, FAKE, 8]  # k, v, scales, pages, page, table, its row stride
+    other = [ctypes.c_void_p(0x10000 * i) for i in (2, 3, 4)]
+    pages = [FAKE, *other, 64, 16, FAKE, 8]  # k, v, scales, pages, page, table, its row stride
     rope = [FAKE, 1024, FAKE, 8192, FAKE, None, None, FAKE, None, *pages, 3, 8, 5, 4, 2, 128, _lib.E4M3, _lib.BF16, None]
 
     def changed(args, at, value):
@@ -123,10 +132,14 @@ def test_c_abi_refusals_before_launch():
     assert lib.omni_rope_kv_paged(*changed(rope, 1, 1016)) == -1  # a row shorter than its vectors
     assert lib.omni_rope_kv_paged(*changed(rope, 16, 7)) == -1  # table rows shorter than their width
     assert lib.omni_rope_kv_paged(*changed(rope, 19, 0)) == 0
+    assert lib.omni_rope_kv_paged(*changed(rope, 10, FAKE)) == -1  # K and V in the same pages
+    assert lib.omni_rope_kv_paged(*changed(rope, 12, rope[11])) == -1
+    assert lib.omni_rope_kv_paged(*changed(rope, 19, 2 ** 24)) == -3
     read = [*pages, 3, 8, FAKE, FAKE, 5, 2, 128, _lib.E4M3, FAKE, FAKE, None]
     assert lib.omni_paged_read(*changed(read, 5, 512)) == -3
     assert lib.omni_paged_read(*changed(read, 10, None)) == -1
     assert lib.omni_paged_read(*changed(read, 12, 0)) == 0
+    assert lib.omni_paged_read(*changed(read, 12, 2 ** 24)) == -3
     ws = lib.omni_paged_attention_workspace(3, 2, 4, 2, 128, 16, 8)
     assert ws > 0
     attn = [FAKE, *pages, 8, FAKE, 3, 2, 4, 2, 128, 0.1, FAKE, FAKE, ws, _lib.E4M3, _lib.BF16, None]
@@ -137,6 +150,7 @@ def test_c_abi_refusals_before_launch():
     assert lib.omni_paged_attention(*changed(attn, 19, ws - 1)) == -4
     assert lib.omni_paged_attention(*changed(attn, 18, ctypes.c_void_p(0x10010))) == -4
     assert lib.omni_paged_attention(*changed(attn, 11, 0)) == 0
+    assert lib.omni_paged_attention(*changed(attn, 11, 2 ** 23)) == -3
     packed = [FAKE, FAKE, FAKE, 256, 128, 256, 128, FAKE, FAKE, 2, 9, 9, 5, 4, 2, 128, 0.1, FAKE, _lib.BF16, None]
     assert lib.omni_packed_attention(*changed(packed, 18, _lib.F32)) == -2
     assert lib.omni_packed_attention(*changed(packed, 15, 64)) == -3
@@ -144,3 +158,7 @@ def test_c_abi_refusals_before_launch():
     assert lib.omni_packed_attention(*changed(packed, 16, -1.0)) == -1
     assert lib.omni_packed_attention(*changed(packed, 1, ctypes.c_void_p(0x10008))) == -1
     assert lib.omni_packed_attention(*changed(packed, 9, 0)) == 0
+    assert lib.omni_packed_attention(*changed(packed, 9, 65536)) == -3
+    big = [*packed[:9], 65535, 2 ** 30, 2 ** 30, 2 ** 24, 4, 4, 512, *packed[16:]]  # 65535 x 2^18 x 4 blocks
+    assert lib.omni_packed_attention(*big) == -3
+    assert lib.omni_packed_attention(*big[:9], 1, 2 ** 30, 2 ** 30, 2 ** 30, 4, 1, 128, *big[16:]) == -3  # 2^25 along x

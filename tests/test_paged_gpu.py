@@ -42,7 +42,8 @@ def close(got, want, size, q, k, scale):
 
 def make_cache(cuda, g, kv, dim, page, reach, fp8, spare=5, shared=0):
     """Pages of random keys for rows of ``reach`` positions, in random order; the rest of the pool and of the last pages
-    holds NaN, the table behind a row's pages is out of range; the first ``shared`` pages of row 1 are row 0's."""
+    holds NaN (e4m3: or, on odd pages, finite codes with exponents that make them infinite or NaN), the table behind a
+    row's pages is out of range; the first ``shared`` pages of row 1 are row 0's."""
     need = [-(-n // page) for n in reach]
     pool = sum(need) + spare
     order = torch.randperm(pool, generator=g)
@@ -65,6 +66,11 @@ def make_cache(cuda, g, kv, dim, page, reach, fp8, spare=5, shared=0):
         if fp8:
             values, byte = op.quantise(x.to(BF).float())
             codes = (values / torch.exp2(byte.double() - 127)[..., None]).float().to(torch.float8_e4m3fn)
+            unused = x[..., 0].isnan()
+            unused[::2] = False
+            codes.view(torch.uint8)[unused] = 0x7E
+            byte[unused] = 254
+            byte[1::4] = torch.where(unused[1::4], torch.full_like(byte[1::4], 255), byte[1::4])
             scales[name] = byte.to(cuda)
             out.append(codes.to(cuda))
         else:
@@ -227,6 +233,26 @@ def test_paged_attention_many_columns(cuda, tokens):
     attention_case(cuda, 3, 1, 512, 16, tokens, [130, 2], True, tokens + 2)
 
 
+def test_paged_attention_of_a_layer_of_a_pool(cuda):
+    """Pages that are one layer of a stack, a table that is a part of a wider one, and more rows in it than are asked."""
+    g, layers, page, dim = gen(33), 3, 32, 128
+    for fp8 in (True, False):
+        k, v, table, scales = make_cache(cuda, g, 2, dim, page, [100, 7, 260], fp8)
+        stack = [torch.stack([torch.zeros_like(x.view(torch.uint8)), x.view(torch.uint8), torch.zeros_like(x.view(torch.uint8))])
+                 .view(x.dtype) for x in (k, v)]
+        wide = torch.full((5, table.size(1) + 9), 2 ** 30, dtype=torch.int32, device=cuda)
+        wide[:3, 4:4 + table.size(1)] = table
+        part = wide[:, 4:4 + table.size(1)]
+        q, n = normal((2, 4, dim), g, cuda), torch.tensor([100, 7], device=cuda)
+        out = kernels.paged_attention(q, stack[0][1], stack[1][1], part, n, 1, 0.1, **scales)
+        same = kernels.paged_attention(q, k, v, table, n, 1, 0.1, **scales)
+        at = torch.tensor([99, 0, 6, 259, 300], device=cuda), torch.tensor([0, 0, 1, 2, 2], device=cuda)
+        one = kernels.paged_read(stack[0][1], stack[1][1], part, at[1], at[0], **scales)
+        two = kernels.paged_read(k, v, table, at[1], at[0], **scales)
+        torch.cuda.synchronize()
+        assert torch.equal(out, same) and all(torch.equal(a[:4], b[:4]) for a, b in zip(one, two))
+
+
 def test_paged_attention_of_long_rows_and_many_rows(cuda):
     attention_case(cuda, 2, 1, 128, 256, 1, [8188], True, 1)
     attention_case(cuda, 2, 2, 128, 64, 1, [8188, 5, 1433], False, 2)
@@ -292,6 +318,21 @@ def test_paged_attention_does_not_see_what_is_masked(cuda, dim, fp8):
           torch.full((1, dim), 4.0, device=cuda), dim ** -0.5)
 
 
+def test_paged_attention_of_values_whose_exponent_makes_them_infinite(cuda):
+    """A key of the step that an earlier query does not see has v = 448 * 2^127, which is infinite."""
+    g, n, tokens = gen(21), 40, 3
+    k, v, table, scales = make_cache(cuda, g, 1, 128, 16, [n + tokens - 1], True)
+    q = normal((tokens, 2, 128), g, cuda)
+    page, off = op.cell(table, 16, k.size(0), 0, n)
+    v.view(torch.uint8)[page, 0, off, 9] = 0x7E
+    scales["v_scale"][page, 0, off] = 254
+    out = kernels.paged_attention(q, k, v, table, torch.tensor([n], device=cuda), tokens, 0.1, **scales)
+    torch.cuda.synchronize()
+    assert out[0].isfinite().all() and out[1:, :, 9].isposinf().all()
+    want, size = op.paged_attention(q[:1], k, v, table, [n], 1, 0.1, **scales)
+    close(out[:1], want, size, q, torch.full((1, 128), 4.0, device=cuda), 0.1)
+
+
 # ---------------------------------------------------------------------------------------------- packed attention
 
 def packed_case(cuda, heads, kv, dim, queries, past, seed, longest=None, behind=0, strided=True, scale=None):
@@ -350,6 +391,66 @@ def test_packed_attention_with_large_scores(cuda):
     packed_case(cuda, 2, 1, 512, [200], 50, 9, scale=1.0)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 128), (32, 8, 128), (8, 8, 512), (16, 2, 256), (8, 8, 256)])
+def test_packed_attention_head_counts(cuda, heads, kv, dim):
+    """Two query heads to a block, and the order of blocks for head counts that are multiples of 8."""
+    packed_case(cuda, heads, kv, dim, [70, 1, 0, 150], [0, 40, 3, 9], heads + kv)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 128), (8, 8, 128), (2, 1, 256), (2, 1, 512)])
+def test_packed_attention_more_sequences_than_are_ranked(cuda, heads, kv, dim):
+    packed_case(cuda, heads, kv, dim, [(13 * i) % 70 for i in range(67)], [(7 * i) % 11 for i in range(67)], dim + heads)
+
+
+def test_packed_attention_strides_and_layers(cuda):
+    """K and V as slices of wide rows, and of a stack of layers."""
+    g, heads, kv, n = gen(31), 4, 2, 150
+    starts = torch.tensor([0, 90, n], device=cuda)
+    for dim in (128, 256, 512):
+        say("packed attention of slices", dim)
+        q = normal((n, heads, dim), g, cuda)
+        wide = normal((n, 3 * kv, 2 * dim + 8), g, cuda)
+        stack = normal((3, kv, n, dim), g, cuda)
+        for k, v in ((wide[:, ::3, :dim], wide[:, 1::3, dim + 8:]), (stack[1].transpose(0, 1), stack[2].transpose(0, 1))):
+            out = kernels.packed_attention(q, k, v, starts, 90, dim ** -0.5)
+            torch.cuda.synchronize()
+            want, size = op.packed_attention(q, k, v, starts.tolist(), starts.tolist(), dim ** -0.5)
+            close(out, want, size, q, k, dim ** -0.5)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (4, 2, 256), (2, 2, 512)])
+def test_packed_attention_captured(cuda, heads, kv, dim):
+    """A captured call reads the starts of the replay; lengths and contents change between replays."""
+    g = gen(dim + 3)
+    q, k, v = (normal((300, h, dim), g, cuda) for h in (heads, kv, kv))
+    starts, k_starts = torch.zeros(4, dtype=torch.long, device=cuda), torch.zeros(4, dtype=torch.long, device=cuda)
+    out = torch.empty_like(q)
+    graphs = batching.GraphCache(cuda, True)
+    run = graphs.runner("packed", lambda: kernels.packed_attention(q, k, v, starts, 200, 0.1, k_starts=k_starts, out=out),
+                        lambda: [])
+    for counts, past in (([100, 0, 200], [0, 0, 0]), ([1, 60, 30], [20, 100, 0]), ([200, 3, 7], [-50, 9, 30])):
+        starts.copy_(torch.tensor([0, *counts]).cumsum(0))
+        k_starts.copy_(torch.tensor([0, *(a + b for a, b in zip(counts, past))]).cumsum(0))
+        q.copy_(normal(q.shape, g, cuda))
+        out.fill_(5.0)
+        run()
+        torch.cuda.synchronize()
+        used = int(starts[-1])
+        eager = kernels.packed_attention(q, k, v, starts, 200, 0.1, k_starts=k_starts)
+        torch.cuda.synchronize()
+        assert torch.equal(out[:used], eager[:used]) and (out[used:] == 5.0).all()
+        want, size = op.packed_attention(q, k, v, starts.tolist(), k_starts.tolist(), 0.1)
+        close(out[:used], want[:used], size[:used], q, k, 0.1)
+
+
+def test_packed_attention_into_its_inputs_is_refused(cuda):
+    x = normal((40, 4, 128), gen(1), cuda)
+    starts = torch.tensor([0, 20], device=cuda)
+    for out in (x[:20], x[20:]):
+        with pytest.raises(ValueError, match="memory of its own"):
+            kernels.packed_attention(x[:20], x[20:], x[20:], starts, 20, 0.1, out=out)
+
+
 def test_packed_attention_nothing(cuda):
     q = torch.zeros(4, 2, 128, dtype=BF, device=cuda)
     k = torch.zeros(0, 2, 128, dtype=BF, device=cuda)
@@ -361,10 +462,10 @@ def test_packed_attention_nothing(cuda):
     assert (kernels.packed_attention(q, q, q, none, 0, 0.1, out=full) == 3).all()
 
 
-@pytest.mark.parametrize("dim", [128, 256, 512])
-def test_packed_attention_does_not_see_what_is_masked(cuda, dim):
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 128), (4, 1, 128), (1, 1, 128), (2, 1, 256), (1, 1, 256), (2, 1, 512)])
+def test_packed_attention_does_not_see_what_is_masked(cuda, heads, kv, dim):
     """NaN and infinities in later positions of a prompt, and in its neighbours, do not reach the queries before them."""
-    g, heads, kv = gen(dim + 1), 2, 1
+    g = gen(dim + 1)
     q, k, v = (normal((230, h, dim), g, cuda) for h in (heads, kv, kv))
     starts = torch.tensor([0, 100, 230], device=cuda)
     k[90, 0, 3], v[95, 0, 7], v[96, 0, 100], v[100] = float("nan"), float("inf"), float("nan"), float("nan")
