@@ -253,6 +253,31 @@ def test_paged_attention_of_a_layer_of_a_pool(cuda):
         assert torch.equal(out, same) and all(torch.equal(a[:4], b[:4]) for a, b in zip(one, two))
 
 
+@pytest.mark.parametrize("fp8", [True, False])
+def test_a_pool_past_32_bits(cuda, fp8):
+    """Pages whose elements lie past 2^31: written, read and attended to as in a small pool."""
+    g, heads, kv, dim, page, n = gen(34), 4, 2, 512, 256, 300
+    pool = 2 ** 31 // (kv * page * dim) + 9
+    far = torch.tensor([[pool - 1, pool - 3], [pool - 4, pool - 8]], dtype=torch.int32, device=cuda)
+    near = torch.tensor([[0, 2], [3, 1]], dtype=torch.int32, device=cuda)
+    slots = torch.arange(2, device=cuda).repeat_interleave(n)
+    pos = torch.arange(n, device=cuda).repeat(2)
+    qkv = normal((2 * n, (heads + 2 * kv) * dim), g, cuda)
+    cs = modeling.rope_table(modeling.DecoderConfig(model_dim=heads * dim, num_heads=heads, max_seq_len=512)).to(cuda)
+    got = []
+    for table, size in ((far, pool), (near, 4)):
+        say("a pool of", size, "pages")
+        k, v = (torch.empty(size, kv, page, dim, device=cuda, dtype=torch.float8_e4m3fn if fp8 else BF) for _ in "kv")
+        scales = {a: torch.empty(size, kv, page, dtype=torch.uint8, device=cuda) for a in ("k_scale", "v_scale")} if fp8 else {}
+        q = kernels.rope_kv_paged(qkv, cs, pos, k, v, table, heads, slots, **scales)
+        kk, vv = kernels.paged_read(k, v, table, slots, pos, **scales)
+        lengths = torch.tensor([n, 17], device=cuda)
+        out = kernels.paged_attention(q[:2], k, v, table, lengths, 1, 0.05, **scales)
+        got.append((q, kk, vv, out))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_paged_attention_of_long_rows_and_many_rows(cuda):
     attention_case(cuda, 2, 1, 128, 256, 1, [8188], True, 1)
     attention_case(cuda, 2, 2, 128, 64, 1, [8188, 5, 1433], False, 2)
@@ -441,6 +466,22 @@ def test_packed_attention_captured(cuda, heads, kv, dim):
         assert torch.equal(out[:used], eager[:used]) and (out[used:] == 5.0).all()
         want, size = op.packed_attention(q, k, v, starts.tolist(), k_starts.tolist(), 0.1)
         close(out[:used], want[:used], size[:used], q, k, 0.1)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 128), (4, 4, 256), (2, 2, 512)])
+def test_packed_attention_past_32_bits(cuda, heads, kv, dim):
+    """Sequences whose rows of q, k, v and out lie past 2^31 elements."""
+    g, used = gen(dim + 4), 200
+    n = 2 ** 31 // (heads * dim) + used
+    q, k, v = (torch.empty(n, heads, dim, dtype=BF, device=cuda) for _ in "qkv")
+    for x in (q, k, v):
+        x[-used:] = normal((used, heads, dim), g, cuda)
+    out = torch.empty_like(q)
+    starts = torch.tensor([0, 150, used], device=cuda)
+    kernels.packed_attention(q, k, v, starts + (n - used), 150, 0.1, out=out)
+    near = kernels.packed_attention(q[-used:], k[-used:], v[-used:], starts, 150, 0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(out[-used:], near)
 
 
 def test_packed_attention_into_its_inputs_is_refused(cuda):
