@@ -463,6 +463,13 @@ int omni_paged_attention(const void *q, const void *k_pages, const void *v_pages
                          int32_t dtype, void *stream);
 
 /*
+ * Bytes of workspace omni_packed_attention needs: 0 but for few queries behind many keys.  ``keys``: as for the call, or
+ * ``longest``, if less, where ``k_starts`` is ``starts``.
+ */
+size_t omni_packed_attention_workspace(int32_t sequences, int64_t keys, int32_t longest, int32_t heads,
+                                       int32_t kv_heads, int32_t head_dim);
+
+/*
  * Causal attention of packed prompts of different lengths (omni_prefill_attention without the padding, over keys that
  * need not be in a cache).  Sequence s: queries starts[s] .. starts[s+1]-1 of ``q`` [queries, heads, head_dim], keys
  * k_starts[s] .. k_starts[s+1]-1 of ``k`` / ``v`` [keys, kv_heads, head_dim] (element strides, multiples of 8, unit stride
@@ -471,13 +478,15 @@ int omni_paged_attention(const void *q, const void *k_pages, const void *v_pages
  * within q and k.  ``longest``: at least the longest sequence's queries (it sizes the grid; queries past it are not
  * computed).  Rows of ``out`` [queries, heads, head_dim] in no sequence are left as they are; ``out`` shares no memory with
  * q, k and v.  bf16, fp32 accumulation,
- * head_dim 128, 256 or 512; heads a multiple of kv_heads; scale > 0.  No workspace.
+ * head_dim 128, 256 or 512; heads a multiple of kv_heads; scale > 0.  ``workspace``:
+ * omni_packed_attention_workspace() bytes, 256-byte aligned, any content.  Results do not depend on timing.
  */
 int omni_packed_attention(const void *q, const void *k, const void *v, int64_t k_stride_pos,
                           int64_t k_stride_head, int64_t v_stride_pos, int64_t v_stride_head,
                           const int64_t *starts, const int64_t *k_starts, int32_t sequences,
                           int64_t queries, int64_t keys, int32_t longest, int32_t heads, int32_t kv_heads,
-                          int32_t head_dim, float scale, void *out, int32_t dtype, void *stream);
+                          int32_t head_dim, float scale, void *out, void *workspace, size_t workspace_bytes,
+                          int32_t dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -75,8 +75,10 @@ _SIGNATURES = {
     "omni_paged_attention_workspace": (c_size_t, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "omni_paged_attention": (c_int, [_P, _P, _P, _P, _P, c_int32, c_int32, _P, c_int64, c_int32, _P, c_int32, c_int32,
                                      c_int32, c_int32, c_int32, c_float, _P, _P, c_size_t, c_int32, c_int32, _P]),
+    "omni_packed_attention_workspace": (c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32, c_int32]),
     "omni_packed_attention": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int32, c_int64,
-                                      c_int64, c_int32, c_int32, c_int32, c_int32, c_float, _P, c_int32, _P]),
+                                      c_int64, c_int32, c_int32, c_int32, c_int32, c_float, _P, _P, c_size_t, c_int32,
+                                      _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -18,6 +18,7 @@ namespace omni {
 // Query p of context b attends to keys [0, p] of its cache row; one workgroup per (query block, head, context), the
 // longest blocks first; every kernel keeps a lazy softmax reference and masks only the tiles on the diagonal.
 typedef short v4i16_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) v4i16_t lds_v4i16;
 typedef __attribute__((address_space(3))) const char lds_char;
 
@@ -38,7 +39,12 @@ struct PrefillArgs {
   int64_t k_pos = 0, k_head = 0, v_pos = 0, v_head = 0;
   int heads_per_kv = 1;
   int together = 1;  // head dims 128 and 256: heads of a kv head in one block (1, 2 or 4)
+  // Blocks in parts (pf_part): at most ``parts``, each with room for its O and its queries' (m, l).
+  int parts = 1;
+  float* part_o = nullptr;   // [part][value wave][query half u][r][e][k][lane][4]
+  float* part_ml = nullptr;  // [part][score wave][lane half][query][2]
 };
+constexpr int kPartO = 4 * 32 * 256, kPartMl = 4 * 2 * 64 * 2;  // floats
 
 // A context's or sequence's part of a call for one head: queries q0 .. q0 + nq - 1, keys 0 .. nk - 1 of k / v, rows
 // k_bytes / v_bytes apart; query i sees keys [0, i + before].
@@ -119,12 +125,34 @@ __device__ __forceinline__ int64_t pf_readlane64(int64_t v, int lane) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
+// Few blocks behind many keys: the longest block is the launch, ~1.05 us for each of its 64-key tiles, while other CUs have
+// nothing.  So a block is cut along its keys into parts, each a workgroup's, and a second launch (packed_attn_join_kernel)
+// joins their (O, m, l).  A part costs its start and end (~8 us) and 128 KB of O written and read, the join ~3 us: parts of
+// kPartLeast tiles and more, blocks of two such at least, at most kPartMost parts.  Measured, us, whole and in parts: 20
+// queries behind 4000 keys, 8 heads x 512 72 / 41, 32 over 8 x 128 75 / 40, 16 over 2 x 256 71 / 39; 64 behind 8000, 8 x 512
+// 179 / 66; 500 behind 6000, 8 x 512 139 / 78, 32 over 8 x 128 123 / 70.  Parts of 2 tiles and more: 20 behind 1500 33 / 30,
+// but one prompt of 1433 45 / 57, four of 200-800 28 / 46.
+constexpr int kPartCus = 256, kPartLeast = 12, kPartMost = 16;
+
 // The sequence of rank r by work (queries x keys, less what causality hides), the most first: so the last blocks of a
 // launch, whose CUs wait for each other, are the short ones.  Past 64 sequences, the order of the call.
-__device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequences, int r) {
+// ``share``, where blocks (of ``queries``, ``heads`` for each) may be in parts: the key tiles of a part, an even one of
+// about what all blocks have for each CU.
+__device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequences, int r, int queries, int heads,
+                                                int& share) {
   if (sequences > kWave) return pf_sequence(a, r);
   const int lane = lane_id();
   const PfSequence mine = pf_sequence(a, min(lane, sequences - 1));
+  if (a.parts > 1) {
+    const int nq = min(mine.nq, a.width), blocks = (nq + queries - 1) / queries;
+    const int64_t mean = ((int64_t)min(nq, queries) + mine.nk - mine.nq + mine.nk) / 2;  // keys of a block, about
+    const int64_t tiles = mean > 0 ? blocks * ((mean + 63) / 64) : 0;
+    int all = lane < sequences ? (int)(tiles < 65536 ? tiles : 65536) : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, kWave);
+    all = __builtin_amdgcn_readfirstlane(all);
+    share = max((int)(((uint32_t)all * (uint32_t)heads + kPartCus - 1) / kPartCus), kPartLeast);
+  }
   const float work = lane < sequences ? (float)mine.nq * (2.f * (float)mine.nk - (float)mine.nq) : -INFINITY;
   int rank = 0;
   for (int t = 0; t < sequences; ++t) {
@@ -145,17 +173,78 @@ __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequen
 struct PfPacked {
   int j, h;
   PfSequence s;
+  int part, parts, slot, share;  // which of how many, the first one's place in part_o and part_ml
 };
-__device__ __forceinline__ PfPacked pf_packed_block(const PrefillArgs& a, int nqb, int heads, int sequences) {
+__device__ __forceinline__ PfPacked pf_packed_block(const PrefillArgs& a, int nqb, int queries, int heads, int sequences) {
   PfBlock p;
+  const int all = nqb * a.parts;  // the first parts of all blocks, the second ones, ...
   if (heads % 8 != 0) {
-    p = pf_block(nqb, heads, sequences);
+    p = pf_block(all, heads, sequences);
   } else {
-    const int L = (int)blockIdx.x + nqb * ((int)blockIdx.y + heads * (int)blockIdx.z);
-    const int k = L / 8, unit = k / nqb;
-    p = PfBlock{k % nqb, L % 8 * (heads / 8) + unit % (heads / 8), unit / (heads / 8)};
+    const int L = (int)blockIdx.x + all * ((int)blockIdx.y + heads * (int)blockIdx.z);
+    const int k = L / 8, unit = k / all;
+    p = PfBlock{k % all, L % 8 * (heads / 8) + unit % (heads / 8), unit / (heads / 8)};
   }
-  return PfPacked{p.j, p.h, pf_ranked(a, sequences, p.b)};
+  PfPacked one = {p.j, p.h, {}, 0, 1, 0, 0};
+  if (a.parts > 1) {
+    one.part = p.j / nqb;
+    one.j = p.j - one.part * nqb;
+    one.slot = ((p.b * heads + p.h) * nqb + one.j) * a.parts;
+  }
+  one.s = pf_ranked(a, sequences, p.b, queries, heads, one.share);
+  return one;
+}
+
+// Parts of a block that sees ``keys`` keys, of about ``share`` tiles.
+__device__ __forceinline__ int pf_parts(const PrefillArgs& a, int keys, int share) {
+  const int nt = (keys + 63) / 64;
+  return a.parts == 1 || nt < 2 * kPartLeast ? 1 : min((nt + share - 1) / share, a.parts);
+}
+
+// This workgroup's part of its block, which sees ``keys`` keys: ``sp`` and ``keys`` narrowed to it; false: there is none.
+__device__ __forceinline__ bool pf_part(const PrefillArgs& a, PfPacked& blk, PfSpan& sp, int& keys) {
+  if (a.parts == 1) return true;
+  const int parts = keys > 0 ? pf_parts(a, keys, blk.share) : 1;
+  if (blk.part >= parts) return false;
+  if (parts == 1) return true;
+  blk.parts = parts;
+  const int nt = (keys + 63) / 64, t0 = (int)((uint32_t)nt * (uint32_t)blk.part / (uint32_t)parts);
+  const int k0 = 64 * t0, k1 = min(64 * (int)((uint32_t)nt * (uint32_t)(blk.part + 1) / (uint32_t)parts), keys);
+  sp.k += k0 * a.k_pos;
+  sp.v += k0 * a.v_pos;
+  sp.nk = min(sp.nk, k1) - k0;
+  sp.before -= k0;
+  keys = k1 - k0;
+  return true;
+}
+
+// Whether the workgroup has a part of a block: the same in every lane, so that neither way out waits for the other.
+__device__ __forceinline__ bool pf_in_parts(const PfPacked& blk) { return __builtin_amdgcn_readfirstlane(blk.parts) > 1; }
+
+// A part's queries' (m, l) from its score wave w: query i of lane half g.
+__device__ __forceinline__ void pf_leave_ml(const PrefillArgs& a, const PfPacked& blk, int w, int g, int i, float m, float l) {
+  *reinterpret_cast<f32x2_t*>(a.part_ml + (int64_t)(blk.slot + blk.part) * kPartMl + ((w * 2 + g) * 64 + i) * 2) =
+      f32x2_t{m, l};
+}
+
+// A part's O from its value wave vw, of the ``n`` queries there are of its 64.
+__device__ __forceinline__ void pf_leave_o(const PrefillArgs& a, const PfPacked& blk, int vw, int lane, int n,
+                                           const f32x16_t (&o)[2][4]) {
+  float* to = a.part_o + (int64_t)(blk.slot + blk.part) * kPartO + vw * (32 * 256) + lane * 4;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if (32 * u + (lane & 31) >= n) return;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = 4 * (r + 2 * k);
+          *reinterpret_cast<f32x4_t*>(to + (((u * 2 + r) * 4 + e) * 2 + k) * 256) =
+              f32x4_t{o[u][e][at], o[u][e][at + 1], o[u][e][at + 2], o[u][e][at + 3]};
+        }
+  }
 }
 
 // On a tile with keys that some query does not see, their probability is 0, but 0 times an infinity or NaN of V would
@@ -167,7 +256,7 @@ __device__ __forceinline__ PfPacked pf_packed_block(const PrefillArgs& a, int nq
 template <int D>
 __device__ __noinline__ void pf_again_16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out,
                                          int64_t q_pos, int64_t k_pos, int64_t v_pos, int n, int whole, int nk,
-                                         float scale_log2) {
+                                         float scale_log2, uint32_t wanted) {
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const int end = whole + n, query = min(c, n - 1), lim = whole + query + 1;
   const uint16_t* qrow = q + query * q_pos + 8 * g;
@@ -210,7 +299,7 @@ __device__ __noinline__ void pf_again_16(const uint16_t* q, const uint16_t* k, c
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float li = __shfl(l, 4 * g + i, kWave), div = li == 0.f ? 1.f : li;
-    if (4 * g + i >= n) continue;
+    if (4 * g + i >= n || !(wanted >> c & 1)) continue;
     u32x4_t w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(o[0][2 * e][i] / div, o[0][2 * e + 1][i] / div);
@@ -218,15 +307,16 @@ __device__ __noinline__ void pf_again_16(const uint16_t* q, const uint16_t* k, c
   }
 }
 
-// Queries q_first .. q_first + 16 groups - 1 of a head again, dimensions slice .. + 127.
+// Queries q_first .. q_first + 16 groups - 1 of a head again, of dimensions slice .. + 127 the ``wanted`` eights.
 template <int D>
-__device__ __forceinline__ void pf_again(const PrefillArgs& a, const PfSpan& sp, int h, int q_first, int groups, int slice) {
+__device__ __forceinline__ void pf_again(const PrefillArgs& a, const PfSpan& sp, int h, int q_first, int groups, int slice,
+                                         uint32_t wanted = 0xffff) {
   for (int i = 0; i < groups; ++i) {
     const int q0 = q_first + 16 * i, n = min(sp.nq - q0, 16);
     if (n <= 0) return;
     const int64_t row = ((sp.q0 + q0) * a.H + h) * D;
     pf_again_16<D>(a.q + row, sp.k, sp.v + slice, a.out + row + slice, (int64_t)a.H * D, a.k_pos, a.v_pos, n,
-                   q0 + sp.before, sp.nk, a.scale_log2);
+                   q0 + sp.before, sp.nk, a.scale_log2, wanted);
   }
 }
 
@@ -511,7 +601,6 @@ constexpr int kWsD = 512, kWsQ = 64, kWsK = 64;
 constexpr int kWsRow = kWsD * 2 + 16;  // LDS bytes per K row
 constexpr int kWsAhead = 4;
 constexpr float kWsGuard = 16.0f;
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
@@ -619,14 +708,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   WsBlock only;  // packed: the one block of the workgroup, and its span
   PfSpan only_span;
+  PfPacked one = {};
   if constexpr (kPacked) {
-    const PfPacked one = pf_packed_block(a, nqb, a.H, (int)gridDim.z);
+    one = pf_packed_block(a, nqb, kWsQ, a.H, (int)gridDim.z);
     only = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, 0};
     only_span = pf_packed_span(a, one.h, one.s);
     if (only.qb >= only_span.nq) return;
     const int end = min(only.qb + kWsQ, only_span.nq);
-    if (end + only_span.before <= 0)
-      return pf_zeros<D>(a, only_span.q0 + only.qb, only_span.q0 + end, only.h);
+    int keys = end + only_span.before;
+    if (!pf_part(a, one, only_span, keys)) return;
+    if (keys <= 0) return pf_zeros<D>(a, only_span.q0 + only.qb, only_span.q0 + end, only.h);
   }
   auto first = [&]() {
     WsBlock blk;
@@ -648,9 +739,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (kPacked) return only_span;
     return pf_span<D>(a, blk.h, blk.b);
   };
-  // The block's last tile: the one of its last query's last key.
+  // The block's last tile: the one of its last query's last key, or of the part's.
   auto last_tile = [&](const WsBlock& blk, const PfSpan& sp) {
-    return kPacked ? (min(blk.qb + kWsQ, sp.nq) - 1 + sp.before) / kWsK : blk.qb / kWsK;
+    return kPacked ? (min(min(blk.qb + kWsQ, sp.nq) + sp.before, sp.nk) - 1) / kWsK : blk.qb / kWsK;
   };
 
   if (w < 4) {  // ------------------------------------------------------------------------------ scores
@@ -746,6 +837,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         l_run += lt;
       }
       lsum[odd][kh][g][32 * qh + x] = l_run;
+      if (kPacked && pf_in_parts(one)) pf_leave_ml(a, one, w, g, x, m_ref, l_run);
       if (!next(blk)) break;
     }
     lds_barrier();
@@ -979,6 +1071,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   attend_v(n - 1, nullptr);
   lds_barrier();
+  if (kPacked && pf_in_parts(one)) return pf_leave_o(a, one, vw, lane, only_span.nq - only.qb, o);
   output(at.blk, odd);
 }
 
@@ -1022,12 +1115,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int together = kPacked ? a.together : 1, queries = kPairQ / together;
   const int nqb = (a.width + queries - 1) / queries;
   int j, hb, b = 0;
-  PfSequence seq = {};
+  PfPacked one = {};
   if constexpr (kPacked) {
-    const PfPacked blk = pf_packed_block(a, nqb, a.H / together, (int)gridDim.z);
-    j = blk.j;
-    hb = blk.h;
-    seq = blk.s;
+    one = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z);
+    j = one.j;
+    hb = one.h;
   } else {
     const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
     j = blk.j;
@@ -1039,23 +1131,24 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), pr = w & 3;
   const int h = kPacked ? hb * together + pr % together : hb;
   PfSpan sp;
-  if constexpr (kPacked) sp = pf_packed_span(a, h, seq);
+  if constexpr (kPacked) sp = pf_packed_span(a, h, one.s);
   else sp = pf_span<D>(a, h, b);
-  const char* kbase = scalar_pointer(sp.k);
-  const char* vbase = scalar_pointer(sp.v);
-  const int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees
+  int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees (packed: of the part's)
   if constexpr (kPacked) {
     if (qb >= sp.nq) return;
+    if (!pf_part(a, one, sp, keys)) return;
     if (keys <= 0) {
       for (int i = 0; i < together; ++i)
         pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), hb * together + i);
       return;
     }
   }
+  const char* kbase = scalar_pointer(sp.k);
+  const char* vbase = scalar_pointer(sp.v);
   const int nt = (keys + kPairK - 1) / kPairK;
   const int qp = qb + 64 * (kPacked ? pr / together : pr);
   // The pair's last tile, which holds its diagonal (-1: no queries, or they see no key).
-  const int lastk = kPacked ? min(qp + 64, sp.nq) - 1 + sp.before : qp;
+  const int lastk = kPacked ? min(min(qp + 64, sp.nq) + sp.before, keys) - 1 : qp;
   const int dq = qp < sp.nq && lastk >= 0 ? lastk / kPairK : -1;
   const int whole = qp + sp.before;  // every query of the pair sees keys [0, whole]
 
@@ -1201,6 +1294,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       if (t <= nt) bring_v(t - 1);
       landed_barrier();
     }
+    if (kPacked && pf_in_parts(one)) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) pf_leave_ml(a, one, pr, g, 32 * u + x, m_ref[u], l_run[u]);
+    }
     return;
   }
 
@@ -1255,6 +1352,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (t >= 2 && t - 2 <= dq) attend_v(t - 2);
     landed_barrier();
   }
+  if (kPacked && pf_in_parts(one)) return pf_leave_o(a, one, pr, lane, sp.nq - qp, o);
   bool again = false;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -1307,14 +1405,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ float lsum[4][2][32];     // [score wave][lane half]
   const int together = a.together, queries = kPmQ / together;
   const int nqb = (a.width + queries - 1) / queries;
-  const PfPacked blk = pf_packed_block(a, nqb, a.H / together, (int)gridDim.z);
+  PfPacked blk = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z);
   const int qb = (nqb - 1 - blk.j) * queries;  // the longest blocks first
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = (w & 3) >> 1, h = blk.h * together + group % together;
-  const PfSpan sp = pf_packed_span(a, h, blk.s);
+  PfSpan sp = pf_packed_span(a, h, blk.s);
   if (qb >= sp.nq) return;
-  const int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees
+  int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees of the part's keys
+  if (!pf_part(a, blk, sp, keys)) return;
   if (keys <= 0) {
     for (int i = 0; i < together; ++i)
       pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), blk.h * together + i);
@@ -1323,7 +1422,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int nt = (keys + kPmK - 1) / kPmK;
   const int qp = qb + 64 * (group / together);  // the group's first query
   // The group's last tile (-1: no queries, or they see no key).
-  const int lastk = min(qp + 64, sp.nq) - 1 + sp.before;
+  const int lastk = min(min(qp + 64, sp.nq) + sp.before, keys) - 1;
   const int dq = qp < sp.nq && lastk >= 0 ? lastk / kPmK : -1;
 
   if (w < 4) {  // ------------------------------------------------------------------------------ scores
@@ -1428,6 +1527,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       t += 1;
     }
     for (; t <= nt + 1; ++t) lds_barrier();
+    if (pf_in_parts(blk)) pf_leave_ml(a, blk, w, g, x, m_ref, l_run);
     return;
   }
 
@@ -1551,6 +1651,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     bring_k(t + 1);
     landed_barrier();
   }
+  if (pf_in_parts(blk)) return pf_leave_o(a, blk, vw, lane, sp.nq - qp, o);
   bool again = false;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -1579,6 +1680,92 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
   }
   if (__any(again)) pf_again<D>(a, sp, h, qp, 4, slice);
+}
+
+// The parts of blocks joined: out = sum_p w_p O_p / sum_p w_p l_p, w_p = exp(m_p - max m).  One workgroup for a quarter
+// (query half u, rows r of O) of a block's four value waves, each lane what it held of O there.
+template <int D>
+__global__ __launch_bounds__(256) void packed_attn_join_kernel(PrefillArgs a) {
+  const int together = a.together, queries = (D == 128 ? kPairQ : D == 256 ? kPmQ : kWsQ) / together;
+  const int nqb = (a.width + queries - 1) / queries, j = (int)blockIdx.x >> 2, u = blockIdx.x >> 1 & 1, r = blockIdx.x & 1;
+  const int hb = blockIdx.y, lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
+  const int vw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int share = kPartLeast;
+  const PfSequence seq = pf_ranked(a, (int)gridDim.z, blockIdx.z, queries, gridDim.y, share);
+  const int qb = (nqb - 1 - j) * queries;
+  const int group = D == 128 ? vw : D == 256 ? vw >> 1 : 0, h = hb * together + group % together;
+  const PfSpan sp = pf_packed_span(a, h, seq);
+  const int keys = min(qb + queries, sp.nq) + sp.before;
+  if (qb >= sp.nq || keys <= 0) return;
+  const int parts = pf_parts(a, keys, share);
+  if (parts == 1) return;
+  const int64_t slot = ((int64_t)((int)blockIdx.z * (int)gridDim.y + hb) * nqb + j) * a.parts;
+  const int slice = D == 128 ? 0 : D == 256 ? 128 * (vw & 1) : 128 * vw;
+  const int first = qb + 64 * (group / together) + 32 * u, query = first + x;
+  // The score waves of the queries, two (by key half) at head dim 512, and the queries' place there.
+  const int sw = D == 128 ? vw : D == 256 ? 2 * group + u : u, at = D == 128 ? 32 * u + x : x;
+  auto ml = [&](int p, int w, int half) {
+    return *reinterpret_cast<const f32x2_t*>(a.part_ml + (slot + p) * kPartMl + ((w * 2 + half) * 64 + at) * 2);
+  };
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, ml(p, sw, 0)[0]);
+  f32x4_t o[4][2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e][0] = o[e][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  if (first >= sp.nq) return;
+#pragma unroll 4
+  for (int p = 0; p < parts && query < sp.nq; ++p) {
+    const float* from = a.part_o + (slot + p) * kPartO + (vw * 4 + u * 2 + r) * (8 * 256) + lane * 4;
+    const f32x2_t one = ml(p, sw, 0);
+    float lp = one[1] + ml(p, sw, 1)[1];
+    if constexpr (D == 512) lp += ml(p, sw + 2, 0)[1] + ml(p, sw + 2, 1)[1];
+    const float f = one[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(one[0] - m);
+    l += f * lp;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) o[e][k] += f * *reinterpret_cast<const f32x4_t*>(from + (e * 2 + k) * 256);
+  }
+  const float inv = l > 0.f ? 1.f / l : 1.f;
+  auto pair = [&](float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
+  };
+  bool again = false;
+  if (query < sp.nq) {
+    uint16_t* orow = a.out + ((sp.q0 + query) * a.H + h) * D + slice + (D == 128 ? 16 * r + 8 * g : 64 * r + 32 * g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4_t out;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        out[2 * k] = D == 128 ? pair(o[i][k][0], o[i][k][1]) : pair(o[0][k][i], o[1][k][i]);
+        out[2 * k + 1] = D == 128 ? pair(o[i][k][2], o[i][k][3]) : pair(o[2][k][i], o[3][k][i]);
+      }
+      *reinterpret_cast<u32x4_t*>(orow + (D == 128 ? 32 : 8) * i) = out;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) again |= pf_nonfinite(out[k]);
+    }
+  }
+  if (__any(again)) pf_again<D>(a, sp, h, first, 2, slice, D == 128 ? 0x3333u << (2 * r) : 0xffu << (8 * r));
+}
+
+// Parts of a block at most, for a launch of ``blocks`` that see up to ``keys`` keys.  (1 where every CU has a block: by then
+// whole blocks take as long.  Where there may be parts but are none, the join costs 2-3 us.)
+inline int packed_parts(int64_t blocks, int sequences, int64_t keys) {
+  const int64_t tiles = (keys + 63) / 64;
+  if (blocks >= kPartCus || sequences > kWave || tiles < 2 * kPartLeast) return 1;
+  return (int)std::min({4 * kPartCus / blocks, tiles / kPartLeast, (int64_t)kPartMost});
+}
+
+// Heads of a kv head in a block, and queries of a head.
+inline int packed_together(int head_dim, int heads_per_kv) {
+  if (head_dim == 128) return heads_per_kv % 4 == 0 ? 4 : heads_per_kv % 2 == 0 ? 2 : 1;
+  return head_dim == 256 && heads_per_kv % 2 == 0 ? 2 : 1;
+}
+inline int packed_queries(int head_dim, int heads_per_kv) {
+  return (head_dim == 128 ? kPairQ : head_dim == 256 ? kPmQ : kWsQ) / packed_together(head_dim, heads_per_kv);
 }
 
 // Head dim 128 in blocks of 192 queries, for the launches of small_blocks: one workgroup of 4 waves, two workgroups per
@@ -1860,11 +2047,22 @@ extern "C" int omni_prefill_attention(const void* q, const void* k_cache, const 
   return omni_launch_status();
 }
 
+extern "C" size_t omni_packed_attention_workspace(int32_t sequences, int64_t keys, int32_t longest, int32_t heads,
+                                                  int32_t kv_heads, int32_t head_dim) {
+  if (sequences <= 0 || keys <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  if (head_dim != 128 && head_dim != 256 && head_dim != 512) return 0;
+  const int group = heads / kv_heads, rows = omni::packed_queries(head_dim, group);
+  const int64_t blocks = (longest + (int64_t)rows - 1) / rows * (heads / omni::packed_together(head_dim, group)) * sequences;
+  const int parts = omni::packed_parts(blocks, sequences, keys);
+  return parts == 1 ? 0 : (size_t)(blocks * parts * (omni::kPartO + omni::kPartMl) * 4);
+}
+
 extern "C" int omni_packed_attention(const void* q, const void* k, const void* v, int64_t k_stride_pos,
                                      int64_t k_stride_head, int64_t v_stride_pos, int64_t v_stride_head,
                                      const int64_t* starts, const int64_t* k_starts, int32_t sequences,
                                      int64_t queries, int64_t keys, int32_t longest, int32_t heads, int32_t kv_heads,
-                                     int32_t head_dim, float scale, void* out, int32_t dtype, void* stream) {
+                                     int32_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes,
+                                     int32_t dtype, void* stream) {
   if (dtype != OMNI_BF16) return OMNI_ERR_DTYPE;
   if (sequences < 0 || queries < 0 || keys < 0 || longest < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads)
     return OMNI_ERR_INVALID;
@@ -1899,16 +2097,33 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
   a.v_pos = v_stride_pos;
   a.v_head = v_stride_head;
   a.heads_per_kv = heads / kv_heads;
-  a.together = 1;
-  if (head_dim == 128) a.together = a.heads_per_kv % 4 == 0 ? 4 : a.heads_per_kv % 2 == 0 ? 2 : 1;
-  if (head_dim == 256) a.together = a.heads_per_kv % 2 == 0 ? 2 : 1;
-  const int rows = (head_dim == 128 ? omni::kPairQ : head_dim == 256 ? omni::kPmQ : omni::kWsQ) / a.together;
-  const dim3 grid((longest + rows - 1) / rows, heads / a.together, sequences);
+  a.together = omni::packed_together(head_dim, a.heads_per_kv);
+  const int rows = omni::packed_queries(head_dim, a.heads_per_kv);
+  dim3 grid((longest + rows - 1) / rows, heads / a.together, sequences);
   // The blocks are counted in 31 bits, a launch's threads along x, 512 to a block, in 32.
   if (grid.x >= (1u << 23) || (int64_t)grid.x * grid.y * grid.z > 0x7fffffffLL) return OMNI_ERR_SHAPE;
+  const int64_t blocks = (int64_t)grid.x * grid.y * grid.z;
+  const int64_t seen = k_starts == starts ? std::min<int64_t>(keys, longest) : keys;  // by one sequence, at most
+  a.parts = omni::packed_parts(blocks, sequences, seen);
+  if (a.parts > 1) {
+    if (!workspace || ((uintptr_t)workspace & 255u) ||
+        workspace_bytes < omni_packed_attention_workspace(sequences, seen, longest, heads, kv_heads, head_dim))
+      return OMNI_ERR_WORKSPACE;
+    a.part_o = (float*)workspace;
+    a.part_ml = a.part_o + blocks * a.parts * omni::kPartO;
+  }
+  const dim3 join(grid.x * 4, grid.y, grid.z);
+  grid.x *= a.parts;
   const hipStream_t s = (hipStream_t)stream;
-  if (head_dim == 128) omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
-  else if (head_dim == 256) omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
-  else omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
+  if (head_dim == 128) {
+    omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
+    if (a.parts > 1) omni::packed_attn_join_kernel<128><<<join, 256, 0, s>>>(a);
+  } else if (head_dim == 256) {
+    omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
+    if (a.parts > 1) omni::packed_attn_join_kernel<256><<<join, 256, 0, s>>>(a);
+  } else {
+    omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
+    if (a.parts > 1) omni::packed_attn_join_kernel<512><<<join, 256, 0, s>>>(a);
+  }
   return omni_launch_status();
 }

@@ -777,6 +777,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _packed_workspace(*shape: int) -> int:
+    return _lib.load().omni_packed_attention_workspace(*shape)
+
+
 def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the memory between the first and last elements of two tensors overlaps."""
     if not a.numel() or not b.numel():
@@ -810,7 +815,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     bounds = starts.numel()
     if bounds < 1 or longest < 0:
         raise ValueError("starts: [S + 1], longest: at least the longest sequence's queries")
-    k_starts = starts if k_starts is None else k_starts
+    own = k_starts is None
+    k_starts = starts if own else k_starts
     device = q.get_device()
     _positions(bounds, device, ("starts", starts), ("k_starts", k_starts))
     if not k.get_device() == v.get_device() == device >= 0:
@@ -821,9 +827,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
         raise ValueError("out: contiguous, q's shape, dtype and device")
     elif any(_share_memory(out, t) for t in (q, k, v)):
         raise ValueError("out: memory of its own, not q's, k's or v's")
+    longest = min(longest, n)
+    size = _packed_workspace(bounds - 1, min(m, longest) if own else m, longest, heads, kv, dim)
+    workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
     _call(device, "packed attention", lib.omni_packed_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pos, k_head,
-          v_pos, v_head, starts.data_ptr(), k_starts.data_ptr(), bounds - 1, n, m, min(longest, n), heads, kv, dim, scale,
-          out.data_ptr(), _lib.BF16)
+          v_pos, v_head, starts.data_ptr(), k_starts.data_ptr(), bounds - 1, n, m, longest, heads, kv, dim, scale,
+          out.data_ptr(), _ptr(workspace), size, _lib.BF16)
     return out
 
 

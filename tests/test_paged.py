@@ -151,8 +151,14 @@ def test_c_abi_refusals_before_launch():
     assert lib.omni_paged_attention(*changed(attn, 18, ctypes.c_void_p(0x10010))) == -4
     assert lib.omni_paged_attention(*changed(attn, 11, 0)) == 0
     assert lib.omni_paged_attention(*changed(attn, 11, 2 ** 23)) == -3
-    packed = [FAKE, FAKE, FAKE, 256, 128, 256, 128, FAKE, FAKE, 2, 9, 9, 5, 4, 2, 128, 0.1, FAKE, _lib.BF16, None]
-    assert lib.omni_packed_attention(*changed(packed, 18, _lib.F32)) == -2
+    packed = [FAKE, FAKE, FAKE, 256, 128, 256, 128, FAKE, other[0], 2, 9, 9, 5, 4, 2, 128, 0.1, FAKE]
+    packed[11] = 4000
+    ws = lib.omni_packed_attention_workspace(2, 4000, 5, 4, 2, 128)
+    assert ws > 0 and lib.omni_packed_attention_workspace(65, 4000, 5, 4, 2, 128) == 0
+    packed += [FAKE, ws, _lib.BF16, None]
+    assert lib.omni_packed_attention(*changed(packed, 19, ws - 1)) == -4
+    assert lib.omni_packed_attention(*changed(packed, 18, None)) == -4
+    assert lib.omni_packed_attention(*changed(packed, 20, _lib.F32)) == -2
     assert lib.omni_packed_attention(*changed(packed, 15, 64)) == -3
     assert lib.omni_packed_attention(*changed(packed, 3, 252)) == -1
     assert lib.omni_packed_attention(*changed(packed, 16, -1.0)) == -1

@@ -422,6 +422,59 @@ def test_packed_attention_head_counts(cuda, heads, kv, dim):
     packed_case(cuda, heads, kv, dim, [70, 1, 0, 150], [0, 40, 3, 9], heads + kv)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (2, 1, 128), (1, 1, 128), (8, 8, 128), (2, 1, 256), (3, 3, 256),
+                                          (2, 2, 512), (8, 8, 512)])
+def test_packed_attention_of_few_queries_behind_many_keys(cuda, heads, kv, dim):
+    """Few blocks, each cut along its keys: one query, a block's worth and one more, keys that end inside a tile."""
+    packed_case(cuda, heads, kv, dim, [1], [2999], dim + heads, longest=1)
+    packed_case(cuda, heads, kv, dim, [20, 1, 64], [4000, 130, 63], dim + heads + 1)
+    packed_case(cuda, heads, kv, dim, [257], [1000], dim + heads + 2)
+    packed_case(cuda, heads, kv, dim, [70, 3], [1500, -3], dim + heads + 3, scale=1.0)
+    packed_case(cuda, heads, kv, dim, [2000], [-300], dim + heads + 4)
+
+
+def test_packed_attention_in_parts_captured(cuda):
+    """One captured launch for lengths that are cut and that are not; calls on two streams share nothing."""
+    g = gen(41)
+    q, k, v = normal((64, 8, 128), g, cuda), normal((4100, 2, 128), g, cuda), normal((4100, 2, 128), g, cuda)
+    starts, k_starts = (torch.tensor([0, 64], device=cuda) for _ in range(2))
+    out = torch.empty_like(q)
+    graphs = batching.GraphCache(cuda, True)
+    run = graphs.runner("parts", lambda: kernels.packed_attention(q, k, v, starts, 64, 0.1, k_starts=k_starts, out=out),
+                        lambda: [])
+    for keys in (4100, 1500, 64, 1601, 0):
+        k_starts[1] = keys
+        q.copy_(normal(q.shape, g, cuda))
+        run()
+        torch.cuda.synchronize()
+        eager = [torch.empty_like(q) for _ in range(2)]
+        for stream, to in zip((torch.cuda.Stream(), torch.cuda.Stream()), eager):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                kernels.packed_attention(q, k, v, starts, 64, 0.1, k_starts=k_starts, out=to)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, to) for to in eager)
+        want, size = op.packed_attention(q, k, v, [0, 64], [0, keys], 0.1)
+        close(out, want, size, q, k, 0.1)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (1, 1, 128), (2, 1, 256), (2, 2, 512)])
+def test_packed_attention_in_parts_does_not_see_what_is_masked(cuda, heads, kv, dim):
+    g, n, past = gen(dim + 5), 90, 700
+    q = normal((n, heads, dim), g, cuda)
+    k, v = (normal((n + past, kv, dim), g, cuda) for _ in "kv")
+    v[past + 40, 0, 7], v[past + 41, 0, 100], v[past + 41, 0, 17] = float("inf"), float("nan"), float("-inf")
+    starts, k_starts = torch.tensor([0, n], device=cuda), torch.tensor([0, n + past], device=cuda)
+    out = [kernels.packed_attention(q, k, v, starts, n, dim ** -0.5, k_starts=k_starts) for _ in range(3)]
+    torch.cuda.synchronize()
+    want, size = op.packed_attention(q, k, v, [0, n], [0, n + past], dim ** -0.5)
+    fine = want.isfinite()
+    assert fine[:40].all() and torch.equal(out[0].isnan(), want.isnan()) and torch.equal(out[0].isposinf(), want.isposinf())
+    assert all(torch.equal(o.view(torch.int16), out[0].view(torch.int16)) for o in out)
+    close(torch.where(fine, out[0].double(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, size, 0.0), q, k,
+          dim ** -0.5)
+
+
 @pytest.mark.parametrize("heads,kv,dim", [(2, 1, 128), (8, 8, 128), (2, 1, 256), (2, 1, 512)])
 def test_packed_attention_more_sequences_than_are_ranked(cuda, heads, kv, dim):
     packed_case(cuda, heads, kv, dim, [(13 * i) % 70 for i in range(67)], [(7 * i) % 11 for i in range(67)], dim + heads)
