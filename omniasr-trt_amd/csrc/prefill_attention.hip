@@ -128,16 +128,16 @@ __device__ __forceinline__ int64_t pf_readlane64(int64_t v, int lane) {
 // Few blocks behind many keys: the longest block is the launch, ~1.05 us for each of its 64-key tiles, while other CUs have
 // nothing.  So a block is cut along its keys into parts, each a workgroup's, and a second launch (packed_attn_join_kernel)
 // joins their (O, m, l).  A part costs its start and end (~8 us) and 128 KB of O written and read, the join ~3 us: parts of
-// kPartLeast tiles and more, blocks of two such at least, at most kPartMost parts.  Measured, us, whole and in parts: 20
-// queries behind 4000 keys, 8 heads x 512 72 / 41, 32 over 8 x 128 75 / 40, 16 over 2 x 256 71 / 39; 64 behind 8000, 8 x 512
-// 179 / 66; 500 behind 6000, 8 x 512 139 / 78, 32 over 8 x 128 123 / 70.  Parts of 2 tiles and more: 20 behind 1500 33 / 30,
-// but one prompt of 1433 45 / 57, four of 200-800 28 / 46.
-constexpr int kPartCus = 256, kPartLeast = 12, kPartMost = 16;
+// kPartLeast tiles and more, at most kPartMost of a block, where the longest block has kPartBlock tiles and 1.5 times what all
+// have for each CU.  Measured, us, whole and in parts: 20 queries behind 4000 keys, 8 heads x 512 72 / 36, 32 over 8 x 128 75 /
+// 34, 16 over 2 x 256 71 / 34; 64 behind 8000, 8 x 512 200 / 66, four of 64 behind 4000 142 / 62; 500 behind 6000, 8 x 512 116
+// / 80, 32 over 8 x 128 120 / 73.  Parts of 2 tiles and more, of any block: one prompt of 1433 45 / 57, four of 200-800 28 / 46.
+constexpr int kPartCus = 256, kPartLeast = 8, kPartBlock = 24, kPartMost = 16;
 
 // The sequence of rank r by work (queries x keys, less what causality hides), the most first: so the last blocks of a
 // launch, whose CUs wait for each other, are the short ones.  Past 64 sequences, the order of the call.
-// ``share``, where blocks (of ``queries``, ``heads`` for each) may be in parts: the key tiles of a part, an even one of
-// about what all blocks have for each CU.
+// ``share``, where blocks (of ``queries``, ``heads`` for each) may be in parts: the key tiles of a part, about what all blocks
+// have for each CU, or what no block is longer than.
 __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequences, int r, int queries, int heads,
                                                 int& share) {
   if (sequences > kWave) return pf_sequence(a, r);
@@ -148,10 +148,15 @@ __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequen
     const int64_t mean = ((int64_t)min(nq, queries) + mine.nk - mine.nq + mine.nk) / 2;  // keys of a block, about
     const int64_t tiles = mean > 0 ? blocks * ((mean + 63) / 64) : 0;
     int all = lane < sequences ? (int)(tiles < 65536 ? tiles : 65536) : 0;
+    int longest = all > 0 ? (mine.nk + 63) / 64 : 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, kWave);
-    all = __builtin_amdgcn_readfirstlane(all);
-    share = max((int)(((uint32_t)all * (uint32_t)heads + kPartCus - 1) / kPartCus), kPartLeast);
+    for (int o = 32; o > 0; o >>= 1) {
+      all += __shfl_xor(all, o, kWave);
+      longest = max(longest, __shfl_xor(longest, o, kWave));
+    }
+    const int even = (int)(((uint32_t)__builtin_amdgcn_readfirstlane(all) * (uint32_t)heads + kPartCus - 1) / kPartCus);
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    share = longest < max(kPartBlock, 3 * even / 2) ? longest : max(even, kPartLeast);
   }
   const float work = lane < sequences ? (float)mine.nq * (2.f * (float)mine.nk - (float)mine.nq) : -INFINITY;
   int rank = 0;
@@ -176,29 +181,25 @@ struct PfPacked {
   int part, parts, slot, share;  // which of how many, the first one's place in part_o and part_ml
 };
 __device__ __forceinline__ PfPacked pf_packed_block(const PrefillArgs& a, int nqb, int queries, int heads, int sequences) {
-  PfBlock p;
-  const int all = nqb * a.parts;  // the first parts of all blocks, the second ones, ...
-  if (heads % 8 != 0) {
-    p = pf_block(all, heads, sequences);
-  } else {
-    const int L = (int)blockIdx.x + all * ((int)blockIdx.y + heads * (int)blockIdx.z);
-    const int k = L / 8, unit = k / all;
-    p = PfBlock{k % all, L % 8 * (heads / 8) + unit % (heads / 8), unit / (heads / 8)};
+  // The first parts of all blocks, then the second ones, ...: most of the later ones are none, and end at once.
+  const int part = a.parts > 1 ? (int)blockIdx.z / sequences : 0, z = (int)blockIdx.z - part * sequences;
+  const int L = (int)blockIdx.x + nqb * ((int)blockIdx.y + heads * z);
+  PfBlock p = {(int)blockIdx.x, (int)blockIdx.y, z};
+  if (heads % 8 == 0) {
+    const int k = L / 8, unit = k / nqb;
+    p = PfBlock{k % nqb, L % 8 * (heads / 8) + unit % (heads / 8), unit / (heads / 8)};
+  } else if (heads * sequences % 8 == 0) {  // as pf_block
+    const int k = L / 8, unit = k / nqb * 8 + L % 8;
+    p = PfBlock{k % nqb, unit % heads, unit / heads};
   }
-  PfPacked one = {p.j, p.h, {}, 0, 1, 0, 0};
-  if (a.parts > 1) {
-    one.part = p.j / nqb;
-    one.j = p.j - one.part * nqb;
-    one.slot = ((p.b * heads + p.h) * nqb + one.j) * a.parts;
-  }
+  PfPacked one = {p.j, p.h, {}, part, 1, ((p.b * heads + p.h) * nqb + p.j) * a.parts, 0};
   one.s = pf_ranked(a, sequences, p.b, queries, heads, one.share);
   return one;
 }
 
 // Parts of a block that sees ``keys`` keys, of about ``share`` tiles.
 __device__ __forceinline__ int pf_parts(const PrefillArgs& a, int keys, int share) {
-  const int nt = (keys + 63) / 64;
-  return a.parts == 1 || nt < 2 * kPartLeast ? 1 : min((nt + share - 1) / share, a.parts);
+  return a.parts == 1 ? 1 : min(((keys + 63) / 64 + share - 1) / share, a.parts);
 }
 
 // This workgroup's part of its block, which sees ``keys`` keys: ``sp`` and ``keys`` narrowed to it; false: there is none.
@@ -710,7 +711,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   PfSpan only_span;
   PfPacked one = {};
   if constexpr (kPacked) {
-    one = pf_packed_block(a, nqb, kWsQ, a.H, (int)gridDim.z);
+    one = pf_packed_block(a, nqb, kWsQ, a.H, (int)gridDim.z / a.parts);
     only = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, 0};
     only_span = pf_packed_span(a, one.h, one.s);
     if (only.qb >= only_span.nq) return;
@@ -1117,7 +1118,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int j, hb, b = 0;
   PfPacked one = {};
   if constexpr (kPacked) {
-    one = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z);
+    one = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z / a.parts);
     j = one.j;
     hb = one.h;
   } else {
@@ -1405,7 +1406,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ float lsum[4][2][32];     // [score wave][lane half]
   const int together = a.together, queries = kPmQ / together;
   const int nqb = (a.width + queries - 1) / queries;
-  PfPacked blk = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z);
+  PfPacked blk = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z / a.parts);
   const int qb = (nqb - 1 - blk.j) * queries;  // the longest blocks first
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1690,7 +1691,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(PrefillArgs a) {
   const int nqb = (a.width + queries - 1) / queries, j = (int)blockIdx.x >> 2, u = blockIdx.x >> 1 & 1, r = blockIdx.x & 1;
   const int hb = blockIdx.y, lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
   const int vw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int share = kPartLeast;
+  int share = 1;
   const PfSequence seq = pf_ranked(a, (int)gridDim.z, blockIdx.z, queries, gridDim.y, share);
   const int qb = (nqb - 1 - j) * queries;
   const int group = D == 128 ? vw : D == 256 ? vw >> 1 : 0, h = hb * together + group % together;
@@ -1751,12 +1752,14 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(PrefillArgs a) {
   if (__any(again)) pf_again<D>(a, sp, h, first, 2, slice, D == 128 ? 0x3333u << (2 * r) : 0xffu << (8 * r));
 }
 
-// Parts of a block at most, for a launch of ``blocks`` that see up to ``keys`` keys.  (1 where every CU has a block: by then
-// whole blocks take as long.  Where there may be parts but are none, the join costs 2-3 us.)
-inline int packed_parts(int64_t blocks, int sequences, int64_t keys) {
+// Parts of a block at most, for a launch of ``blocks`` that see up to ``keys`` keys: 1 where every CU has a block.  (Their
+// workgroups are launched before it is known how many there are.  Up to 4 x 256 of them cost 2 x 600 behind 3000 10 us where
+// there were none, 2 x 256 4 us; three prompts of 60-200 behind 1000, with none, take 37 us in place of 34.)
+inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int longest) {
   const int64_t tiles = (keys + 63) / 64;
-  if (blocks >= kPartCus || sequences > kWave || tiles < 2 * kPartLeast) return 1;
-  return (int)std::min({4 * kPartCus / blocks, tiles / kPartLeast, (int64_t)kPartMost});
+  if (blocks >= kPartCus || sequences > kWave || tiles < kPartBlock) return 1;
+  if (keys <= longest && 3 * blocks >= 2 * kPartCus) return 1;  // no earlier keys: a block's mean is half the longest
+  return (int)std::min({kPartCus / blocks + 1, tiles / kPartLeast, (int64_t)kPartMost});
 }
 
 // Heads of a kv head in a block, and queries of a head.
@@ -2053,7 +2056,7 @@ extern "C" size_t omni_packed_attention_workspace(int32_t sequences, int64_t key
   if (head_dim != 128 && head_dim != 256 && head_dim != 512) return 0;
   const int group = heads / kv_heads, rows = omni::packed_queries(head_dim, group);
   const int64_t blocks = (longest + (int64_t)rows - 1) / rows * (heads / omni::packed_together(head_dim, group)) * sequences;
-  const int parts = omni::packed_parts(blocks, sequences, keys);
+  const int parts = omni::packed_parts(blocks, sequences, keys, longest);
   return parts == 1 ? 0 : (size_t)(blocks * parts * (omni::kPartO + omni::kPartMl) * 4);
 }
 
@@ -2104,7 +2107,7 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
   if (grid.x >= (1u << 23) || (int64_t)grid.x * grid.y * grid.z > 0x7fffffffLL) return OMNI_ERR_SHAPE;
   const int64_t blocks = (int64_t)grid.x * grid.y * grid.z;
   const int64_t seen = k_starts == starts ? std::min<int64_t>(keys, longest) : keys;  // by one sequence, at most
-  a.parts = omni::packed_parts(blocks, sequences, seen);
+  a.parts = omni::packed_parts(blocks, sequences, seen, longest);
   if (a.parts > 1) {
     if (!workspace || ((uintptr_t)workspace & 255u) ||
         workspace_bytes < omni_packed_attention_workspace(sequences, seen, longest, heads, kv_heads, head_dim))
@@ -2113,7 +2116,7 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
     a.part_ml = a.part_o + blocks * a.parts * omni::kPartO;
   }
   const dim3 join(grid.x * 4, grid.y, grid.z);
-  grid.x *= a.parts;
+  grid.z *= a.parts;
   const hipStream_t s = (hipStream_t)stream;
   if (head_dim == 128) {
     omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
