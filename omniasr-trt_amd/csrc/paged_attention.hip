@@ -152,7 +152,10 @@ struct PagedPiece {
   const int32_t* table;
 };
 
-// NB: blocks of 16 query columns that share a read of the keys.
+// NB: blocks of 16 query columns that share a read of the keys.  Two at most: four spill registers (64
+// columns, 42 us against 31 in twos).  Measured, with the second launch's 4-5 us: 8 slots x 5 of 750-2400 keys, 8 heads
+// x 512 e4m3 26 us (the stream at 4.2 TB/s), 32 x 128 bf16 44; 16 slots of 4000-8188, 32 over 8 x 128 e4m3 48 (5.1 TB/s).
+// Three tiles ahead in place of two 28.6 against 27.1 us; 1024, 768 and 256 workgroups 31, 29 and 27 against 27.
 template <int D, bool kF8, int NB>
 __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2))) void paged_attn_kernel(PagedAttn a) {
   constexpr int kRowB = D * (kF8 ? 1 : 2), kAhead = paged_ahead<kF8, NB>();

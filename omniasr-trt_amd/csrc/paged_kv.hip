@@ -8,7 +8,7 @@
 // binade above 2^-6, 14 below the largest.)  k is quantised from the rotated fp32 values, not from their bf16 rounding.
 //
 // Both kernels are one pass over their bytes, 16 (8 for e4m3) of one vector a thread: a step's launch is latency, a
-// prompt's is HBM.
+// prompt's is HBM.  Measured, 8 prompts of 750-2400, 8 heads x 512, e4m3: write 102 us (4.7 TB/s), read 45-50 us (5.4-6.1).
 #include "common.h"
 #include "paged.h"
 
@@ -54,7 +54,8 @@ struct PagedWrite {
 };
 
 // One workgroup per token; a thread keeps the same 8 dimensions of every vector it takes, so the token's angles are read
-// once and its cell is found once.
+// once and its cell is found once.  (Threads over all vectors of all tokens: those prompts written and read back 190 us, so
+// 151.)
 template <int D, bool kF8>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite w, PagedCache a) {
   constexpr int kLanes = D / 8;  // of one vector; a vector never spans two waves
