@@ -50,17 +50,6 @@ __device__ __forceinline__ PagedReach paged_reach(const PagedAttn& a, int b) {
   return {n, (int)(last < a.cache.positions ? last : a.cache.positions)};
 }
 
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);  // row_bcast 15, 31
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);
-  return v;
-}
-
 // The line: 64 rows at a time in the lanes of a wave, lane's row with ``tiles`` for each of its units, after ``before``
 // places of the rows ahead of it.
 struct PagedLine {

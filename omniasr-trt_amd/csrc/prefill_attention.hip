@@ -47,6 +47,7 @@ struct PrefillArgs {
   int parts = 1;
   float* part_o = nullptr;   // [part][value wave][query half u][r][e][k][lane][4]
   float* part_ml = nullptr;  // [part][score wave][lane half][query][2]
+  int sequences = 0;  // head dim 512 in chains
 };
 constexpr int kPartO = 4 * 32 * 256, kPartMl = 4 * 2 * 64 * 2;  // floats
 
@@ -138,7 +139,19 @@ __device__ __forceinline__ int64_t pf_readlane64(int64_t v, int lane) {
 // / 80, 32 over 8 x 128 120 / 73.  Parts of 2 tiles and more, of any block: one prompt of 1433 45 / 57, four of 200-800 28 / 46.
 constexpr int kPartCus = 256, kPartLeast = 8, kPartBlock = 24, kPartMost = 16;
 
-// The sequence of rank r by work (queries x keys, less what causality hides), the most first: so the last blocks of a
+// The rank of a lane's sequence by work (queries x keys, less what causality hides), the most first.
+__device__ __forceinline__ int pf_rank(const PfSequence& mine, int sequences) {
+  const int lane = lane_id();
+  const float work = lane < sequences ? (float)mine.nq * (2.f * (float)mine.nk - (float)mine.nq) : -INFINITY;
+  int rank = 0;
+  for (int t = 0; t < sequences; ++t) {
+    const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(work), t));
+    rank += other > work || (other == work && t < lane) ? 1 : 0;
+  }
+  return rank;
+}
+
+// The sequence of rank r by work, the most first: so the last blocks of a
 // launch, whose CUs wait for each other, are the short ones.  Past 64 sequences, the order of the call.
 // ``share``, where blocks (of ``queries``, ``heads`` for each) may be in parts: the key tiles of a part, about what all blocks
 // have for each CU, or what no block is longer than.
@@ -162,13 +175,7 @@ __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequen
     longest = __builtin_amdgcn_readfirstlane(longest);
     share = longest < max(kPartBlock, 3 * even / 2) ? longest : max(even, kPartLeast);
   }
-  const float work = lane < sequences ? (float)mine.nq * (2.f * (float)mine.nk - (float)mine.nq) : -INFINITY;
-  int rank = 0;
-  for (int t = 0; t < sequences; ++t) {
-    const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(work), t));
-    rank += other > work || (other == work && t < lane) ? 1 : 0;
-  }
-  const int l = __builtin_ctzll(__ballot(lane < sequences && rank == r));
+  const int l = __builtin_ctzll(__ballot(lane < sequences && pf_rank(mine, sequences) == r));
   PfSequence p;
   p.q0 = pf_readlane64(mine.q0, l);
   p.k0 = pf_readlane64(mine.k0, l);
@@ -678,6 +685,12 @@ inline int ws_group(int nqb, int units8) {
   return pick;
 }
 
+// Packed prompts in chains: the blocks of an XCD's heads (the same for each head) in a list, sequence by sequence, those with
+// the most work and their longest blocks first, heads beside each other.  32 blocks at a time are dealt to its workgroups, the
+// longest to the one with the fewest tiles so far.  Every workgroup does that for itself from the lengths.
+constexpr int kWsRounds = 128;
+static_assert(kWsRounds * kWsPerXcd * 8 <= 2 * kWsK * kWsRow, "the list fits where K will be");
+
 // A query block of a workgroup at head dim 512, its chain's ``round``-th.
 struct WsBlock {
   int round, qb, h, b;
@@ -697,12 +710,23 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ float als[kWsQ];          // then: the factors O is rescaled by
   __shared__ float lsum[2][2][2][kWsQ];  // [parity of the block in the chain]: probability sums by key half, lane half
   __shared__ int moved[4];             // by tile % 4: a score passed the guard
+  constexpr bool kListed = kChain && kPacked;
+  __shared__ PfSequence seqs[kListed ? kWave : 1];
+  // The chain: sequence << 24 | query block << 12 | of the XCD's heads; -1 behind the last.
+  __shared__ int list[kListed ? kWsRounds : 1];
+  __shared__ uint32_t redo[4][kListed ? kWsRounds / 32 : 1];  // [value wave]: rounds with outputs that are not finite
   const int nqb = (a.width + kWsQ - 1) / kWsQ;
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (tid < 4) moved[tid] = 0;
   // The workgroup's block of a round, from its XCD's list; false past its end.
   auto place = [&](WsBlock& blk, int round) {
+    if constexpr (kListed) {
+      const int e = round < kWsRounds ? __builtin_amdgcn_readfirstlane(list[round]) : -1;
+      if (e < 0) return false;
+      blk = WsBlock{round, (e >> 12 & 0xfff) * kWsQ, (int)blockIdx.x % 8 * (a.H / 8) + (e & 0xfff), e >> 24};
+      return true;
+    }
     const int c = (int)blockIdx.x / 8;
     const int p = round * kWsPerXcd + (round & 1 ? kWsPerXcd - 1 - c : c);
     if (p >= a.units8 * nqb) return false;
@@ -714,7 +738,70 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   WsBlock only;  // packed: the one block of the workgroup, and its span
   PfSpan only_span;
   PfPacked one = {};
-  if constexpr (kPacked) {
+  if constexpr (kListed) {
+    {
+      const PfSequence one = pf_sequence(a, min(lane, a.sequences - 1));
+      const int rank = pf_rank(one, a.sequences);
+      if (w == 0 && lane < a.sequences) seqs[rank] = one;
+      if (tid < 4 * (kWsRounds / 32)) redo[0][tid] = 0;
+    }
+    lds_barrier();
+    // A lane's sequence, and its blocks: ``seen`` that see a key, of which ``upto`` come up to its end.
+    const PfSequence mine = seqs[min(lane, a.sequences - 1)];
+    const int nq = min(mine.nq, a.width), before = mine.nk - mine.nq;
+    const int blocks = lane < a.sequences ? (nq + kWsQ - 1) / kWsQ : 0;
+    const int blind = before >= 0 || blocks == 0 ? 0 : nq + before <= 0 ? blocks : min(blocks - 1, -before / kWsQ);
+    const int seen = blocks - blind, upto = wave_scan(seen);
+    const int members = a.H / 8, listed = __builtin_amdgcn_readlane(upto, kWave - 1) * members;
+    // Rounds of 32 blocks by their tiles, each wave some: twice the tiles and one for the start, and the block.
+    u32x2_t(*sorted)[kWsPerXcd] = reinterpret_cast<u32x2_t(*)[kWsPerXcd]>(&kls[0][0]);
+    auto of = [&](int from, int v) { return __builtin_amdgcn_ds_bpermute(from * 4, v); };
+    for (int round = w; round < kWsRounds && round * kWsPerXcd < listed; round += 8) {
+      const int p = round * kWsPerXcd + (lane & 31), i = p / members;
+      int s = 0;
+      for (int t = 0; t < a.sequences - 1; ++t) s += __builtin_amdgcn_readlane(upto, t) <= i ? 1 : 0;
+      const int j = of(s, blocks) - 1 - (i - (of(s, upto) - of(s, seen)));
+      const uint32_t tiles = (uint32_t)(min(kWsQ * (j + 1), of(s, nq)) + of(s, before) + kWsK - 1) / kWsK;
+      const uint32_t cost = p < listed ? 2 * tiles + 1 : 0;
+      int rank = 0;
+#pragma unroll 4
+      for (int t = 0; t < kWsPerXcd; ++t) {
+        const uint32_t other = __builtin_amdgcn_readlane(cost, t);
+        rank += other > cost || (other == cost && t < (lane & 31)) ? 1 : 0;
+      }
+      if (lane < kWsPerXcd) sorted[round][rank] = u32x2_t{cost, p < listed ? (uint32_t)(s << 24 | j << 12 | (p - i * members)) : ~0u};
+    }
+    // Blocks that see no key at all.
+    for (uint64_t with = __ballot(blind > 0); with; with &= with - 1) {
+      const int s = __builtin_ctzll(with), n = __builtin_amdgcn_readlane(blind, s);
+      const int64_t q0 = pf_readlane64(mine.q0, s), end = q0 + __builtin_amdgcn_readlane(nq, s);
+      for (int64_t i = blockIdx.x; i < (int64_t)n * a.H; i += gridDim.x) {
+        const int64_t at = q0 + i / a.H * kWsQ;
+        pf_zeros<D>(a, at, at + kWsQ < end ? at + kWsQ : end, (int)(i % a.H));
+      }
+    }
+    lds_barrier();
+    if (w == 0) {
+      uint32_t load = 0;  // of the XCD's workgroup lane % 32
+      for (int round = 0; round < kWsRounds; ++round) {
+        if (round * kWsPerXcd >= listed) {
+          if (lane == 0) list[round] = -1;
+          break;
+        }
+        int rank = 0;
+#pragma unroll 4
+        for (int t = 0; t < kWsPerXcd; ++t) {
+          const uint32_t other = __builtin_amdgcn_readlane(load, t);
+          rank += other < load || (other == load && t < (lane & 31)) ? 1 : 0;
+        }
+        const u32x2_t its = sorted[round][rank];
+        load += its[0];
+        if (lane == (int)blockIdx.x / 8) list[round] = (int)its[1];
+      }
+    }
+    lds_barrier();
+    if (list[0] < 0) return;
+  } else if constexpr (kPacked) {
     one = pf_packed_block(a, nqb, kWsQ, a.H, (int)gridDim.z / a.parts);
     only = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, 0};
     only_span = pf_packed_span(a, one.h, one.s);
@@ -726,10 +813,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   auto first = [&]() {
     WsBlock blk;
-    if constexpr (kPacked) {
-      blk = only;
-    } else if constexpr (kChain) {
+    if constexpr (kChain) {
       place(blk, 0);
+    } else if constexpr (kPacked) {
+      blk = only;
     } else {
       const PfBlock one = pf_block(nqb, a.H, (int)gridDim.z);
       blk = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, one.b};  // the longest blocks first
@@ -741,6 +828,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     return false;
   };
   auto span = [&](const WsBlock& blk) {
+    if constexpr (kListed) {
+      const PfSequence& s = seqs[blk.b];
+      return pf_packed_span(a, blk.h, PfSequence{pf_readlane64(s.q0, 0), pf_readlane64(s.k0, 0),
+                                                 __builtin_amdgcn_readfirstlane(s.nq),
+                                                 __builtin_amdgcn_readfirstlane(s.nk)});
+    }
     if constexpr (kPacked) return only_span;
     return pf_span<D>(a, blk.h, blk.b);
   };
@@ -842,7 +935,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         l_run += lt;
       }
       lsum[odd][kh][g][32 * qh + x] = l_run;
-      if (kPacked && pf_in_parts(one)) pf_leave_ml(a, one, w, g, x, m_ref, l_run);
+      if (kPacked && !kChain && pf_in_parts(one)) pf_leave_ml(a, one, w, g, x, m_ref, l_run);
       if (!next(blk)) break;
     }
     lds_barrier();
@@ -1005,7 +1098,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
     }
-    if (kPacked && __any(again)) pf_again<D>(a, sp, blk.h, blk.qb, 4, 128 * vw);
+    if (kPacked && __any(again)) {
+      if constexpr (kListed) redo[vw][blk.round >> 5] |= 1u << (blk.round & 31);
+      else pf_again<D>(a, sp, blk.h, blk.qb, 4, 128 * vw);
+    }
   };
   auto open = [&](WsTile& c) {  // the block's first tile
     const PfSpan sp = span(c.blk);
@@ -1076,8 +1172,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   attend_v(n - 1, nullptr);
   lds_barrier();
-  if (kPacked && pf_in_parts(one)) return pf_leave_o(a, one, vw, lane, only_span.nq - only.qb, o);
+  if (kPacked && !kChain && pf_in_parts(one)) return pf_leave_o(a, one, vw, lane, only_span.nq - only.qb, o);
   output(at.blk, odd);
+  if constexpr (kListed) {
+    WsBlock blk = first();
+    do {
+      if (redo[vw][blk.round >> 5] >> (blk.round & 31) & 1) pf_again<D>(a, span(blk), blk.h, blk.qb, 4, 128 * vw);
+    } while (next(blk));
+  }
 }
 
 // Head dim 128: 256 queries per workgroup, four pairs of a score wave and a value wave (see prefill_attn_ws_kernel), each
@@ -1766,6 +1868,12 @@ inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int longest
   return (int)std::min({kPartCus / blocks + 1, tiles / kPartLeast, (int64_t)kPartMost});
 }
 
+// Whether a launch at head dim 512 runs its blocks in chains.
+inline bool packed_chains(int64_t nqb, int heads, int sequences) {
+  const int64_t each = nqb * sequences * (heads / 8);  // blocks of an XCD, at most
+  return heads % 8 == 0 && sequences <= kWave && each >= 2 * kWsPerXcd && each <= kWsRounds * kWsPerXcd;
+}
+
 // Heads of a kv head in a block, and queries of a head.
 inline int packed_together(int head_dim, int heads_per_kv) {
   if (head_dim == 128) return heads_per_kv % 4 == 0 ? 4 : heads_per_kv % 2 == 0 ? 2 : 1;
@@ -2129,7 +2237,12 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
     omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
     if (a.parts > 1) omni::packed_attn_join_kernel<256><<<join, 256, 0, s>>>(a);
   } else {
-    omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
+    if (omni::packed_chains(grid.x, heads, sequences)) {
+      a.sequences = sequences;
+      omni::prefill_attn_ws_kernel<true, true><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);
+    } else {
+      omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
+    }
     if (a.parts > 1) omni::packed_attn_join_kernel<512><<<join, 256, 0, s>>>(a);
   }
   return omni_launch_status();
