@@ -8,7 +8,7 @@
 // keys [0, i + nk - nq] of nk.  What bounds a tile is the same; what they add is lengths from the device, rows of any stride, a
 // mask on every tile that not all of a wave's queries see, and at head dim 128 up to four heads of a kv head in a block (64
 // queries of each: a short prompt fills a block, and the heads share its tiles).  Measured, us: 8 prompts of 750-2400, 8 heads
-// x 512 213 (640 TFLOP/s), 32 over 8 x 128 200; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 80 (a head to a block
+// x 512 206 (666 TFLOP/s), 32 over 8 x 128 200; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 80 (a head to a block
 // 113); one of 1433, 32 x 128 42.
 #include <math.h>
 
@@ -687,7 +687,10 @@ inline int ws_group(int nqb, int units8) {
 
 // Packed prompts in chains: the blocks of an XCD's heads (the same for each head) in a list, sequence by sequence, those with
 // the most work and their longest blocks first, heads beside each other.  32 blocks at a time are dealt to its workgroups, the
-// longest to the one with the fewest tiles so far.  Every workgroup does that for itself from the lengths.
+// longest to the one with the fewest tiles so far.  Every workgroup does that for itself from the lengths, in ~3 us of a
+// launch.  Measured, us, blocks one by one and in chains, 8 heads: 8 prompts of 750-2400 225 / 206, of 2048 375 / 360, of 300-700
+// 59 / 52; 32 of 100-800 168 / 133, 64 of 20-600 229 / 171, 16 of up to 500 behind up to 900 keys 109 / 101; 8 of 3000-6000 1338 /
+// 1346, of 60-200 17.0 / 17.1.  Dealt there and back instead, groups of sequences each longest first: 223, 1445 for the longest.
 constexpr int kWsRounds = 128;
 static_assert(kWsRounds * kWsPerXcd * 8 <= 2 * kWsK * kWsRow, "the list fits where K will be");
 
@@ -1868,7 +1871,8 @@ inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int longest
   return (int)std::min({kPartCus / blocks + 1, tiles / kPartLeast, (int64_t)kPartMost});
 }
 
-// Whether a launch at head dim 512 runs its blocks in chains.
+// Whether a launch at head dim 512 runs its blocks in chains: where an XCD has two or more for each of its workgroups (no more
+// than their lists hold, and sequences that one wave's lanes hold), and the same heads for every sequence.
 inline bool packed_chains(int64_t nqb, int heads, int sequences) {
   const int64_t each = nqb * sequences * (heads / 8);  // blocks of an XCD, at most
   return heads % 8 == 0 && sequences <= kWave && each >= 2 * kWsPerXcd && each <= kWsRounds * kWsPerXcd;
