@@ -8,7 +8,7 @@
 // keys [0, i + nk - nq] of nk.  What bounds a tile is the same; what they add is lengths from the device, rows of any stride, a
 // mask on every tile that not all of a wave's queries see, and at head dim 128 up to four heads of a kv head in a block (64
 // queries of each: a short prompt fills a block, and the heads share its tiles).  Measured, us: 8 prompts of 750-2400, 8 heads
-// x 512 206 (666 TFLOP/s), 32 over 8 x 128 200; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 80 (a head to a block
+// x 512 195 (705 TFLOP/s), 32 over 8 x 128 175; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 80 (a head to a block
 // 113); one of 1433, 32 x 128 42.
 #include <math.h>
 
@@ -47,7 +47,7 @@ struct PrefillArgs {
   int parts = 1;
   float* part_o = nullptr;   // [part][value wave][query half u][r][e][k][lane][4]
   float* part_ml = nullptr;  // [part][score wave][lane half][query][2]
-  int sequences = 0;  // head dim 512 in chains
+  int sequences = 0;  // in chains
 };
 constexpr int kPartO = 4 * 32 * 256, kPartMl = 4 * 2 * 64 * 2;  // floats
 
@@ -688,11 +688,106 @@ inline int ws_group(int nqb, int units8) {
 // Packed prompts in chains: the blocks of an XCD's heads (the same for each head) in a list, sequence by sequence, those with
 // the most work and their longest blocks first, heads beside each other.  32 blocks at a time are dealt to its workgroups, the
 // longest to the one with the fewest tiles so far.  Every workgroup does that for itself from the lengths, in ~3 us of a
-// launch.  Measured, us, blocks one by one and in chains, 8 heads: 8 prompts of 750-2400 225 / 206, of 2048 375 / 360, of 300-700
-// 59 / 52; 32 of 100-800 168 / 133, 64 of 20-600 229 / 171, 16 of up to 500 behind up to 900 keys 109 / 101; 8 of 3000-6000 1338 /
-// 1346, of 60-200 17.0 / 17.1.  Dealt there and back instead, groups of sequences each longest first: 223, 1445 for the longest.
-constexpr int kWsRounds = 128;
-static_assert(kWsRounds * kWsPerXcd * 8 <= 2 * kWsK * kWsRow, "the list fits where K will be");
+// launch.
+// Measured, us, blocks one by one and in chains: 8 heads x 512, 8 prompts of 750-2400 218 / 195, of 300-700 59 / 52, 32 of 100-800
+// 169 / 133, 64 of 20-600 229 / 171, 8 of 3000-6000 1338 / 1346.  At head dim 128, where only the next block's first K tile is
+// brought beside a block's output: 32 heads, 4 of 2048 201 / 169, 64 of 20-600 258 / 216, 16 of up to 500 behind up to 900 keys
+// 106 / 91; 32 over 8 heads, 32 of 100-800 137 / 120, 16 of up to 500 behind up to 900 81 / 81, 8 of 3000-6000 1167 / 1200.  Dealt
+// there and back instead, groups of sequences each longest first (head dim 512): 8 of 750-2400 223, of 3000-6000 1445.
+constexpr int kPfRounds = 128;
+constexpr int kPfListBytes = kPfRounds * kWsPerXcd * 8;
+
+struct PfChain {
+  PfSequence seqs[kWave];  // by rank
+  int list[kPfRounds];     // the chain: sequence << 24 | query block << 12 | of the XCD's blocks of heads; -1 behind the last
+  uint32_t redo[4][kPfRounds / 32];  // [value wave]: rounds with outputs that are not finite
+};
+
+// Blocks of ``queries``, ``heads`` blocks of heads.  ``scratch``: kPfListBytes.  Queries of blocks that see no key are zeroed.
+template <int D>
+__device__ __forceinline__ void pf_chain(const PrefillArgs& a, int queries, int heads, PfChain& c, char* scratch) {
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  {
+    const PfSequence one = pf_sequence(a, min(lane, a.sequences - 1));
+    const int rank = pf_rank(one, a.sequences);
+    if (w == 0 && lane < a.sequences) c.seqs[rank] = one;
+    if (tid < 4 * (kPfRounds / 32)) c.redo[0][tid] = 0;
+  }
+  lds_barrier();
+  // A lane's sequence, and its blocks: ``seen`` that see a key, of which ``upto`` come up to its end.
+  const PfSequence mine = c.seqs[min(lane, a.sequences - 1)];
+  const int nq = min(mine.nq, a.width), before = mine.nk - mine.nq;
+  const int blocks = lane < a.sequences ? (nq + queries - 1) / queries : 0;
+  const int blind = before >= 0 || blocks == 0 ? 0 : nq + before <= 0 ? blocks : min(blocks - 1, -before / queries);
+  const int seen = blocks - blind, upto = wave_scan(seen);
+  const int members = heads / 8, listed = __builtin_amdgcn_readlane(upto, kWave - 1) * members;
+  // Rounds of 32 blocks by their time, each wave some.  (A tile of one 64-query group takes ~0.9 us, of four, at head dim 128,
+  // ~1.6; a start and end what half a tile takes.)
+  u32x2_t(*sorted)[kWsPerXcd] = reinterpret_cast<u32x2_t(*)[kWsPerXcd]>(scratch);
+  auto of = [&](int from, int v) { return __builtin_amdgcn_ds_bpermute(from * 4, v); };
+  for (int round = w; round < kPfRounds && round * kWsPerXcd < listed; round += 8) {
+    const int p = round * kWsPerXcd + (lane & 31), i = p / members;
+    int s = 0;
+    for (int t = 0; t < a.sequences - 1; ++t) s += __builtin_amdgcn_readlane(upto, t) <= i ? 1 : 0;
+    const int j = of(s, blocks) - 1 - (i - (of(s, upto) - of(s, seen)));
+    const int end = min(queries * (j + 1), of(s, nq)), groups = (end - queries * j + 63) / 64 * a.together;
+    const uint32_t tiles = (uint32_t)(end + of(s, before) + 63) / 64;
+    const uint32_t cost = p < listed ? tiles * (3 + groups) + 2 : 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int t = 0; t < kWsPerXcd; ++t) {
+      const uint32_t other = __builtin_amdgcn_readlane(cost, t);
+      rank += other > cost || (other == cost && t < (lane & 31)) ? 1 : 0;
+    }
+    if (lane < kWsPerXcd)
+      sorted[round][rank] = u32x2_t{cost, p < listed ? (uint32_t)(s << 24 | j << 12 | (p - i * members)) : ~0u};
+  }
+  // Blocks that see no key at all.
+  for (uint64_t with = __ballot(blind > 0); with; with &= with - 1) {
+    const int s = __builtin_ctzll(with), n = __builtin_amdgcn_readlane(blind, s);
+    const int64_t q0 = pf_readlane64(mine.q0, s), end = q0 + __builtin_amdgcn_readlane(nq, s);
+    for (int64_t i = blockIdx.x; i < (int64_t)n * a.H; i += gridDim.x) {
+      const int64_t at = q0 + i / a.H * queries;
+      pf_zeros<D>(a, at, at + queries < end ? at + queries : end, (int)(i % a.H));
+    }
+  }
+  lds_barrier();
+  if (w == 0) {
+    uint32_t load = 0;  // of the XCD's workgroup lane % 32
+    for (int round = 0; round < kPfRounds; ++round) {
+      if (round * kWsPerXcd >= listed) {
+        if (lane == 0) c.list[round] = -1;
+        break;
+      }
+      int rank = 0;
+#pragma unroll 4
+      for (int t = 0; t < kWsPerXcd; ++t) {
+        const uint32_t other = __builtin_amdgcn_readlane(load, t);
+        rank += other < load || (other == load && t < (lane & 31)) ? 1 : 0;
+      }
+      const u32x2_t its = sorted[round][rank];
+      load += its[0];
+      if (lane == (int)blockIdx.x / 8) c.list[round] = (int)its[1];
+    }
+  }
+  lds_barrier();
+}
+
+// The block of a round of the chain: sequence (by rank), query block, block of heads; false past its end.
+struct PfListed {
+  int s, j, h;
+};
+__device__ __forceinline__ bool pf_listed(const PfChain& c, int round, int heads, PfListed& at) {
+  const int e = round < kPfRounds ? __builtin_amdgcn_readfirstlane(c.list[round]) : -1;
+  if (e < 0) return false;
+  at = PfListed{e >> 24, e >> 12 & 0xfff, (int)blockIdx.x % 8 * (heads / 8) + (e & 0xfff)};
+  return true;
+}
+__device__ __forceinline__ PfSequence pf_of(const PfChain& c, int s) {
+  const PfSequence& q = c.seqs[s];
+  return PfSequence{pf_readlane64(q.q0, 0), pf_readlane64(q.k0, 0), __builtin_amdgcn_readfirstlane(q.nq),
+                    __builtin_amdgcn_readfirstlane(q.nk)};
+}
 
 // A query block of a workgroup at head dim 512, its chain's ``round``-th.
 struct WsBlock {
@@ -714,10 +809,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ float lsum[2][2][2][kWsQ];  // [parity of the block in the chain]: probability sums by key half, lane half
   __shared__ int moved[4];             // by tile % 4: a score passed the guard
   constexpr bool kListed = kChain && kPacked;
-  __shared__ PfSequence seqs[kListed ? kWave : 1];
-  // The chain: sequence << 24 | query block << 12 | of the XCD's heads; -1 behind the last.
-  __shared__ int list[kListed ? kWsRounds : 1];
-  __shared__ uint32_t redo[4][kListed ? kWsRounds / 32 : 1];  // [value wave]: rounds with outputs that are not finite
+  static_assert(kPfListBytes <= sizeof(kls), "");
+  __shared__ char chain_at[kListed ? sizeof(PfChain) : 1] __attribute__((aligned(16)));
+  PfChain& chain = *reinterpret_cast<PfChain*>(chain_at);
   const int nqb = (a.width + kWsQ - 1) / kWsQ;
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -725,9 +819,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // The workgroup's block of a round, from its XCD's list; false past its end.
   auto place = [&](WsBlock& blk, int round) {
     if constexpr (kListed) {
-      const int e = round < kWsRounds ? __builtin_amdgcn_readfirstlane(list[round]) : -1;
-      if (e < 0) return false;
-      blk = WsBlock{round, (e >> 12 & 0xfff) * kWsQ, (int)blockIdx.x % 8 * (a.H / 8) + (e & 0xfff), e >> 24};
+      PfListed at;
+      if (!pf_listed(chain, round, a.H, at)) return false;
+      blk = WsBlock{round, at.j * kWsQ, at.h, at.s};
       return true;
     }
     const int c = (int)blockIdx.x / 8;
@@ -742,68 +836,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   PfSpan only_span;
   PfPacked one = {};
   if constexpr (kListed) {
-    {
-      const PfSequence one = pf_sequence(a, min(lane, a.sequences - 1));
-      const int rank = pf_rank(one, a.sequences);
-      if (w == 0 && lane < a.sequences) seqs[rank] = one;
-      if (tid < 4 * (kWsRounds / 32)) redo[0][tid] = 0;
-    }
-    lds_barrier();
-    // A lane's sequence, and its blocks: ``seen`` that see a key, of which ``upto`` come up to its end.
-    const PfSequence mine = seqs[min(lane, a.sequences - 1)];
-    const int nq = min(mine.nq, a.width), before = mine.nk - mine.nq;
-    const int blocks = lane < a.sequences ? (nq + kWsQ - 1) / kWsQ : 0;
-    const int blind = before >= 0 || blocks == 0 ? 0 : nq + before <= 0 ? blocks : min(blocks - 1, -before / kWsQ);
-    const int seen = blocks - blind, upto = wave_scan(seen);
-    const int members = a.H / 8, listed = __builtin_amdgcn_readlane(upto, kWave - 1) * members;
-    // Rounds of 32 blocks by their tiles, each wave some: twice the tiles and one for the start, and the block.
-    u32x2_t(*sorted)[kWsPerXcd] = reinterpret_cast<u32x2_t(*)[kWsPerXcd]>(&kls[0][0]);
-    auto of = [&](int from, int v) { return __builtin_amdgcn_ds_bpermute(from * 4, v); };
-    for (int round = w; round < kWsRounds && round * kWsPerXcd < listed; round += 8) {
-      const int p = round * kWsPerXcd + (lane & 31), i = p / members;
-      int s = 0;
-      for (int t = 0; t < a.sequences - 1; ++t) s += __builtin_amdgcn_readlane(upto, t) <= i ? 1 : 0;
-      const int j = of(s, blocks) - 1 - (i - (of(s, upto) - of(s, seen)));
-      const uint32_t tiles = (uint32_t)(min(kWsQ * (j + 1), of(s, nq)) + of(s, before) + kWsK - 1) / kWsK;
-      const uint32_t cost = p < listed ? 2 * tiles + 1 : 0;
-      int rank = 0;
-#pragma unroll 4
-      for (int t = 0; t < kWsPerXcd; ++t) {
-        const uint32_t other = __builtin_amdgcn_readlane(cost, t);
-        rank += other > cost || (other == cost && t < (lane & 31)) ? 1 : 0;
-      }
-      if (lane < kWsPerXcd) sorted[round][rank] = u32x2_t{cost, p < listed ? (uint32_t)(s << 24 | j << 12 | (p - i * members)) : ~0u};
-    }
-    // Blocks that see no key at all.
-    for (uint64_t with = __ballot(blind > 0); with; with &= with - 1) {
-      const int s = __builtin_ctzll(with), n = __builtin_amdgcn_readlane(blind, s);
-      const int64_t q0 = pf_readlane64(mine.q0, s), end = q0 + __builtin_amdgcn_readlane(nq, s);
-      for (int64_t i = blockIdx.x; i < (int64_t)n * a.H; i += gridDim.x) {
-        const int64_t at = q0 + i / a.H * kWsQ;
-        pf_zeros<D>(a, at, at + kWsQ < end ? at + kWsQ : end, (int)(i % a.H));
-      }
-    }
-    lds_barrier();
-    if (w == 0) {
-      uint32_t load = 0;  // of the XCD's workgroup lane % 32
-      for (int round = 0; round < kWsRounds; ++round) {
-        if (round * kWsPerXcd >= listed) {
-          if (lane == 0) list[round] = -1;
-          break;
-        }
-        int rank = 0;
-#pragma unroll 4
-        for (int t = 0; t < kWsPerXcd; ++t) {
-          const uint32_t other = __builtin_amdgcn_readlane(load, t);
-          rank += other < load || (other == load && t < (lane & 31)) ? 1 : 0;
-        }
-        const u32x2_t its = sorted[round][rank];
-        load += its[0];
-        if (lane == (int)blockIdx.x / 8) list[round] = (int)its[1];
-      }
-    }
-    lds_barrier();
-    if (list[0] < 0) return;
+    pf_chain<D>(a, kWsQ, a.H, chain, &kls[0][0]);
+    if (chain.list[0] < 0) return;
   } else if constexpr (kPacked) {
     one = pf_packed_block(a, nqb, kWsQ, a.H, (int)gridDim.z / a.parts);
     only = WsBlock{0, (nqb - 1 - one.j) * kWsQ, one.h, 0};
@@ -832,10 +866,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   auto span = [&](const WsBlock& blk) {
     if constexpr (kListed) {
-      const PfSequence& s = seqs[blk.b];
-      return pf_packed_span(a, blk.h, PfSequence{pf_readlane64(s.q0, 0), pf_readlane64(s.k0, 0),
-                                                 __builtin_amdgcn_readfirstlane(s.nq),
-                                                 __builtin_amdgcn_readfirstlane(s.nk)});
+      return pf_packed_span(a, blk.h, pf_of(chain, blk.b));
     }
     if constexpr (kPacked) return only_span;
     return pf_span<D>(a, blk.h, blk.b);
@@ -1102,7 +1133,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
     }
     if (kPacked && __any(again)) {
-      if constexpr (kListed) redo[vw][blk.round >> 5] |= 1u << (blk.round & 31);
+      if constexpr (kListed) chain.redo[vw][blk.round >> 5] |= 1u << (blk.round & 31);
       else pf_again<D>(a, sp, blk.h, blk.qb, 4, 128 * vw);
     }
   };
@@ -1180,7 +1211,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   if constexpr (kListed) {
     WsBlock blk = first();
     do {
-      if (redo[vw][blk.round >> 5] >> (blk.round & 31) & 1) pf_again<D>(a, span(blk), blk.h, blk.qb, 4, 128 * vw);
+      if (chain.redo[vw][blk.round >> 5] >> (blk.round & 31) & 1) pf_again<D>(a, span(blk), blk.h, blk.qb, 4, 128 * vw);
     } while (next(blk));
   }
 }
@@ -1211,7 +1242,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-template <bool kPacked>
+// kChain (packed): a workgroup runs a list of blocks, see pf_chain.
+template <bool kPacked, bool kChain>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill_attn_pairs_kernel(
     PrefillArgs a) {
   constexpr int D = 128;
@@ -1221,46 +1253,63 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ float als[4][4][64];         // [pair][tile % 4]: O's factors, when the reference moved
   __shared__ int moved[4][4];
   __shared__ float lsum[4][2][64];        // [pair][lane half]
+  static_assert(kPfListBytes <= sizeof(kls), "");
+  __shared__ char chain_at[kChain ? sizeof(PfChain) : 1] __attribute__((aligned(16)));
+  PfChain& chain = *reinterpret_cast<PfChain*>(chain_at);
   // The pairs' 64 queries: of one head one after another, or (packed) of 2 or 4 heads that read the same keys.
   const int together = kPacked ? a.together : 1, queries = kPairQ / together;
   const int nqb = (a.width + queries - 1) / queries;
-  int j, hb, b = 0;
-  PfPacked one = {};
-  if constexpr (kPacked) {
-    one = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z / a.parts);
-    j = one.j;
-    hb = one.h;
-  } else {
-    const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
-    j = blk.j;
-    hb = blk.h;
-    b = blk.b;
-  }
-  const int qb = (nqb - 1 - j) * queries;  // the longest blocks first
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), pr = w & 3;
-  const int h = kPacked ? hb * together + pr % together : hb;
+  PfPacked one = {};
   PfSpan sp;
-  if constexpr (kPacked) sp = pf_packed_span(a, h, one.s);
-  else sp = pf_span<D>(a, h, b);
-  int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees (packed: of the part's)
-  if constexpr (kPacked) {
+  int qb, h, keys;  // the block's first query, the pair's head, what the block's last query sees (packed: of the part's)
+  // The chain's block of ``round``; false past its end.
+  auto enter = [&](int round) {
+    PfListed at;
+    if (!pf_listed(chain, round, a.H / together, at)) return false;
+    qb = at.j * queries;
+    h = at.h * together + pr % together;
+    sp = pf_packed_span(a, h, pf_of(chain, at.s));
+    keys = min(qb + queries, sp.nq) + sp.before;
+    return true;
+  };
+  if constexpr (kChain) {
+    pf_chain<D>(a, queries, a.H / together, chain, &kls[0][0]);
+    if (!enter(0)) return;
+  } else if constexpr (kPacked) {
+    one = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z / a.parts);
+    qb = (nqb - 1 - one.j) * queries;  // the longest blocks first
+    h = one.h * together + pr % together;
+    sp = pf_packed_span(a, h, one.s);
+    keys = min(qb + queries, sp.nq) + sp.before;
     if (qb >= sp.nq) return;
     if (!pf_part(a, one, sp, keys)) return;
     if (keys <= 0) {
       for (int i = 0; i < together; ++i)
-        pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), hb * together + i);
+        pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), one.h * together + i);
       return;
     }
+  } else {
+    const PfBlock blk = pf_block(nqb, a.H, (int)gridDim.z);
+    qb = (nqb - 1 - blk.j) * queries;
+    h = blk.h;
+    sp = pf_span<D>(a, h, blk.b);
+    keys = min(qb + queries, sp.nq) + sp.before;
   }
-  const char* kbase = scalar_pointer(sp.k);
-  const char* vbase = scalar_pointer(sp.v);
-  const int nt = (keys + kPairK - 1) / kPairK;
-  const int qp = qb + 64 * (kPacked ? pr / together : pr);
-  // The pair's last tile, which holds its diagonal (-1: no queries, or they see no key).
-  const int lastk = kPacked ? min(min(qp + 64, sp.nq) + sp.before, keys) - 1 : qp;
-  const int dq = qp < sp.nq && lastk >= 0 ? lastk / kPairK : -1;
-  const int whole = qp + sp.before;  // every query of the pair sees keys [0, whole]
+  const char *kbase, *vbase;
+  int nt, qp, dq, whole;  // tiles; the pair's first query, its last tile, and the last key that all its queries see
+  auto derive = [&]() {
+    kbase = scalar_pointer(sp.k);
+    vbase = scalar_pointer(sp.v);
+    nt = (keys + kPairK - 1) / kPairK;
+    qp = qb + 64 * (kPacked ? pr / together : pr);
+    // The pair's last tile holds its diagonal (-1: no queries, or they see no key).
+    const int lastk = kPacked ? min(min(qp + 64, sp.nq) + sp.before, keys) - 1 : qp;
+    dq = qp < sp.nq && lastk >= 0 ? lastk / kPairK : -1;
+    whole = qp + sp.before;
+  };
+  derive();
 
   // Rows 16 pr .. + 15 of tile t to LDS; rows past the context read its last key (finite: masked).  ``swap``: the chunk
   // permutation of key row r of a 16-row group.
@@ -1281,145 +1330,151 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   if (w < 4) {  // ------------------------------------------------------------------------------ scores
     auto bring_v = [&](int t) { bring(vbase, sp.v_bytes, vls[t & 1], t, [](int r) { return 4 * (r & 3); }); };
-    u32x4_t q[2][D / 16];  // q[query][16s + 8g .. + 7], query qp + 32u + x
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint16_t* qrow =
-          a.q + ((sp.q0 + min(qp + 32 * u + x, sp.nq - 1)) * a.H + h) * D + g * 8;
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) q[u][s] = *reinterpret_cast<const u32x4_t*>(qrow + s * 16);
-    }
-    float m_ref[2] = {-INFINITY, -INFINITY}, thr[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-    const int klane = x * (D * 2) + ((g ^ (x & 15)) * 16);
-    auto k_at = [&](int t, int m, int s) {
-      return *reinterpret_cast<const u32x4_t*>(&kls[t & 1][32 * m * (D * 2) + (klane ^ (32 * s))]);
-    };
-    typedef f32x16_t Scores[2][2];  // [key half m][query half u]
-    f32x16_t zero;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-    // One 16-key step's probabilities of query half u: keys 16 (2m + hf) .., as the value wave's operand.
-    auto put_p = [&](const Scores& sc, int t, int m, int hf, int u, float mu) {
-      u32x4_t pop;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][u][8 * hf + 2 * e], a.scale_log2, -mu));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][u][8 * hf + 2 * e + 1], a.scale_log2, -mu));
-        l_run[u] += p0 + p1;
-        pop[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
-      }
-      ps[pr][t & 1][u][2 * m + hf][lane] = pop;
-    };
-    // The reference of tile t's scores (masked on the pair's last tile).
-    auto refer = [&](Scores& sc, int t) {
-      // max3's operands come from the matrix unit: every product has written its result after 24 wait states.
-      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sc[0][0]), "+v"(sc[0][1]), "+v"(sc[1][0]), "+v"(sc[1][1]));
-      if (kPacked ? t * kPairK + kPairK - 1 > whole : t == dq) {
-        const int off = kPacked ? whole - t * kPairK : 0;
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int rel = off + 32 * u + x - (32 * m + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sc[m][u][i] = 8 * (i >> 2) + (i & 3) <= rel ? sc[m][u][i] : -INFINITY;
-          }
-      }
-      float mx[2];
+    for (int round = 0;; ++round) {
+      u32x4_t q[2][D / 16];  // q[query][16s + 8g .. + 7], query qp + 32u + x
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        mx[u] = max3(sc[0][u][0], sc[1][u][0], sc[0][u][1]);
-        mx[u] = max3(mx[u], sc[1][u][1], sc[1][u][1]);
+        const uint16_t* qrow =
+            a.q + ((sp.q0 + min(qp + 32 * u + x, sp.nq - 1)) * a.H + h) * D + g * 8;
 #pragma unroll
-        for (int i = 2; i < 16; ++i) mx[u] = max3(mx[u], sc[0][u][i], sc[1][u][i]);
+        for (int s = 0; s < D / 16; ++s) q[u][s] = *reinterpret_cast<const u32x4_t*>(qrow + s * 16);
       }
-      const bool move = __any(mx[0] > thr[0] || mx[1] > thr[1]);
-      if (lane == 0) moved[pr][t & 3] = move ? 1 : 0;
-      if (move) {
+      float m_ref[2] = {-INFINITY, -INFINITY}, thr[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+      const int klane = x * (D * 2) + ((g ^ (x & 15)) * 16);
+      auto k_at = [&](int t, int m, int s) {
+        return *reinterpret_cast<const u32x4_t*>(&kls[t & 1][32 * m * (D * 2) + (klane ^ (32 * s))]);
+      };
+      typedef f32x16_t Scores[2][2];  // [key half m][query half u]
+      f32x16_t zero;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+      // One 16-key step's probabilities of query half u: keys 16 (2m + hf) .., as the value wave's operand.
+      auto put_p = [&](const Scores& sc, int t, int m, int hf, int u, float mu) {
+        u32x4_t pop;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][u][8 * hf + 2 * e], a.scale_log2, -mu));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][u][8 * hf + 2 * e + 1], a.scale_log2, -mu));
+          l_run[u] += p0 + p1;
+          pop[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
+        }
+        ps[pr][t & 1][u][2 * m + hf][lane] = pop;
+      };
+      // The reference of tile t's scores (masked on the pair's last tile).
+      auto refer = [&](Scores& sc, int t) {
+        // max3's operands come from the matrix unit: every product has written its result after 24 wait states.
+        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sc[0][0]), "+v"(sc[0][1]), "+v"(sc[1][0]), "+v"(sc[1][1]));
+        if (kPacked ? t * kPairK + kPairK - 1 > whole : t == dq) {
+          const int off = kPacked ? whole - t * kPairK : 0;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int rel = off + 32 * u + x - (32 * m + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sc[m][u][i] = 8 * (i >> 2) + (i & 3) <= rel ? sc[m][u][i] : -INFINITY;
+            }
+        }
+        float mx[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float top = fmaxf(mx[u], __shfl_xor(mx[u], 32, kWave));
-          const float m_new = fmaxf(m_ref[u], top * a.scale_log2);
-          const float alpha = __builtin_amdgcn_exp2f(m_ref[u] - (m_new == -INFINITY ? 0.f : m_new));  // m_ref = -inf: 0
-          if (g == 0) als[pr][t & 3][32 * u + x] = alpha;
-          l_run[u] *= alpha;
-          m_ref[u] = m_new;
-          thr[u] = m_new == -INFINITY ? -INFINITY : (m_new + kWsGuard) / a.scale_log2;
+          mx[u] = max3(sc[0][u][0], sc[1][u][0], sc[0][u][1]);
+          mx[u] = max3(mx[u], sc[1][u][1], sc[1][u][1]);
+#pragma unroll
+          for (int i = 2; i < 16; ++i) mx[u] = max3(mx[u], sc[0][u][i], sc[1][u][i]);
         }
-      }
-    };
-    // Step t: tile t's products into ``to``, the softmax of tile t - 1's scores ``from`` beside them.
-    auto step = [&](const Scores& from, Scores& to, int t, bool soft) {
-      u32x4_t kf[2] = {k_at(t, 0, 0), k_at(t, 1, 0)};
-      const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
+        const bool move = __any(mx[0] > thr[0] || mx[1] > thr[1]);
+        if (lane == 0) moved[pr][t & 3] = move ? 1 : 0;
+        if (move) {
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) to[m][u] = mfma32(kf[m], q[u][s], s == 0 ? zero : to[m][u]);
-        if (s + 1 < D / 16) {
-#pragma unroll
-          for (int m = 0; m < 2; ++m) kf[m] = k_at(t, m, s + 1);
+          for (int u = 0; u < 2; ++u) {
+            const float top = fmaxf(mx[u], __shfl_xor(mx[u], 32, kWave));
+            const float m_new = fmaxf(m_ref[u], top * a.scale_log2);
+            const float alpha = __builtin_amdgcn_exp2f(m_ref[u] - (m_new == -INFINITY ? 0.f : m_new));  // m_ref = -inf: 0
+            if (g == 0) als[pr][t & 3][32 * u + x] = alpha;
+            l_run[u] *= alpha;
+            m_ref[u] = m_new;
+            thr[u] = m_new == -INFINITY ? -INFINITY : (m_new + kWsGuard) / a.scale_log2;
+          }
         }
-        if (soft) put_p(from, t - 1, s >> 2, (s >> 1) & 1, s & 1, s & 1 ? m1 : m0);
+      };
+      // Step t: tile t's products into ``to``, the softmax of tile t - 1's scores ``from`` beside them.
+      auto step = [&](const Scores& from, Scores& to, int t, bool soft) {
+        u32x4_t kf[2] = {k_at(t, 0, 0), k_at(t, 1, 0)};
+        const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) to[m][u] = mfma32(kf[m], q[u][s], s == 0 ? zero : to[m][u]);
+          if (s + 1 < D / 16) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) kf[m] = k_at(t, m, s + 1);
+          }
+          if (soft) put_p(from, t - 1, s >> 2, (s >> 1) & 1, s & 1, s & 1 ? m1 : m0);
+        }
+        refer(to, t);
+      };
+      auto finish = [&](const Scores& from, int t) {  // the pair's last tile
+        const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) put_p(from, t, s >> 2, (s >> 1) & 1, s & 1, s & 1 ? m1 : m0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) lsum[pr][g][32 * u + x] = l_run[u];
+      };
+      Scores sa, sb;
+      lds_barrier();  // the first K tile (these waves have brought nothing yet)
+      if (dq >= 0) step(sb, sa, 0, false);
+      lds_barrier();
+      int t = 1;
+      for (; t + 1 <= dq; t += 2) {
+        bring_v(t - 1);
+        step(sa, sb, t, true);
+        landed_barrier();
+        bring_v(t);
+        step(sb, sa, t + 1, true);
+        landed_barrier();
       }
-      refer(to, t);
-    };
-    auto finish = [&](const Scores& from, int t) {  // the pair's last tile
-      const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
+      if (t <= dq) {  // one more, then its scores are in sb
+        bring_v(t - 1);
+        step(sa, sb, t, true);
+        landed_barrier();
+        bring_v(t);
+        finish(sb, t);
+        landed_barrier();
+        t += 2;
+      } else if (dq >= 0) {
+        bring_v(t - 1);
+        finish(sa, t - 1);
+        landed_barrier();
+        t += 1;
+      }
+      for (; t <= nt + 1; ++t) {
+        if (t <= nt) bring_v(t - 1);
+        landed_barrier();
+      }
+      if (kPacked && pf_in_parts(one)) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) put_p(from, t, s >> 2, (s >> 1) & 1, s & 1, s & 1 ? m1 : m0);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) lsum[pr][g][32 * u + x] = l_run[u];
-    };
-    Scores sa, sb;
-    lds_barrier();  // the first K tile (these waves have brought nothing yet)
-    if (dq >= 0) step(sb, sa, 0, false);
-    lds_barrier();
-    int t = 1;
-    for (; t + 1 <= dq; t += 2) {
-      bring_v(t - 1);
-      step(sa, sb, t, true);
-      landed_barrier();
-      bring_v(t);
-      step(sb, sa, t + 1, true);
-      landed_barrier();
+        for (int u = 0; u < 2; ++u) pf_leave_ml(a, one, pr, g, 32 * u + x, m_ref[u], l_run[u]);
+      }
+      if (!kChain || !enter(round + 1)) return;
+      derive();
     }
-    if (t <= dq) {  // one more, then its scores are in sb
-      bring_v(t - 1);
-      step(sa, sb, t, true);
-      landed_barrier();
-      bring_v(t);
-      finish(sb, t);
-      landed_barrier();
-      t += 2;
-    } else if (dq >= 0) {
-      bring_v(t - 1);
-      finish(sa, t - 1);
-      landed_barrier();
-      t += 1;
-    }
-    for (; t <= nt + 1; ++t) {
-      if (t <= nt) bring_v(t - 1);
-      landed_barrier();
-    }
-    if (kPacked && pf_in_parts(one)) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) pf_leave_ml(a, one, pr, g, 32 * u + x, m_ref[u], l_run[u]);
-    }
-    return;
   }
 
   // ---------------------------------------------------------------------------------------------- values
   auto bring_k = [&](int t) { bring(kbase, sp.k_bytes, kls[t & 1], t, [](int r) { return r; }); };
   f32x16_t o[2][4];  // [query half][e]: row 16k + 4q + i is dimension 32e + 8q + 4k + i, column x query x of the half
+  auto clear = [&]() {
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
+        for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
+  };
+  clear();
   // V operands by transpose reads: within 16 lanes (k = lane / 16 % 2), lane 4r + q points at key 4g + r, dimensions
   // 32e + 8q + 4k .., and lane 4q + i receives dimension 32e + 8q + 4k + i of the four keys.
   const int r = (lane & 15) >> 2, q4 = lane & 3, k2 = (lane >> 4) & 1;
@@ -1455,44 +1510,70 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int u = 0; u < 2; ++u) o[u][e] = mfma32(vop, p[u][s], o[u][e]);
       }
   };
+  // O of a block's queries from ``first``; whether some is not finite.
+  auto output = [&](const PfSpan& s, int head, int first, int d) {
+    bool again = false;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int query = first + 32 * u + x;
+      if (query >= s.nq) continue;
+      const float l = kPacked && d < 0 ? 0.f : lsum[pr][0][32 * u + x] + lsum[pr][1][32 * u + x];
+      const float inv = l > 0.f ? 1.f / l : 1.f;
+      uint16_t* orow = a.out + ((s.q0 + query) * a.H + head) * D + 8 * g;
+      auto pair = [&](float lo, float hi) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
+      };
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {  // dimensions 32e + 16 rb + 8g .. + 7
+          u32x4_t out;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int at = 4 * (rb + 2 * k);
+            out[2 * k] = pair(o[u][e][at], o[u][e][at + 1]);
+            out[2 * k + 1] = pair(o[u][e][at + 2], o[u][e][at + 3]);
+          }
+          *reinterpret_cast<u32x4_t*>(orow + 32 * e + 16 * rb) = out;
+          if constexpr (kPacked) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) again |= pf_nonfinite(out[i]);
+          }
+        }
+    }
+    return again;
+  };
   bring_k(0);
   landed_barrier();
-  for (int t = 0; t <= nt + 1; ++t) {
-    if (t + 1 < nt) bring_k(t + 1);
-    if (t >= 2 && t - 2 <= dq) attend_v(t - 2);
-    landed_barrier();
-  }
-  if (kPacked && pf_in_parts(one)) return pf_leave_o(a, one, pr, lane, sp.nq - qp, o);
-  bool again = false;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int query = qp + 32 * u + x;
-    if (query >= sp.nq) continue;
-    const float l = kPacked && dq < 0 ? 0.f : lsum[pr][0][32 * u + x] + lsum[pr][1][32 * u + x];
-    const float inv = l > 0.f ? 1.f / l : 1.f;
-    uint16_t* orow = a.out + ((sp.q0 + query) * a.H + h) * D + 8 * g;
-    auto pair = [&](float lo, float hi) {
-      return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
-    };
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {  // dimensions 32e + 16 rb + 8g .. + 7
-        u32x4_t out;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int at = 4 * (rb + 2 * k);
-          out[2 * k] = pair(o[u][e][at], o[u][e][at + 1]);
-          out[2 * k + 1] = pair(o[u][e][at + 2], o[u][e][at + 3]);
-        }
-        *reinterpret_cast<u32x4_t*>(orow + 32 * e + 16 * rb) = out;
-        if constexpr (kPacked) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) again |= pf_nonfinite(out[i]);
-        }
+  for (int round = 0;; ++round) {
+    for (int t = 0; t <= nt + 1; ++t) {
+      if (t + 1 < nt) bring_k(t + 1);
+      if (t >= 2 && t - 2 <= dq) attend_v(t - 2);
+      landed_barrier();
+    }
+    if constexpr (kChain) {
+      // The next block's first K tile on its way (the score waves are past their last one) beside this block's output.
+      const PfSpan was = sp;
+      const int head = h, first = qp, d = dq;
+      const bool more = enter(round + 1);
+      if (more) {
+        derive();
+        bring_k(0);
       }
+      if (__any(output(was, head, first, d))) chain.redo[pr][round >> 5] |= 1u << (round & 31);
+      if (!more) break;
+      clear();
+      landed_barrier();
+    } else {
+      if (kPacked && pf_in_parts(one)) return pf_leave_o(a, one, pr, lane, sp.nq - qp, o);
+      if (__any(output(sp, h, qp, dq)) && kPacked) pf_again<D>(a, sp, h, qp, 4, 0);
+      return;
+    }
   }
-  if (kPacked && __any(again)) pf_again<D>(a, sp, h, qp, 4, 0);
+  for (int round = 0; enter(round); ++round) {
+    derive();
+    if (chain.redo[pr][round >> 5] >> (round & 31) & 1) pf_again<D>(a, sp, h, qp, 4, 0);
+  }
 }
 
 // Packed prompts at head dim 256: 128 queries and 64-key tiles per workgroup of 8 waves, in two groups of 64 queries, of one
@@ -1871,11 +1952,13 @@ inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int longest
   return (int)std::min({kPartCus / blocks + 1, tiles / kPartLeast, (int64_t)kPartMost});
 }
 
-// Whether a launch at head dim 512 runs its blocks in chains: where an XCD has two or more for each of its workgroups (no more
-// than their lists hold, and sequences that one wave's lanes hold), and the same heads for every sequence.
-inline bool packed_chains(int64_t nqb, int heads, int sequences) {
+// Whether a launch runs its blocks in chains: where an XCD has two (head dim 128: three; 10 of 260-300, 32 heads, 2.5 for each,
+// take 48 us in place of 45.5) or more for each of its workgroups (no more than their lists hold, and sequences that one wave's
+// lanes hold), and the same ``heads`` blocks of heads for every sequence.
+inline bool packed_chains(int64_t nqb, int heads, int sequences, int head_dim) {
   const int64_t each = nqb * sequences * (heads / 8);  // blocks of an XCD, at most
-  return heads % 8 == 0 && sequences <= kWave && each >= 2 * kWsPerXcd && each <= kWsRounds * kWsPerXcd;
+  return heads % 8 == 0 && sequences <= kWave && each >= (head_dim == 512 ? 2 : 3) * kWsPerXcd &&
+         each <= kPfRounds * kWsPerXcd;
 }
 
 // Heads of a kv head in a block, and queries of a head.
@@ -2146,7 +2229,7 @@ extern "C" int omni_prefill_attention(const void* q, const void* k_cache, const 
       omni::prefill_attn_kernel<<<grid, omni::kPfThreads, 0, s>>>(a);
     } else {
       dim3 grid((width + omni::kPairQ - 1) / omni::kPairQ, heads, contexts);
-      omni::prefill_attn_pairs_kernel<false><<<grid, 512, 0, s>>>(a);
+      omni::prefill_attn_pairs_kernel<false, false><<<grid, 512, 0, s>>>(a);
     }
   } else if (head_dim == 512) {
     const int nqb = (width + omni::kWsQ - 1) / omni::kWsQ, units = heads * contexts;
@@ -2231,22 +2314,21 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
     a.part_o = (float*)workspace;
     a.part_ml = a.part_o + blocks * a.parts * omni::kPartO;
   }
+  const bool chains = omni::packed_chains(grid.x, grid.y, sequences, head_dim);
+  a.sequences = sequences;
   const dim3 join(grid.x * 4, grid.y, grid.z);
   grid.z *= a.parts;
   const hipStream_t s = (hipStream_t)stream;
   if (head_dim == 128) {
-    omni::prefill_attn_pairs_kernel<true><<<grid, 512, 0, s>>>(a);
+    if (chains) omni::prefill_attn_pairs_kernel<true, true><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);
+    else omni::prefill_attn_pairs_kernel<true, false><<<grid, 512, 0, s>>>(a);
     if (a.parts > 1) omni::packed_attn_join_kernel<128><<<join, 256, 0, s>>>(a);
   } else if (head_dim == 256) {
     omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
     if (a.parts > 1) omni::packed_attn_join_kernel<256><<<join, 256, 0, s>>>(a);
   } else {
-    if (omni::packed_chains(grid.x, heads, sequences)) {
-      a.sequences = sequences;
-      omni::prefill_attn_ws_kernel<true, true><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);
-    } else {
-      omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
-    }
+    if (chains) omni::prefill_attn_ws_kernel<true, true><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);
+    else omni::prefill_attn_ws_kernel<false, true><<<grid, 512, 0, s>>>(a);
     if (a.parts > 1) omni::packed_attn_join_kernel<512><<<join, 256, 0, s>>>(a);
   }
   return omni_launch_status();

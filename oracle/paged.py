@@ -57,15 +57,15 @@ def softmax_product(q, k, v, scale: float, limit):
     """q [T, D], k / v [N, D]; query t sees keys [0, limit[t]).  (out, sum of weights |v|), float64; none: zeros.  Keys and
     values that a query does not see take no part, whatever they hold."""
     q, k, v = q.double(), k.double(), v.double()
-    out = torch.zeros(q.size(0), v.size(1), dtype=torch.float64, device=q.device)
-    size = torch.zeros_like(out)
-    for t, n in enumerate(int(x) for x in limit):
-        n = min(n, k.size(0))
-        if n <= 0:
-            continue
-        w = torch.softmax((k[:n] @ q[t]) * scale, 0)
-        out[t] = w @ v[:n]
-        size[t] = w @ v[:n].abs()
+    limit = torch.tensor([int(x) for x in limit], device=q.device)
+    seen = torch.arange(k.size(0), device=q.device) < limit[:, None]
+    w = torch.softmax(((q @ k.T) * scale).masked_fill(~seen, -torch.inf), 1).masked_fill(~seen, 0.0)
+    fine = v.isfinite()
+    kept = v.masked_fill(~fine, 0.0)
+    out, size = w @ kept, w @ kept.abs()
+    for n in (~fine).any(1).nonzero().flatten().tolist():  # an infinity or NaN, to the queries that see it
+        out[seen[:, n]] += v[n].masked_fill(fine[n], 0.0)
+        size[seen[:, n]] += v[n].masked_fill(fine[n], 0.0).abs()
     return out, size
 
 

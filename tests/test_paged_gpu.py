@@ -422,25 +422,30 @@ def test_packed_attention_head_counts(cuda, heads, kv, dim):
     packed_case(cuda, heads, kv, dim, [70, 1, 0, 150], [0, 40, 3, 9], heads + kv)
 
 
-@pytest.mark.parametrize("heads,kv", [(8, 8), (16, 2), (24, 3)])
-def test_packed_attention_in_chains(cuda, heads, kv):
-    """Head dim 512 with many blocks for each workgroup: one after another, of sequences long, short and empty, behind
-    earlier keys and before the first key."""
-    packed_case(cuda, heads, kv, 512, [400, 0, 64, 65, 1, 127, 300, 20, 33, 192, 257, 5], 0, heads, behind=9)
-    packed_case(cuda, heads, kv, 512, [400, 0, 64, 65, 1, 127, 300, 20, 33, 192, 257, 5],
-                [30, 7, -64, -65, 500, -100, -290, 64, 0, 1, -10, 2000], heads + 1, strided=False)
-    packed_case(cuda, heads, kv, 512, [(37 * i) % 130 for i in range(64)], [(11 * i) % 90 for i in range(64)], heads + 2)
-    packed_case(cuda, heads, kv, 512, [3, 2], 0, heads + 3, longest=5000, behind=4995)
-    packed_case(cuda, heads, kv, 512, [0, 0, 0], 0, heads + 4, longest=5000, behind=4995)
-    packed_case(cuda, heads, kv, 512, [700, 900], [-700, -901], heads + 5, longest=4000, behind=2400)
+CHAINED = [(8, 8, 512), (16, 2, 512), (24, 3, 512), (32, 8, 128), (16, 8, 128), (32, 32, 128), (24, 24, 128)]
 
 
-def test_packed_attention_in_chains_up_to_longest(cuda):
+@pytest.mark.parametrize("heads,kv,dim", CHAINED)
+def test_packed_attention_in_chains(cuda, heads, kv, dim):
+    """Many blocks for each workgroup: one after another, of sequences long, short and empty, behind earlier keys and before
+    the first key."""
+    packed_case(cuda, heads, kv, dim, [400, 0, 64, 65, 1, 127, 300, 20, 33, 192, 257, 5] * 2, 0, heads, behind=9)
+    packed_case(cuda, heads, kv, dim, [400, 0, 64, 65, 1, 127, 300, 20, 33, 192, 257, 5] * 2,
+                [30, 7, -64, -65, 500, -100, -290, 64, 0, 1, -10, 2000] * 2, heads + 1, strided=False)
+    packed_case(cuda, heads, kv, dim, [(37 * i) % 130 for i in range(64)], [(11 * i) % 90 for i in range(64)], heads + 2,
+                longest=300)
+    packed_case(cuda, heads, kv, dim, [3, 2], 0, heads + 3, longest=5000, behind=4995)
+    packed_case(cuda, heads, kv, dim, [0, 0, 0], 0, heads + 4, longest=5000, behind=4995)
+    packed_case(cuda, heads, kv, dim, [700, 900], [-700, -901], heads + 5, longest=4000, behind=2400)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (32, 8, 128), (32, 32, 128)])
+def test_packed_attention_in_chains_up_to_longest(cuda, heads, kv, dim):
     """Queries past ``longest`` of a sequence are not computed, the others see what they see."""
     g, counts = gen(51), [300, 40, 129, 64, 200, 10, 70, 90, 100, 128, 192, 1, 2, 3, 65, 66]
     starts = torch.tensor([0, *counts]).cumsum(0)
     n = int(starts[-1])
-    q, k, v = (normal((n, 8, 512), g, cuda) for _ in "qkv")
+    q, k, v = (normal((n, h, dim), g, cuda) for h in (heads, kv, kv))
     out = torch.full_like(q, 7.0)
     kernels.packed_attention(q, k, v, starts.to(cuda), 256, 0.05, out=out)
     want = kernels.packed_attention(q, k, v, starts.to(cuda), 300, 0.05)
@@ -453,14 +458,15 @@ def test_packed_attention_in_chains_up_to_longest(cuda):
     assert torch.equal(out[kept], want[kept]) and (out[~kept] == 7.0).all()
 
 
-def test_packed_attention_in_chains_does_not_see_what_is_masked(cuda):
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 512), (32, 8, 128), (32, 32, 128)])
+def test_packed_attention_in_chains_does_not_see_what_is_masked(cuda, heads, kv, dim):
     g, counts = gen(52), [300, 90, 129, 64, 200, 10, 70, 90, 100, 128, 192, 1, 2, 3, 65, 66]
     starts = torch.tensor([0, *counts]).cumsum(0)
     n = int(starts[-1])
-    q, k, v = normal((n, 8, 512), g, cuda), normal((n, 2, 512), g, cuda), normal((n, 2, 512), g, cuda)
+    q, k, v = normal((n, heads, dim), g, cuda), normal((n, kv, dim), g, cuda), normal((n, kv, dim), g, cuda)
     for s, at in ((0, 250), (1, 70), (2, 128), (8, 99), (11, 0), (15, 30)):
         row = int(starts[s]) + at
-        v[row, 0, 3], v[row, 1, 200], v[row, 1, 511] = float("inf"), float("nan"), float("-inf")
+        v[row, 0, 3], v[row, 1, dim // 2], v[row, 1, dim - 1] = float("inf"), float("nan"), float("-inf")
     k[int(starts[4]) + 150, 1, 9] = float("nan")
     out = [kernels.packed_attention(q, k, v, starts.to(cuda), 300, 0.05) for _ in range(3)]
     torch.cuda.synchronize()
@@ -469,13 +475,14 @@ def test_packed_attention_in_chains_does_not_see_what_is_masked(cuda):
     assert not fine.all() and torch.equal(out[0].isnan(), want.isnan()) and torch.equal(out[0].isposinf(), want.isposinf())
     assert all(torch.equal(o.view(torch.int16), out[0].view(torch.int16)) for o in out)
     close(torch.where(fine, out[0].double(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, size, 0.0), q,
-          torch.full((1, 512), 4.0, device=cuda), 0.05)
+          torch.full((1, dim), 4.0, device=cuda), 0.05)
 
 
-def test_packed_attention_in_chains_captured(cuda):
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (32, 8, 128)])
+def test_packed_attention_in_chains_captured(cuda, heads, kv, dim):
     """One captured launch whose chains follow from the lengths of each replay."""
     g = gen(53)
-    q, k, v = (normal((1500, 8, 512), g, cuda) for _ in "qkv")
+    q, k, v = (normal((1500, h, dim), g, cuda) for h in (heads, kv, kv))
     starts, k_starts = torch.zeros(17, dtype=torch.long, device=cuda), torch.zeros(17, dtype=torch.long, device=cuda)
     out = torch.empty_like(q)
     graphs = batching.GraphCache(cuda, True)
