@@ -692,7 +692,8 @@ inline int ws_group(int nqb, int units8) {
 // Measured, us, blocks one by one and in chains: 8 heads x 512, 8 prompts of 750-2400 218 / 195, of 300-700 59 / 52, 32 of 100-800
 // 169 / 133, 64 of 20-600 229 / 171, 8 of 3000-6000 1338 / 1346.  At head dim 128, where only the next block's first K tile is
 // brought beside a block's output: 32 heads, 4 of 2048 201 / 169, 64 of 20-600 258 / 216, 16 of up to 500 behind up to 900 keys
-// 106 / 91; 32 over 8 heads, 32 of 100-800 137 / 120, 16 of up to 500 behind up to 900 81 / 81, 8 of 3000-6000 1167 / 1200.  Dealt
+// 106 / 91; 32 over 8 heads, 32 of 100-800 137 / 120, 16 of up to 500 behind up to 900 81 / 81, 8 of 3000-6000 1167 / 1200; at head dim 256, 16 over 2 heads, 32 of
+// 100-800 144 / 121, 64 of 20-600 203 / 156.  Dealt
 // there and back instead, groups of sequences each longest first (head dim 512): 8 of 750-2400 223, of 3000-6000 1445.
 constexpr int kPfRounds = 128;
 constexpr int kPfListBytes = kPfRounds * kWsPerXcd * 8;
@@ -1583,10 +1584,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // ahead, two tiles behind the scores.  K goes to LDS by direct loads, two rows each, 16-byte chunk c of row r at position
 // c ^ (r % 16).  One barrier per tile.
 // What bounds a tile is what bounds prefill_attn_ws_kernel's: as many products for 3/4 of its bytes.  Measured, 16 heads
-// over 2: 8 prompts of 750-2400 186 us (729 TFLOP/s), 16 of up to 500 behind up to 900 keys 79 us; the form of
+// over 2: 8 prompts of 750-2400 178 us (772 TFLOP/s; block by block 184), 16 of up to 500 behind up to 900 keys 79 us; the form of
 // prefill_attn_wide_kernel (192 queries, partial scores added through LDS) 346 and 135 us.
 constexpr int kPmQ = 128, kPmK = 64, kPmD = 256;
 
+template <bool kChain>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void packed_attn_mid_kernel(PrefillArgs a) {
   constexpr int D = kPmD;
   __shared__ __attribute__((aligned(16))) char kls[2][kPmK * D * 2];
@@ -1594,145 +1596,176 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ float als[4][4][32];      // [score wave][tile % 4]: O's factors, when the reference moved
   __shared__ int moved[4][4];
   __shared__ float lsum[4][2][32];     // [score wave][lane half]
+  static_assert(kPfListBytes <= sizeof(kls), "");
+  __shared__ char chain_at[kChain ? sizeof(PfChain) : 1] __attribute__((aligned(16)));
+  PfChain& chain = *reinterpret_cast<PfChain*>(chain_at);
   const int together = a.together, queries = kPmQ / together;
-  const int nqb = (a.width + queries - 1) / queries;
-  PfPacked blk = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z / a.parts);
-  const int qb = (nqb - 1 - blk.j) * queries;  // the longest blocks first
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int group = (w & 3) >> 1, h = blk.h * together + group % together;
-  PfSpan sp = pf_packed_span(a, h, blk.s);
-  if (qb >= sp.nq) return;
-  int keys = min(qb + queries, sp.nq) + sp.before;  // what the block's last query sees of the part's keys
-  if (!pf_part(a, blk, sp, keys)) return;
-  if (keys <= 0) {
-    for (int i = 0; i < together; ++i)
-      pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), blk.h * together + i);
-    return;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), group = (w & 3) >> 1;
+  PfPacked blk = {};
+  PfSpan sp;
+  int qb, h, keys;  // the block's first query, the group's head, what the block's last query sees of the part's keys
+  // The chain's block of ``round``; false past its end.
+  auto enter = [&](int round) {
+    PfListed at;
+    if (!pf_listed(chain, round, a.H / together, at)) return false;
+    qb = at.j * queries;
+    h = at.h * together + group % together;
+    sp = pf_packed_span(a, h, pf_of(chain, at.s));
+    keys = min(qb + queries, sp.nq) + sp.before;
+    return true;
+  };
+  if constexpr (kChain) {
+    pf_chain<D>(a, queries, a.H / together, chain, &kls[0][0]);
+    if (!enter(0)) return;
+  } else {
+    const int nqb = (a.width + queries - 1) / queries;
+    blk = pf_packed_block(a, nqb, queries, a.H / together, (int)gridDim.z / a.parts);
+    qb = (nqb - 1 - blk.j) * queries;  // the longest blocks first
+    h = blk.h * together + group % together;
+    sp = pf_packed_span(a, h, blk.s);
+    keys = min(qb + queries, sp.nq) + sp.before;
+    if (qb >= sp.nq) return;
+    if (!pf_part(a, blk, sp, keys)) return;
+    if (keys <= 0) {
+      for (int i = 0; i < together; ++i)
+        pf_zeros<D>(a, sp.q0 + qb, sp.q0 + min(qb + queries, sp.nq), blk.h * together + i);
+      return;
+    }
   }
-  const int nt = (keys + kPmK - 1) / kPmK;
-  const int qp = qb + 64 * (group / together);  // the group's first query
-  // The group's last tile (-1: no queries, or they see no key).
-  const int lastk = min(min(qp + 64, sp.nq) + sp.before, keys) - 1;
-  const int dq = qp < sp.nq && lastk >= 0 ? lastk / kPmK : -1;
+  int nt, qp, dq;  // tiles; the group's first query and its last tile (-1: no queries, or they see no key)
+  const char *kbase, *vbase;
+  auto derive = [&]() {
+    kbase = scalar_pointer(sp.k);
+    vbase = scalar_pointer(sp.v);
+    nt = (keys + kPmK - 1) / kPmK;
+    qp = qb + 64 * (group / together);
+    const int lastk = min(min(qp + 64, sp.nq) + sp.before, keys) - 1;
+    dq = qp < sp.nq && lastk >= 0 ? lastk / kPmK : -1;
+  };
+  derive();
 
   if (w < 4) {  // ------------------------------------------------------------------------------ scores
-    const int query = qp + 32 * (w & 1) + x, whole = qp + 32 * (w & 1) + sp.before;  // all 32 see keys [0, whole]
-    u32x4_t q[D / 16];  // q[query][16s + 8g .. + 7]
-    {
-      const uint16_t* qrow = a.q + ((sp.q0 + min(query, sp.nq - 1)) * a.H + h) * D + g * 8;
+    for (int round = 0;; ++round) {
+      const int query = qp + 32 * (w & 1) + x, whole = qp + 32 * (w & 1) + sp.before;  // all 32 see keys [0, whole]
+      u32x4_t q[D / 16];  // q[query][16s + 8g .. + 7]
+      {
+        const uint16_t* qrow = a.q + ((sp.q0 + min(query, sp.nq - 1)) * a.H + h) * D + g * 8;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4_t*>(qrow + s * 16);
-    }
-    float m_ref = -INFINITY, thr = -INFINITY, l_run = 0.f;
-    const int klane = x * (D * 2) + ((g ^ (x & 15)) * 16);
-    auto k_at = [&](int t, int m, int s) {
-      return *reinterpret_cast<const u32x4_t*>(&kls[t & 1][32 * m * (D * 2) + (klane ^ (32 * s))]);
-    };
-    typedef f32x16_t Scores[2];  // [key half m]
-    f32x16_t zero;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-    // One 16-key step's probabilities: keys 16 (2m + hf) .., as the value wave's operand.
-    auto put_p = [&](const Scores& sc, int t, int m, int hf, float mu) {
-      u32x4_t pop;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][8 * hf + 2 * e], a.scale_log2, -mu));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][8 * hf + 2 * e + 1], a.scale_log2, -mu));
-        l_run += p0 + p1;
-        pop[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
+        for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4_t*>(qrow + s * 16);
       }
-      ps[t & 1][w][2 * m + hf][lane] = pop;
-    };
-    // The reference of tile t's scores (masked where not every query sees every key).
-    auto refer = [&](Scores& sc, int t) {
-      // max3's operands come from the matrix unit: every product has written its result after 24 wait states.
-      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sc[0]), "+v"(sc[1]));
-      if (t * kPmK + kPmK - 1 > whole) {
+      float m_ref = -INFINITY, thr = -INFINITY, l_run = 0.f;
+      const int klane = x * (D * 2) + ((g ^ (x & 15)) * 16);
+      auto k_at = [&](int t, int m, int s) {
+        return *reinterpret_cast<const u32x4_t*>(&kls[t & 1][32 * m * (D * 2) + (klane ^ (32 * s))]);
+      };
+      typedef f32x16_t Scores[2];  // [key half m]
+      f32x16_t zero;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int rel = whole - t * kPmK + x - (32 * m + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
+      for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+      // One 16-key step's probabilities: keys 16 (2m + hf) .., as the value wave's operand.
+      auto put_p = [&](const Scores& sc, int t, int m, int hf, float mu) {
+        u32x4_t pop;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[m][i] = 8 * (i >> 2) + (i & 3) <= rel ? sc[m][i] : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][8 * hf + 2 * e], a.scale_log2, -mu));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][8 * hf + 2 * e + 1], a.scale_log2, -mu));
+          l_run += p0 + p1;
+          pop[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
         }
-      }
-      float mx = max3(sc[0][0], sc[1][0], sc[0][1]);
-      mx = max3(mx, sc[1][1], sc[1][1]);
+        ps[t & 1][w][2 * m + hf][lane] = pop;
+      };
+      // The reference of tile t's scores (masked where not every query sees every key).
+      auto refer = [&](Scores& sc, int t) {
+        // max3's operands come from the matrix unit: every product has written its result after 24 wait states.
+        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sc[0]), "+v"(sc[1]));
+        if (t * kPmK + kPmK - 1 > whole) {
 #pragma unroll
-      for (int i = 2; i < 16; ++i) mx = max3(mx, sc[0][i], sc[1][i]);
-      const bool move = __any(mx > thr);
-      if (lane == 0) moved[w][t & 3] = move ? 1 : 0;
-      if (move) {
-        const float top = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-        const float m_new = fmaxf(m_ref, top * a.scale_log2);
-        const float alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -INFINITY ? 0.f : m_new));  // m_ref = -inf: 0
-        if (g == 0) als[w][t & 3][x] = alpha;
-        l_run *= alpha;
-        m_ref = m_new;
-        thr = m_new == -INFINITY ? -INFINITY : (m_new + kWsGuard) / a.scale_log2;
-      }
-    };
-    // Step t: tile t's products into ``to``, the softmax of tile t - 1's scores ``from`` beside them.
-    auto step = [&](const Scores& from, Scores& to, int t, bool soft) {
-      u32x4_t kf[2] = {k_at(t, 0, 0), k_at(t, 1, 0)};
-      const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+          for (int m = 0; m < 2; ++m) {
+            const int rel = whole - t * kPmK + x - (32 * m + 4 * g);  // keys 8 (i / 4) + i % 4 <= rel are seen
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) to[m] = mfma32(kf[m], q[s], s == 0 ? zero : to[m]);
-        if (s + 1 < D / 16) {
-#pragma unroll
-          for (int m = 0; m < 2; ++m) kf[m] = k_at(t, m, s + 1);
+            for (int i = 0; i < 16; ++i) sc[m][i] = 8 * (i >> 2) + (i & 3) <= rel ? sc[m][i] : -INFINITY;
+          }
         }
-        if (soft && (s & 3) == 3) put_p(from, t - 1, s >> 3, (s >> 2) & 1, mu);
-      }
-      refer(to, t);
-    };
-    auto finish = [&](const Scores& from, int t) {  // the group's last tile
-      const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+        float mx = max3(sc[0][0], sc[1][0], sc[0][1]);
+        mx = max3(mx, sc[1][1], sc[1][1]);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) put_p(from, t, s >> 1, s & 1, mu);
-      lsum[w][g][x] = l_run;
-    };
-    Scores sa, sb;
-    lds_barrier();  // the first K tile
-    if (dq >= 0) step(sb, sa, 0, false);
-    lds_barrier();
-    int t = 1;
-    for (; t + 1 <= dq; t += 2) {
-      step(sa, sb, t, true);
+        for (int i = 2; i < 16; ++i) mx = max3(mx, sc[0][i], sc[1][i]);
+        const bool move = __any(mx > thr);
+        if (lane == 0) moved[w][t & 3] = move ? 1 : 0;
+        if (move) {
+          const float top = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+          const float m_new = fmaxf(m_ref, top * a.scale_log2);
+          const float alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -INFINITY ? 0.f : m_new));  // m_ref = -inf: 0
+          if (g == 0) als[w][t & 3][x] = alpha;
+          l_run *= alpha;
+          m_ref = m_new;
+          thr = m_new == -INFINITY ? -INFINITY : (m_new + kWsGuard) / a.scale_log2;
+        }
+      };
+      // Step t: tile t's products into ``to``, the softmax of tile t - 1's scores ``from`` beside them.
+      auto step = [&](const Scores& from, Scores& to, int t, bool soft) {
+        u32x4_t kf[2] = {k_at(t, 0, 0), k_at(t, 1, 0)};
+        const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) to[m] = mfma32(kf[m], q[s], s == 0 ? zero : to[m]);
+          if (s + 1 < D / 16) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) kf[m] = k_at(t, m, s + 1);
+          }
+          if (soft && (s & 3) == 3) put_p(from, t - 1, s >> 3, (s >> 2) & 1, mu);
+        }
+        refer(to, t);
+      };
+      auto finish = [&](const Scores& from, int t) {  // the group's last tile
+        const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) put_p(from, t, s >> 1, s & 1, mu);
+        lsum[w][g][x] = l_run;
+      };
+      Scores sa, sb;
+      lds_barrier();  // the first K tile
+      if (dq >= 0) step(sb, sa, 0, false);
       lds_barrier();
-      step(sb, sa, t + 1, true);
-      lds_barrier();
+      int t = 1;
+      for (; t + 1 <= dq; t += 2) {
+        step(sa, sb, t, true);
+        lds_barrier();
+        step(sb, sa, t + 1, true);
+        lds_barrier();
+      }
+      if (t <= dq) {  // one more, then its scores are in sb
+        step(sa, sb, t, true);
+        lds_barrier();
+        finish(sb, t);
+        lds_barrier();
+        t += 2;
+      } else if (dq >= 0) {
+        finish(sa, t - 1);
+        lds_barrier();
+        t += 1;
+      }
+      for (; t <= nt + 1; ++t) lds_barrier();
+      if (!kChain && pf_in_parts(blk)) pf_leave_ml(a, blk, w, g, x, m_ref, l_run);
+      if (!kChain || !enter(round + 1)) return;
+      derive();
     }
-    if (t <= dq) {  // one more, then its scores are in sb
-      step(sa, sb, t, true);
-      lds_barrier();
-      finish(sb, t);
-      lds_barrier();
-      t += 2;
-    } else if (dq >= 0) {
-      finish(sa, t - 1);
-      lds_barrier();
-      t += 1;
-    }
-    for (; t <= nt + 1; ++t) lds_barrier();
-    if (pf_in_parts(blk)) pf_leave_ml(a, blk, w, g, x, m_ref, l_run);
-    return;
   }
 
   // ---------------------------------------------------------------------------------------------- values
   const int vw = w - 4, slice = 128 * (vw & 1);
-  const char* kbase = scalar_pointer(sp.k);
-  const char* vbase = scalar_pointer(sp.v);
   f32x16_t o[2][4];  // as prefill_attn_ws_kernel's, of queries qp + 32u + x and dimensions slice ..
+  auto clear = [&]() {
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
+        for (int i = 0; i < 16; ++i) o[u][e][i] = 0.f;
+  };
+  clear();
   // K rows 16 vw .. + 15 of tile t to LDS (past the last tile: that tile again, not used); rows past the sequence read its
   // last key (finite or masked).
   auto bring_k = [&](int t) {
@@ -1748,7 +1781,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           kr, (__attribute__((address_space(3))) void*)&kls[t & 1][(16 * vw + 2 * r2) * (D * 2)], 16, from, 0, 0, 0);
     }
   };
-  const uint32_t vlane = (uint32_t)(8 * (x >> 4) + 4 * g) * sp.v_bytes + (uint32_t)(slice + 8 * (x & 15)) * 2;
+  const uint32_t v_bytes = (uint32_t)a.v_pos * 2;
+  const uint32_t vlane = (uint32_t)(8 * (x >> 4) + 4 * g) * v_bytes + (uint32_t)(slice + 8 * (x & 15)) * 2;
   u32x4_t v[4][4];
   auto load_v = [&](int t, int s) {  // 16-key step s of tile t; rows past the sequence read 0
     const int at = t * kPmK + 16 * s, rows = min(sp.nk - at, 16);
@@ -1757,7 +1791,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         0x00020000);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      v[s][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, vlane + j * sp.v_bytes, 0, 0));
+      v[s][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, vlane + j * v_bytes, 0, 0));
   };
   // O^T += V^T P^T for tile t, and the loads of tile ``ahead`` as its registers fall free.
   auto attend_v = [&](int t, int ahead) {
@@ -1820,57 +1854,83 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
   };
+  // O of a block's queries from ``first``; whether some is not finite.
+  auto output = [&](const PfSpan& s, int head, int first, int d) {
+    bool again = false;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int query = first + 32 * u + x;
+      if (query >= s.nq) continue;
+      const float l = d < 0 ? 0.f : lsum[2 * group + u][0][x] + lsum[2 * group + u][1][x];
+      const float inv = l > 0.f ? 1.f / l : 1.f;
+      uint16_t* orow = a.out + ((s.q0 + query) * a.H + head) * D + slice + 32 * g;
+      auto pair = [&](float lo, float hi) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
+      };
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // dimensions 64r + 32g + 8i + 4k + e, k = 0, 1
+          u32x4_t out;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int at = 4 * (r + 2 * k) + i;
+            out[2 * k] = pair(o[u][0][at], o[u][1][at]);
+            out[2 * k + 1] = pair(o[u][2][at], o[u][3][at]);
+          }
+          *reinterpret_cast<u32x4_t*>(orow + 64 * r + 8 * i) = out;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) again |= pf_nonfinite(out[k]);
+        }
+    }
+    return again;
+  };
   bring_k(0);
   landed_barrier();
-  bring_k(1);
-  landed_barrier();  // step 0
-  int t = 1;
-  if (dq >= 0) {
-    bring_k(2);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) load_v(0, s);
-    k_landed();  // step 1
-    for (t = 2; t <= dq + 2; ++t) {
-      bring_k(t + 1);
+  for (int round = 0;; ++round) {
+    bring_k(1);
+    landed_barrier();  // step 0
+    int t = 1;
+    if (dq >= 0) {
+      bring_k(2);
       __builtin_amdgcn_sched_barrier(0);
-      attend_v(t - 2, min(t - 1, dq));
-      k_landed();
+#pragma unroll
+      for (int s = 0; s < 4; ++s) load_v(0, s);
+      k_landed();  // step 1
+      for (t = 2; t <= dq + 2; ++t) {
+        bring_k(t + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        attend_v(t - 2, min(t - 1, dq));
+        k_landed();
+      }
+    }
+    for (; t <= nt + 1; ++t) {
+      bring_k(t + 1);
+      landed_barrier();
+    }
+    if constexpr (kChain) {
+      // As prefill_attn_pairs_kernel's.
+      const PfSpan was = sp;
+      const int head = h, first = qp, d = dq;
+      const bool more = enter(round + 1);
+      if (more) {
+        derive();
+        bring_k(0);
+      }
+      if (__any(output(was, head, first, d))) chain.redo[vw][round >> 5] |= 1u << (round & 31);
+      if (!more) break;
+      clear();
+      landed_barrier();
+    } else {
+      if (pf_in_parts(blk)) return pf_leave_o(a, blk, vw, lane, sp.nq - qp, o);
+      if (__any(output(sp, h, qp, dq))) pf_again<D>(a, sp, h, qp, 4, slice);
+      return;
     }
   }
-  for (; t <= nt + 1; ++t) {
-    bring_k(t + 1);
-    landed_barrier();
+  for (int round = 0; enter(round); ++round) {
+    derive();
+    if (chain.redo[vw][round >> 5] >> (round & 31) & 1) pf_again<D>(a, sp, h, qp, 4, slice);
   }
-  if (pf_in_parts(blk)) return pf_leave_o(a, blk, vw, lane, sp.nq - qp, o);
-  bool again = false;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int query = qp + 32 * u + x;
-    if (query >= sp.nq) continue;
-    const float l = dq < 0 ? 0.f : lsum[2 * group + u][0][x] + lsum[2 * group + u][1][x];
-    const float inv = l > 0.f ? 1.f / l : 1.f;
-    uint16_t* orow = a.out + ((sp.q0 + query) * a.H + h) * D + slice + 32 * g;
-    auto pair = [&](float lo, float hi) {
-      return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo * inv, hi * inv}), bf16x2_t));
-    };
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // dimensions 64r + 32g + 8i + 4k + e, k = 0, 1
-        u32x4_t out;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int at = 4 * (r + 2 * k) + i;
-          out[2 * k] = pair(o[u][0][at], o[u][1][at]);
-          out[2 * k + 1] = pair(o[u][2][at], o[u][3][at]);
-        }
-        *reinterpret_cast<u32x4_t*>(orow + 64 * r + 8 * i) = out;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) again |= pf_nonfinite(out[k]);
-      }
-  }
-  if (__any(again)) pf_again<D>(a, sp, h, qp, 4, slice);
 }
 
 // The parts of blocks joined: out = sum_p w_p O_p / sum_p w_p l_p, w_p = exp(m_p - max m).  One workgroup for a quarter
@@ -1952,7 +2012,7 @@ inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int longest
   return (int)std::min({kPartCus / blocks + 1, tiles / kPartLeast, (int64_t)kPartMost});
 }
 
-// Whether a launch runs its blocks in chains: where an XCD has two (head dim 128: three; 10 of 260-300, 32 heads, 2.5 for each,
+// Whether a launch runs its blocks in chains: where an XCD has two (head dims 128 and 256: three; 10 of 260-300, 32 heads, 2.5 for each,
 // take 48 us in place of 45.5) or more for each of its workgroups (no more than their lists hold, and sequences that one wave's
 // lanes hold), and the same ``heads`` blocks of heads for every sequence.
 inline bool packed_chains(int64_t nqb, int heads, int sequences, int head_dim) {
@@ -2324,7 +2384,8 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
     else omni::prefill_attn_pairs_kernel<true, false><<<grid, 512, 0, s>>>(a);
     if (a.parts > 1) omni::packed_attn_join_kernel<128><<<join, 256, 0, s>>>(a);
   } else if (head_dim == 256) {
-    omni::packed_attn_mid_kernel<<<grid, 512, 0, s>>>(a);
+    if (chains) omni::packed_attn_mid_kernel<true><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);
+    else omni::packed_attn_mid_kernel<false><<<grid, 512, 0, s>>>(a);
     if (a.parts > 1) omni::packed_attn_join_kernel<256><<<join, 256, 0, s>>>(a);
   } else {
     if (chains) omni::prefill_attn_ws_kernel<true, true><<<8 * omni::kWsPerXcd, 512, 0, s>>>(a);

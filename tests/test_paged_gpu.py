@@ -422,7 +422,8 @@ def test_packed_attention_head_counts(cuda, heads, kv, dim):
     packed_case(cuda, heads, kv, dim, [70, 1, 0, 150], [0, 40, 3, 9], heads + kv)
 
 
-CHAINED = [(8, 8, 512), (16, 2, 512), (24, 3, 512), (32, 8, 128), (16, 8, 128), (32, 32, 128), (24, 24, 128)]
+CHAINED = [(8, 8, 512), (16, 2, 512), (24, 3, 512), (32, 8, 128), (16, 8, 128), (32, 32, 128), (24, 24, 128), (16, 2, 256),
+           (8, 8, 256)]
 
 
 @pytest.mark.parametrize("heads,kv,dim", CHAINED)
@@ -439,7 +440,7 @@ def test_packed_attention_in_chains(cuda, heads, kv, dim):
     packed_case(cuda, heads, kv, dim, [700, 900], [-700, -901], heads + 5, longest=4000, behind=2400)
 
 
-@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (32, 8, 128), (32, 32, 128)])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (32, 8, 128), (32, 32, 128), (16, 2, 256)])
 def test_packed_attention_in_chains_up_to_longest(cuda, heads, kv, dim):
     """Queries past ``longest`` of a sequence are not computed, the others see what they see."""
     g, counts = gen(51), [300, 40, 129, 64, 200, 10, 70, 90, 100, 128, 192, 1, 2, 3, 65, 66]
@@ -458,7 +459,7 @@ def test_packed_attention_in_chains_up_to_longest(cuda, heads, kv, dim):
     assert torch.equal(out[kept], want[kept]) and (out[~kept] == 7.0).all()
 
 
-@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 512), (32, 8, 128), (32, 32, 128)])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 512), (32, 8, 128), (32, 32, 128), (16, 2, 256)])
 def test_packed_attention_in_chains_does_not_see_what_is_masked(cuda, heads, kv, dim):
     g, counts = gen(52), [300, 90, 129, 64, 200, 10, 70, 90, 100, 128, 192, 1, 2, 3, 65, 66]
     starts = torch.tensor([0, *counts]).cumsum(0)
@@ -478,7 +479,7 @@ def test_packed_attention_in_chains_does_not_see_what_is_masked(cuda, heads, kv,
           torch.full((1, dim), 4.0, device=cuda), 0.05)
 
 
-@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (32, 8, 128)])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (32, 8, 128), (16, 2, 256)])
 def test_packed_attention_in_chains_captured(cuda, heads, kv, dim):
     """One captured launch whose chains follow from the lengths of each replay."""
     g = gen(53)
