@@ -43,6 +43,7 @@ struct PrefillArgs {
   int64_t k_pos = 0, k_head = 0, v_pos = 0, v_head = 0;
   int heads_per_kv = 1;
   int together = 1;  // head dims 128 and 256: heads of a kv head in one block (1, 2 or 4)
+  int block = 0;     // head dims 128 and 256: queries of each head in a block
   // Blocks in parts (pf_part): at most ``parts``, each with room for its O and its queries' (m, l).
   int parts = 1;
   float* part_o = nullptr;   // [part][value wave][query half u][r][e][k][lane][4]
@@ -1258,7 +1259,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ char chain_at[kChain ? sizeof(PfChain) : 1] __attribute__((aligned(16)));
   PfChain& chain = *reinterpret_cast<PfChain*>(chain_at);
   // The pairs' 64 queries: of one head one after another, or (packed) of 2 or 4 heads that read the same keys.
-  const int together = kPacked ? a.together : 1, queries = kPairQ / together;
+  const int together = kPacked ? a.together : 1, queries = kPacked ? a.block : kPairQ;
   const int nqb = (a.width + queries - 1) / queries;
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), pr = w & 3;
@@ -1305,6 +1306,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     vbase = scalar_pointer(sp.v);
     nt = (keys + kPairK - 1) / kPairK;
     qp = qb + 64 * (kPacked ? pr / together : pr);
+    if (kPacked && qp >= qb + queries) qp = sp.nq;  // a block of fewer pairs
     // The pair's last tile holds its diagonal (-1: no queries, or they see no key).
     const int lastk = kPacked ? min(min(qp + 64, sp.nq) + sp.before, keys) - 1 : qp;
     dq = qp < sp.nq && lastk >= 0 ? lastk / kPairK : -1;
@@ -1599,7 +1601,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   static_assert(kPfListBytes <= sizeof(kls), "");
   __shared__ char chain_at[kChain ? sizeof(PfChain) : 1] __attribute__((aligned(16)));
   PfChain& chain = *reinterpret_cast<PfChain*>(chain_at);
-  const int together = a.together, queries = kPmQ / together;
+  const int together = a.together, queries = a.block;
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), group = (w & 3) >> 1;
   PfPacked blk = {};
@@ -1640,6 +1642,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     vbase = scalar_pointer(sp.v);
     nt = (keys + kPmK - 1) / kPmK;
     qp = qb + 64 * (group / together);
+    if (qp >= qb + queries) qp = sp.nq;  // a block of one group
     const int lastk = min(min(qp + 64, sp.nq) + sp.before, keys) - 1;
     dq = qp < sp.nq && lastk >= 0 ? lastk / kPmK : -1;
   };
@@ -2012,6 +2015,14 @@ inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int longest
   return (int)std::min({kPartCus / blocks + 1, tiles / kPartLeast, (int64_t)kPartMost});
 }
 
+// Queries of a head in a block, ``rows`` or fewer: fewer to a block take less time, if every CU still has one block at most.
+// Measured at head dim 128, us, blocks of 256 and fewer, 32 heads: one prompt of 200 14.5 / 12.0, four of 60-200 15.9 / 14.2; 8
+// heads, one of 1433 41.8 / 38.4; past one block for a CU, 32 heads, one of 1433 43 / 59.
+inline int packed_block(int rows, int64_t longest, int64_t units) {
+  while (rows > 64 && (longest + rows / 2 - 1) / (rows / 2) * units <= kPartCus) rows /= 2;
+  return rows;
+}
+
 // Whether a launch runs its blocks in chains: where an XCD has two (head dims 128 and 256: three; 10 of 260-300, 32 heads, 2.5 for each,
 // take 48 us in place of 45.5) or more for each of its workgroups (no more than their lists hold, and sequences that one wave's
 // lanes hold), and the same ``heads`` blocks of heads for every sequence.
@@ -2376,6 +2387,11 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
   }
   const bool chains = omni::packed_chains(grid.x, grid.y, sequences, head_dim);
   a.sequences = sequences;
+  a.block = rows;
+  if (a.parts == 1 && !chains) {
+    a.block = omni::packed_block(rows, longest, blocks / grid.x);
+    grid.x = (longest + a.block - 1) / a.block;
+  }
   const dim3 join(grid.x * 4, grid.y, grid.z);
   grid.z *= a.parts;
   const hipStream_t s = (hipStream_t)stream;
