@@ -690,12 +690,13 @@ inline int ws_group(int nqb, int units8) {
 // the most work and their longest blocks first, heads beside each other.  32 blocks at a time are dealt to its workgroups, the
 // longest to the one with the fewest tiles so far.  Every workgroup does that for itself from the lengths, in ~3 us of a
 // launch.
-// Measured, us, blocks one by one and in chains: 8 heads x 512, 8 prompts of 750-2400 218 / 195, of 300-700 59 / 52, 32 of 100-800
-// 169 / 133, 64 of 20-600 229 / 171, 8 of 3000-6000 1338 / 1346.  At head dim 128, where only the next block's first K tile is
-// brought beside a block's output: 32 heads, 4 of 2048 201 / 169, 64 of 20-600 258 / 216, 16 of up to 500 behind up to 900 keys
-// 106 / 91; 32 over 8 heads, 32 of 100-800 137 / 120, 16 of up to 500 behind up to 900 81 / 81, 8 of 3000-6000 1167 / 1200; at head dim 256, 16 over 2 heads, 32 of
-// 100-800 144 / 121, 64 of 20-600 203 / 156.  Dealt
-// there and back instead, groups of sequences each longest first (head dim 512): 8 of 750-2400 223, of 3000-6000 1445.
+// Measured, us, blocks one by one and in chains: 8 heads x 512, 8 prompts of 750-2400 218 / 195, of 300-700 59 / 52, 32
+// of 100-800 169 / 133, 64 of 20-600 229 / 171, 8 of 3000-6000 1338 / 1346.  At head dim 128, where only the next
+// block's first K tile is brought beside a block's output: 32 heads, 4 of 2048 201 / 169, 64 of 20-600 258 / 216, 16 of
+// up to 500 behind up to 900 keys 106 / 91; 32 over 8 heads, 32 of 100-800 137 / 120, 16 of up to 500 behind up to 900
+// 81 / 81, 8 of 3000-6000 1167 / 1200; at head dim 256, 16 over 2 heads, 32 of 100-800 144 / 121, 64 of 20-600 203 /
+// 156.  Dealt there and back instead, groups of sequences each longest first (head dim 512): 8 of 750-2400 223, of
+// 3000-6000 1445.
 constexpr int kPfRounds = 128;
 constexpr int kPfListBytes = kPfRounds * kWsPerXcd * 8;
 
