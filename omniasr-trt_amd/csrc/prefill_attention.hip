@@ -714,7 +714,7 @@ __device__ __forceinline__ void pf_chain(const PrefillArgs& a, int queries, int 
     const PfSequence one = pf_sequence(a, min(lane, a.sequences - 1));
     const int rank = pf_rank(one, a.sequences);
     if (w == 0 && lane < a.sequences) c.seqs[rank] = one;
-    if (tid < 4 * (kPfRounds / 32)) c.redo[0][tid] = 0;
+    if (tid < 4 * (kPfRounds / 32)) c.redo[tid % 4][tid / 4] = 0;
   }
   lds_barrier();
   // A lane's sequence, and its blocks: ``seen`` that see a key, of which ``upto`` come up to its end.
