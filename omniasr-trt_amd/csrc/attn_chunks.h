@@ -29,28 +29,35 @@ struct KvChunk {
   u32x4_t r[kF8 ? 4 : 8];
 };
 
+// kOnce: memory that no other workgroup reads, loaded past the caches that others' data would stay in.
+template <bool kOnce, typename T>
+__device__ __forceinline__ T load_as(const char* p) {
+  if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  return *reinterpret_cast<const T*>(p);
+}
+
 // K: bf16 row mb at r[4 mb + s], dimensions 32s + 8g ..; e4m3 at r[2 mb + p], dimensions 64p + 16g ...  ``row``: row
 // c % 4 of the lane's 8 keys, 16g bytes on; rows are kRowB bytes apart.
-template <bool kF8, int kRowB>
+template <bool kF8, int kRowB, bool kOnce>
 __device__ __forceinline__ void load_k_chunk(KvChunk<kF8>& t, const char* row) {
   constexpr int kSteps = kF8 ? 2 : 4;
 #pragma unroll
   for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) t.r[kSteps * mb + s] = ld16(row + 4 * mb * kRowB + 64 * s);
+    for (int s = 0; s < kSteps; ++s) t.r[kSteps * mb + s] = load_as<kOnce, u32x4_t>(row + 4 * mb * kRowB + 64 * s);
 }
 
 // V row j: dimensions 8c .. + 7 of the chunk.  ``row``: the first of the lane's 8 keys, at its dimensions.
-template <bool kF8, int kRowB>
+template <bool kF8, int kRowB, bool kOnce>
 __device__ __forceinline__ void load_v_chunk(KvChunk<kF8>& t, const char* row) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if constexpr (kF8) {
-      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(row + j * kRowB);
+      const u32x2_t w = load_as<kOnce, u32x2_t>(row + j * kRowB);
       t.r[j >> 1][2 * (j & 1)] = w[0];
       t.r[j >> 1][2 * (j & 1) + 1] = w[1];
     } else {
-      t.r[j] = ld16(row + j * kRowB);
+      t.r[j] = load_as<kOnce, u32x4_t>(row + j * kRowB);
     }
   }
 }

@@ -144,10 +144,14 @@ struct PagedPiece {
 // NB: blocks of 16 query columns that share a read of the keys.  Two at most: four spill registers (64
 // columns, 42 us against 31 in twos).  Measured, with the second launch's 4-5 us: 8 slots x 5 of 750-2400 keys, 8 heads
 // x 512 e4m3 26 us (the stream at 4.2 TB/s), 32 x 128 bf16 44; 16 slots of 4000-8188, 32 over 8 x 128 e4m3 48 (5.1 TB/s).
-// Three tiles ahead in place of two 28.6 against 27.1 us; 1024, 768 and 256 workgroups 31, 29 and 27 against 27.
+// Three tiles ahead in place of two 28.6 against 27.1 us; 1024, 768 and 256 workgroups 31, 29 and 27 against 27.  Loads that
+// are not kept in the caches, over more caches than those hold: the first of these 28.6 to 27.1, the second 45.6 to 42.8, the
+// third 48.7 to 44.6 (in bf16 83.8 to 75.3), 8 x 512 bf16 43.3 to 40.6; but 16 tokens, 16 over 2 heads x 256, whose keys four
+// units read, 35.9 to 39.2, and K's at head dim 512 28.2 in place of 27.1 (a wave reads a line of K in two halves).
 template <int D, bool kF8, int NB>
 __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2))) void paged_attn_kernel(PagedAttn a) {
   constexpr int kRowB = D * (kF8 ? 1 : 2), kAhead = paged_ahead<kF8, NB>();
+  constexpr bool kOnce = NB == 1;  // two blocks may be a part of more columns, whose other units read the same keys
   constexpr int kSlices = D / 128, kStep = kPaWaves / kSlices;  // waves to a tile, tiles at a time
   constexpr int kQRow = D * 2 + 16;  // LDS bytes of a query, padded against bank conflicts
   constexpr int kQPieces = 16 * NB * (D / 8) / (64 * kPaWaves);  // of 16 bytes, of the blocks' queries, for a thread
@@ -211,7 +215,7 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
     }
     constexpr int kSliceB = 128 * (kF8 ? 1 : 2);
     vrow = i < p.mine ? a.cache.v + vc * kRowB + sl * kSliceB + c * (kF8 ? 8 : 16) : a.cache.v;
-    load_k_chunk<kF8, kRowB>(t.k, i < p.mine ? a.cache.k + kc * kRowB + sl * kSliceB + g * 16 : a.cache.k);
+    load_k_chunk<kF8, kRowB, kOnce && D == 128>(t.k, i < p.mine ? a.cache.k + kc * kRowB + sl * kSliceB + g * 16 : a.cache.k);
   };
 
   PagedPiece p;
@@ -235,7 +239,7 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
       for (int i = 0; i < kAhead; ++i) {
         const char* vrow;
         load_k(tile[i], p, i, at[i], vrow, tile[i].vs);
-        load_v_chunk<kF8, kRowB>(tile[i].v, vrow);
+        load_v_chunk<kF8, kRowB, kOnce>(tile[i].v, vrow);
       }
       pages = look(p, kAhead);
 #pragma unroll
@@ -306,7 +310,7 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
         for (int j = 0; j < 8; ++j) vscale[j] = scale_of((t.vs[j >> 2] >> (8 * (j & 3))) & 0xffu);
         chunk_values<kF8, NB>(t.v, pop, vscale, o);
       }
-      load_v_chunk<kF8, kRowB>(t.v, vrow);
+      load_v_chunk<kF8, kRowB, kOnce>(t.v, vrow);
       t.vs = vs;
       __builtin_amdgcn_sched_barrier(0);
     };
