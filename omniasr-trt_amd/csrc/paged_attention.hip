@@ -143,7 +143,7 @@ struct PagedPiece {
 
 // NB: blocks of 16 query columns that share a read of the keys.  Two at most: four spill registers (64
 // columns, 42 us against 31 in twos).  Measured, with the second launch's 4-5 us: 8 slots x 5 of 750-2400 keys, 8 heads
-// x 512 e4m3 26 us (the stream at 4.2 TB/s), 32 x 128 bf16 44; 16 slots of 4000-8188, 32 over 8 x 128 e4m3 48 (5.1 TB/s).
+// x 512 e4m3 26 us (the stream at 4.1 TB/s), 32 x 128 bf16 43; 16 slots of 4000-8188, 32 over 8 x 128 e4m3 45 (5.4 TB/s).
 // Three tiles ahead in place of two 28.6 against 27.1 us; 1024, 768 and 256 workgroups 31, 29 and 27 against 27.  Loads that
 // are not kept in the caches, over more caches than those hold: the first of these 28.6 to 27.1, the second 45.6 to 42.8, the
 // third 48.7 to 44.6 (in bf16 83.8 to 75.3), 8 x 512 bf16 43.3 to 40.6; but 16 tokens, 16 over 2 heads x 256, whose keys four

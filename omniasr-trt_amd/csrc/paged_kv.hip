@@ -8,7 +8,9 @@
 // binade above 2^-6, 14 below the largest.)  k is quantised from the rotated fp32 values, not from their bf16 rounding.
 //
 // Both kernels are one pass over their bytes, 16 (8 for e4m3) of one vector a thread: a step's launch is latency, a
-// prompt's is HBM.  Measured, 8 prompts of 750-2400, 8 heads x 512, e4m3: write 102 us (4.7 TB/s), read 45-50 us (5.4-6.1).
+// prompt's is HBM.  Measured, 8 prompts of 750-2400, 8 heads x 512, e4m3: write 102-105 us (4.6 TB/s), read 43-44 us (6.3).
+// Pages go past the caches, which hold what the next kernels read: q, k and v.  The same prompts written and attended to 374 us,
+// so 370; 16 rows of 1500 read back for 64 queries each 93, so 91.  All of it past the caches: one prompt of 1433 58, so 71.
 #include "common.h"
 #include "paged.h"
 
@@ -100,7 +102,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite w, PagedCac
       const int64_t cell = cell0 + ((int64_t)head << a.page_log2);
       char* pages = is_k ? a.k : a.v;
       if constexpr (!kF8) {
-        *reinterpret_cast<u32x4_t*>(pages + (cell * D + e0) * 2) = bf;
+        __builtin_nontemporal_store(bf, reinterpret_cast<u32x4_t*>(pages + (cell * D + e0) * 2));
       } else {
         uint32_t top = 0;
 #pragma unroll
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite w, PagedCac
           const int half = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
           codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], half, true);
         }
-        *reinterpret_cast<u32x2_t*>(pages + cell * D + e0) = codes;
+        __builtin_nontemporal_store(codes, reinterpret_cast<u32x2_t*>(pages + cell * D + e0));
         if (e0 == 0) (is_k ? a.k_scale : a.v_scale)[cell] = (uint8_t)(exponent + 127);
       }
     }
@@ -153,10 +155,10 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead r, PagedCache
       out[k] = u32x4_t{0u, 0u, 0u, 0u};
       if (cell0 < 0 || vec >= vectors) continue;
       if constexpr (kF8) {
-        out[k] = e4m3x8_to_bf16(*reinterpret_cast<const u32x2_t*>(pages + cell * D + e0),
+        out[k] = e4m3x8_to_bf16(__builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(pages + cell * D + e0)),
                                 scale_of((is_k ? a.k_scale : a.v_scale)[cell]));
       } else {
-        out[k] = *reinterpret_cast<const u32x4_t*>(pages + (cell * D + e0) * 2);
+        out[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(pages + (cell * D + e0) * 2));
       }
     }
 #pragma unroll
