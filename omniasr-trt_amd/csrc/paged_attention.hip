@@ -9,7 +9,7 @@
 // What bounds it is the HBM stream of the keys, so every CU is to stream the same share from start to end.  The 32-key
 // tiles of all units stand in one line (row after row, unit after unit), cut into equal shares, one for each workgroup of
 // four waves, whatever the rows' lengths: a share is the end of one unit, whole units, and the beginning of another.  A
-// unit's start counts as kPaStart more tiles, about what it costs.  A wave holds 128 dimensions, so the waves take a unit's
+// unit's start counts as some more tiles (paged_start), about what it costs.  A wave holds 128 dimensions, so the waves take a unit's
 // tiles in turn at head dim 128, in pairs at 256 and together at 512, where their partial scores are added through LDS;
 // each has the next tiles' loads in flight in registers.  A unit within one share is written at once; of the others each
 // share leaves (O, m, l) in fp32, and a second launch joins them:
@@ -23,7 +23,6 @@
 namespace omni {
 
 constexpr int kPaWaves = 4;
-constexpr int kPaStart = 3;
 constexpr int kPaLeast = 3;  // places of a share, at least
 
 struct PagedAttn {
@@ -32,6 +31,7 @@ struct PagedAttn {
   const int64_t* lengths;
   int rows, T, H, group, cols, qblocks;
   int units;  // of a row: kv heads x qblocks
+  int start;  // tiles that a unit's start counts as
   float scale_log2;
   float* part_o;   // [2 * workgroups][16 NB][D]: share w's unit begun before it at 2 w, its unit that goes on at 2 w + 1
   float* part_ml;  // [2 * workgroups][16 NB][2]
@@ -53,18 +53,18 @@ __device__ __forceinline__ PagedReach paged_reach(const PagedAttn& a, int b) {
 // The line: 64 rows at a time in the lanes of a wave, lane's row with ``tiles`` for each of its units, after ``before``
 // places of the rows ahead of it.
 struct PagedLine {
-  int b0, n, tiles, before;
-  __device__ int places() const { return tiles > 0 ? tiles + kPaStart : 0; }  // of a unit
+  int b0, n, tiles, before, places;  // places: of a unit
   // Rows b0 .. b0 + 63, the first after ``ahead`` places; returns the places up to their end.
   __device__ int take(const PagedAttn& a, int lane, int first, int ahead) {
     b0 = first;
-    n = tiles = 0;
+    n = tiles = places = 0;
     if (first + lane < a.rows) {
       const PagedReach r = paged_reach(a, first + lane);
       n = r.first;
       tiles = (r.last + 31) >> 5;
+      places = tiles > 0 ? tiles + a.start : 0;
     }
-    const int mine = places() * a.units, sum = wave_scan(mine);
+    const int mine = places * a.units, sum = wave_scan(mine);
     before = ahead + sum - mine;
     return ahead + __builtin_amdgcn_readlane(sum, kWave - 1);
   }
@@ -78,10 +78,8 @@ __device__ __forceinline__ int paged_total(const PagedAttn& a, int lane, PagedLi
 }
 
 // Places of a share: an even part of all for each workgroup, but not so few that what the second launch has to read
-// outweighs them.  Measured, a unit's start counted as 2, 3, 4 and 6 tiles and shares of 2, 3, 4 places and more, us: 1 slot
-// x 1433 keys, 8 x 512 e4m3, shares of 2 12.5, 3 13.3, 4 14.4, 8 18.2 (a tile after the other takes 1.1 us there); 32 over 8
-// x 128 9.8, 9.3, 9.4, 12.1; 8 slots x 5 of 750-2400 keys within 26-27 whichever; 16 slots of 4000-8188 keys, 16 over 2 x
-// 256, starts of 2 30.9, 3 30.5, 4 29.8.
+// outweighs them.  Measured, shares of 2, 3, 4, 8 places and more, us: 1 slot x 1433 keys, 8 x 512 e4m3 12.5, 13.3, 14.4, 18.2
+// (a tile after the other takes 1.1 us there); 32 over 8 x 128 9.8, 9.3, 9.4, 12.1.
 __device__ __forceinline__ int paged_share(int total) { return max((total + kPaSlots - 1) / kPaSlots, kPaLeast); }
 
 // A unit, and where its tiles are in the line: [from, from + tiles).
@@ -94,16 +92,16 @@ __device__ __forceinline__ PagedUnit paged_find(const PagedAttn& a, int lane, Pa
   int ahead = 0;
   if (a.rows > kWave) ahead = line.take(a, lane, 0, 0);
   for (;;) {
-    const uint64_t hit = __ballot(x >= line.before && x < line.before + line.places() * a.units);
+    const uint64_t hit = __ballot(x >= line.before && x < line.before + line.places * a.units);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       PagedUnit u;
       u.b = line.b0 + l;
       u.n = __builtin_amdgcn_readlane(line.n, l);
       u.tiles = __builtin_amdgcn_readlane(line.tiles, l);
-      const int start = __builtin_amdgcn_readlane(line.before, l), places = u.tiles + kPaStart;
+      const int start = __builtin_amdgcn_readlane(line.before, l), places = u.tiles + a.start;
       u.unit = (int)((uint32_t)(x - start) / (uint32_t)places);
-      u.from = start + u.unit * places + kPaStart;
+      u.from = start + u.unit * places + a.start;
       return u;
     }
     // (Past the last row only where another stream changed the lengths meanwhile: no unit, so that the search ends.)
@@ -143,7 +141,7 @@ struct PagedPiece {
 
 // NB: blocks of 16 query columns that share a read of the keys.  Two at most: four spill registers (64
 // columns, 42 us against 31 in twos).  Measured, with the second launch's 4-5 us: 8 slots x 5 of 750-2400 keys, 8 heads
-// x 512 e4m3 26 us (the stream at 4.1 TB/s), 32 x 128 bf16 43; 16 slots of 4000-8188, 32 over 8 x 128 e4m3 45 (5.4 TB/s).
+// x 512 e4m3 26 us (the stream at 4.1 TB/s), 32 x 128 bf16 37; 16 slots of 4000-8188, 32 over 8 x 128 e4m3 43 (5.5 TB/s).
 // Three tiles ahead in place of two 28.6 against 27.1 us; 1024, 768 and 256 workgroups 31, 29 and 27 against 27.  Loads that
 // are not kept in the caches, over more caches than those hold: the first of these 28.6 to 27.1, the second 45.6 to 42.8, the
 // third 48.7 to 44.6 (in bf16 83.8 to 75.3), 8 x 512 bf16 43.3 to 40.6; but 16 tokens, 16 over 2 heads x 256, whose keys four
@@ -451,7 +449,7 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
     for (int e = threadIdx.x; e < D; e += 64 * kPaWaves) out[e] = 0;
     return;
   }
-  const uint32_t from = before + unit * (tiles + kPaStart) + kPaStart, share = paged_share(total);
+  const uint32_t from = before + unit * (tiles + a.start) + a.start, share = paged_share(total);
   const int w0 = from / share, w1 = (from + tiles - 1) / share;
   if (w0 == w1) return;
   auto slot = [&](int part) { return (2 * (int64_t)part + (part == w0 ? 1 : 0)) * 16 * NB + col % (16 * NB); };
@@ -513,9 +511,15 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
   }
 }
 
+// Tiles that a unit's start counts as: more at head dim 128, where each of the four waves has tiles of its own, and more of
+// them of e4m3, which are shorter.  Measured, 3, 6 and 8, us: 8 slots x 5 of 750-2400 keys, 32 x 128 e4m3 35.7, 28.1, 25.9, bf16
+// 42.3, 37.2, 37.9; 8 slots, 32 over 8 x 128 e4m3 15.6, 13.7, 13.6; 16 over 2 x 256 bf16 13.7, 16.3, 16.2; 8 x 512 bf16 40.4,
+// 42.2, 42.1.
+inline int paged_start(int head_dim, bool f8) { return head_dim > 128 ? 3 : f8 ? 8 : 6; }
+
 // Workgroups of a call: what runs at once, but none that a full table would leave without a share.
-inline int paged_workgroups(int64_t units, int64_t positions) {
-  const int64_t places = units * ((positions + 31) / 32 + kPaStart), want = (places + kPaLeast - 1) / kPaLeast;
+inline int paged_workgroups(int64_t units, int64_t positions, int start) {
+  const int64_t places = units * ((positions + 31) / 32 + start), want = (places + kPaLeast - 1) / kPaLeast;
   return (int)(want < kPaSlots ? want : kPaSlots);
 }
 
@@ -538,7 +542,7 @@ extern "C" size_t omni_paged_attention_workspace(int64_t rows, int32_t tokens, i
   if (rows <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
   const int cols = tokens * (heads / kv_heads), wide = 16 * paged_blocks(cols);
   const int64_t units = rows * kv_heads * ((cols + wide - 1) / wide);
-  return (size_t)(2LL * paged_workgroups(units, (int64_t)width * page) * wide * (head_dim + 2) * 4);
+  return (size_t)(2LL * paged_workgroups(units, (int64_t)width * page, paged_start(head_dim, true)) * wide * (head_dim + 2) * 4);
 }
 
 extern "C" int omni_paged_attention(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
@@ -576,15 +580,16 @@ extern "C" int omni_paged_attention(const void* q, const void* k_pages, const vo
   const int64_t units = (int64_t)rows * a.units;
   // Places of the line, keys and groups are counted in 31 bits.
   if (a.cache.positions > 0x7fffff00LL || units > 0x7fffff00LL ||
-      units * ((a.cache.positions + 31) / 32 + kPaStart) > 0x7fffff00LL)
+      units * ((a.cache.positions + 31) / 32 + 8) > 0x7fff0000LL)
     return OMNI_ERR_SHAPE;
-  const int workgroups = paged_workgroups(units, a.cache.positions);
+  const bool f8 = cache_dtype == OMNI_E4M3;
+  a.start = paged_start(head_dim, f8);
+  const int workgroups = paged_workgroups(units, a.cache.positions, a.start);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + 2LL * workgroups * wide * head_dim;
   a.out = (uint16_t*)out;
   const hipStream_t s = (hipStream_t)stream;
-  const bool f8 = cache_dtype == OMNI_E4M3;
   if (head_dim == 128) {
     if (blocks == 1) paged_launch<128, 1>(a, f8, workgroups, s);
     else paged_launch<128, 2>(a, f8, workgroups, s);
