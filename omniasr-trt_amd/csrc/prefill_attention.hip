@@ -131,14 +131,16 @@ __device__ __forceinline__ int64_t pf_readlane64(int64_t v, int lane) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// Few blocks behind many keys: the longest block is the launch, ~1.05 us for each of its 64-key tiles, while other CUs have
+// Few blocks behind many keys: the longest block is the launch, ~1.4 us for each of its 64-key tiles, while other CUs have
 // nothing.  So a block is cut along its keys into parts, each a workgroup's, and a second launch (packed_attn_join_kernel)
-// joins their (O, m, l).  A part costs its start and end (~8 us) and 128 KB of O written and read, the join ~3 us: parts of
-// kPartLeast tiles and more, at most kPartMost of a block, where the longest block has kPartBlock tiles and 1.5 times what all
-// have for each CU.  Measured, us, whole and in parts: 20 queries behind 4000 keys, 8 heads x 512 72 / 36, 32 over 8 x 128 75 /
-// 34, 16 over 2 x 256 71 / 34; 64 behind 8000, 8 x 512 200 / 66, four of 64 behind 4000 142 / 62; 500 behind 6000, 8 x 512 116
-// / 80, 32 over 8 x 128 120 / 73.  Parts of 2 tiles and more, of any block: one prompt of 1433 45 / 57, four of 200-800 28 / 46.
-constexpr int kPartCus = 256, kPartLeast = 8, kPartBlock = 24, kPartMost = 16;
+// joins their (O, m, l).  A part costs its start and end (~8 us) and 128 KB of O written and read (~1 us of the join, which
+// takes 3 by itself): parts of kPartLeast tiles and more, at most kPartMost of a block; where CUs are plenty of
+// 0.8 sqrt(the block's tiles), so that the longest part and the join of all take the least together; where the longest block has kPartLong tiles and 1.5 times what all have for
+// each CU, or kPartBlock and four times.  Measured, us, whole and in parts: 20 queries behind 1000 keys, 8 heads x 512 30.0 /
+// 21.9, 32 over 8 x 128 29.0 / 19.4, 16 over 2 x 256 29.1 / 19.9; behind 4000, 8 x 512 72 / 31.0, 32 over 8 x 128 75 / 29.5; 64
+// behind 8000, 8 x 512 200 / 57; 300 behind 1000 38.3 / 30.8; 500 behind 6000 116 / 80.  Parts of 2 tiles and more, of any
+// block: one prompt of 1433 45 / 57, four of 200-800 28 / 46.
+constexpr int kPartCus = 256, kPartLeast = 4, kPartBlock = 12, kPartLong = 24, kPartMost = 16;
 
 // The rank of a lane's sequence by work (queries x keys, less what causality hides), the most first.
 __device__ __forceinline__ int pf_rank(const PfSequence& mine, int sequences) {
@@ -166,15 +168,21 @@ __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequen
     const int64_t mean = ((int64_t)min(nq, queries) + mine.nk - mine.nq + mine.nk) / 2;  // keys of a block, about
     const int64_t tiles = mean > 0 ? blocks * ((mean + 63) / 64) : 0;
     int all = lane < sequences ? (int)(tiles < 65536 ? tiles : 65536) : 0;
-    int longest = all > 0 ? (mine.nk + 63) / 64 : 0;
+    int longest = all > 0 ? (mine.nk + 63) / 64 : 0, count = lane < sequences ? blocks : 0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       all += __shfl_xor(all, o, kWave);
+      count += __shfl_xor(count, o, kWave);
       longest = max(longest, __shfl_xor(longest, o, kWave));
     }
-    const int even = (int)(((uint32_t)__builtin_amdgcn_readfirstlane(all) * (uint32_t)heads + kPartCus - 1) / kPartCus);
     longest = __builtin_amdgcn_readfirstlane(longest);
-    share = longest < max(kPartBlock, 3 * even / 2) ? longest : max(even, kPartLeast);
+    // Parts are whole tiles: half a part of each block's is lost.
+    const int room = max(kPartCus - __builtin_amdgcn_readfirstlane(count) * heads / 2, kPartCus / 4);
+    const int even = ((int)((uint32_t)__builtin_amdgcn_readfirstlane(all) * (uint32_t)heads) + room - 1) / room;
+    int least = kPartLeast;
+    while (25 * least * least < 16 * longest && least < 64) ++least;
+    const bool cut = longest >= kPartLong ? 2 * longest >= 3 * even : longest >= kPartBlock && longest >= 4 * even;
+    share = cut ? max(even, least) : longest;
   }
   const int l = __builtin_ctzll(__ballot(lane < sequences && pf_rank(mine, sequences) == r));
   PfSequence p;
@@ -1941,7 +1949,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // (query half u, rows r of O) of a block's four value waves, each lane what it held of O there.
 template <int D>
 __global__ __launch_bounds__(256) void packed_attn_join_kernel(PrefillArgs a) {
-  const int together = a.together, queries = (D == 128 ? kPairQ : D == 256 ? kPmQ : kWsQ) / together;
+  const int together = a.together, queries = D == 512 ? kWsQ : a.block;
   const int nqb = (a.width + queries - 1) / queries, j = (int)blockIdx.x >> 2, u = blockIdx.x >> 1 & 1, r = blockIdx.x & 1;
   const int hb = blockIdx.y, lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
   const int vw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1949,6 +1957,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(PrefillArgs a) {
   const PfSequence seq = pf_ranked(a, (int)gridDim.z, blockIdx.z, queries, gridDim.y, share);
   const int qb = (nqb - 1 - j) * queries;
   const int group = D == 128 ? vw : D == 256 ? vw >> 1 : 0, h = hb * together + group % together;
+  if (64 * (group / together) >= queries) return;  // no queries
   const PfSpan sp = pf_packed_span(a, h, seq);
   const int keys = min(qb + queries, sp.nq) + sp.before;
   if (qb >= sp.nq || keys <= 0) return;
@@ -1970,7 +1979,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(PrefillArgs a) {
   for (int e = 0; e < 4; ++e) o[e][0] = o[e][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
   if (first >= sp.nq) return;
-#pragma unroll 4
+#pragma unroll 1  // (by 4 the launch of 16 parts takes 84 us in place of 57)
   for (int p = 0; p < parts && query < sp.nq; ++p) {
     const float* from = a.part_o + (slot + p) * kPartO + (vw * 4 + u * 2 + r) * (8 * 256) + lane * 4;
     const f32x2_t one = ml(p, sw, 0);
@@ -2009,10 +2018,12 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(PrefillArgs a) {
 // Parts of a block at most, for a launch of ``blocks`` that see up to ``keys`` keys: 1 where every CU has a block.  (Their
 // workgroups are launched before it is known how many there are.  Up to 4 x 256 of them cost 2 x 600 behind 3000 10 us where
 // there were none, 2 x 256 4 us; three prompts of 60-200 behind 1000, with none, take 37 us in place of 34.)
-inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int longest) {
+inline int packed_parts(int64_t blocks, int sequences, int64_t keys, int64_t longest) {
   const int64_t tiles = (keys + 63) / 64;
   if (blocks >= kPartCus || sequences > kWave || tiles < kPartBlock) return 1;
-  if (keys <= longest && 3 * blocks >= 2 * kPartCus) return 1;  // no earlier keys: a block's mean is half the longest
+  if (tiles < kPartLong && 3 * blocks > kPartCus) return 1;  // not four times an even part
+  // No earlier keys: a block's mean is half the longest.
+  if (keys <= longest && (tiles < kPartLong || 3 * blocks >= 2 * kPartCus)) return 1;
   return (int)std::min({kPartCus / blocks + 1, tiles / kPartLeast, (int64_t)kPartMost});
 }
 
@@ -2033,13 +2044,29 @@ inline bool packed_chains(int64_t nqb, int heads, int sequences, int head_dim) {
          each <= kPfRounds * kWsPerXcd;
 }
 
-// Heads of a kv head in a block, and queries of a head.
-inline int packed_together(int head_dim, int heads_per_kv) {
-  if (head_dim == 128) return heads_per_kv % 4 == 0 ? 4 : heads_per_kv % 2 == 0 ? 2 : 1;
-  return head_dim == 256 && heads_per_kv % 2 == 0 ? 2 : 1;
-}
-inline int packed_queries(int head_dim, int heads_per_kv) {
-  return (head_dim == 128 ? kPairQ : head_dim == 256 ? kPmQ : kWsQ) / packed_together(head_dim, heads_per_kv);
+// How a call is launched: heads of a kv head and queries of each in a block, blocks in all, in chains, in parts.
+struct PackedPlan {
+  int together, rows, parts;
+  bool chains;
+  int64_t units, blocks;  // units: blocks of heads x sequences
+};
+inline PackedPlan packed_plan(int head_dim, int heads, int kv_heads, int sequences, int64_t longest, int64_t keys) {
+  const int group = heads / kv_heads;
+  PackedPlan p;
+  p.together = 1;
+  if (head_dim == 128) p.together = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  if (head_dim == 256) p.together = group % 2 == 0 ? 2 : 1;
+  p.rows = (head_dim == 128 ? kPairQ : head_dim == 256 ? kPmQ : kWsQ) / p.together;
+  p.units = (int64_t)heads / p.together * sequences;
+  auto count = [&] { return p.blocks = (longest + p.rows - 1) / p.rows * p.units; };
+  p.chains = packed_chains(count() / p.units, heads / p.together, sequences, head_dim);
+  p.parts = 1;
+  if (p.chains) return p;
+  if ((keys + 63) / 64 >= kPartLong) p.parts = packed_parts(p.blocks, sequences, keys, longest);
+  if (p.parts > 1) return p;
+  p.rows = packed_block(p.rows, longest, p.units);
+  p.parts = packed_parts(count(), sequences, keys, longest);
+  return p;
 }
 
 // Head dim 128 in blocks of 192 queries, for the launches of small_blocks: one workgroup of 4 waves, two workgroups per
@@ -2325,10 +2352,8 @@ extern "C" size_t omni_packed_attention_workspace(int32_t sequences, int64_t key
                                                   int32_t kv_heads, int32_t head_dim) {
   if (sequences <= 0 || keys <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
   if (head_dim != 128 && head_dim != 256 && head_dim != 512) return 0;
-  const int group = heads / kv_heads, rows = omni::packed_queries(head_dim, group);
-  const int64_t blocks = (longest + (int64_t)rows - 1) / rows * (heads / omni::packed_together(head_dim, group)) * sequences;
-  const int parts = omni::packed_parts(blocks, sequences, keys, longest);
-  return parts == 1 ? 0 : (size_t)(blocks * parts * (omni::kPartO + omni::kPartMl) * 4);
+  const omni::PackedPlan p = omni::packed_plan(head_dim, heads, kv_heads, sequences, longest, keys);
+  return p.parts == 1 ? 0 : (size_t)(p.blocks * p.parts * (omni::kPartO + omni::kPartMl) * 4);
 }
 
 extern "C" int omni_packed_attention(const void* q, const void* k, const void* v, int64_t k_stride_pos,
@@ -2371,27 +2396,22 @@ extern "C" int omni_packed_attention(const void* q, const void* k, const void* v
   a.v_pos = v_stride_pos;
   a.v_head = v_stride_head;
   a.heads_per_kv = heads / kv_heads;
-  a.together = omni::packed_together(head_dim, a.heads_per_kv);
-  const int rows = omni::packed_queries(head_dim, a.heads_per_kv);
-  dim3 grid((longest + rows - 1) / rows, heads / a.together, sequences);
-  // The blocks are counted in 31 bits, a launch's threads along x, 512 to a block, in 32.
-  if (grid.x >= (1u << 23) || (int64_t)grid.x * grid.y * grid.z > 0x7fffffffLL) return OMNI_ERR_SHAPE;
-  const int64_t blocks = (int64_t)grid.x * grid.y * grid.z;
   const int64_t seen = k_starts == starts ? std::min<int64_t>(keys, longest) : keys;  // by one sequence, at most
-  a.parts = omni::packed_parts(blocks, sequences, seen, longest);
+  const omni::PackedPlan p = omni::packed_plan(head_dim, heads, kv_heads, sequences, longest, seen);
+  dim3 grid(p.blocks / p.units, heads / p.together, sequences);
+  // The blocks are counted in 31 bits, a launch's threads along x, 512 to a block, in 32.
+  if (grid.x >= (1u << 23) || p.blocks > 0x7fffffffLL) return OMNI_ERR_SHAPE;
+  a.together = p.together;
+  a.block = p.rows;
+  a.parts = p.parts;
+  a.sequences = sequences;
+  const bool chains = p.chains;
   if (a.parts > 1) {
     if (!workspace || ((uintptr_t)workspace & 255u) ||
         workspace_bytes < omni_packed_attention_workspace(sequences, seen, longest, heads, kv_heads, head_dim))
       return OMNI_ERR_WORKSPACE;
     a.part_o = (float*)workspace;
-    a.part_ml = a.part_o + blocks * a.parts * omni::kPartO;
-  }
-  const bool chains = omni::packed_chains(grid.x, grid.y, sequences, head_dim);
-  a.sequences = sequences;
-  a.block = rows;
-  if (a.parts == 1 && !chains) {
-    a.block = omni::packed_block(rows, longest, blocks / grid.x);
-    grid.x = (longest + a.block - 1) / a.block;
+    a.part_ml = a.part_o + p.blocks * a.parts * omni::kPartO;
   }
   const dim3 join(grid.x * 4, grid.y, grid.z);
   grid.z *= a.parts;

@@ -517,6 +517,14 @@ def test_packed_attention_of_few_queries_behind_many_keys(cuda, heads, kv, dim):
     packed_case(cuda, heads, kv, dim, [2000], [-300], dim + heads + 4)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(24, 24, 128), (12, 6, 128), (24, 24, 256), (16, 8, 256), (4, 4, 512)])
+def test_packed_attention_in_parts_of_smaller_blocks(cuda, heads, kv, dim):
+    """Blocks of fewer queries, cut along their keys: around 12 and 24 tiles, and in sequences of unlike lengths."""
+    for i, (n, past) in enumerate([(64, 640), (65, 650), (100, 700), (130, 1350), (190, 1410)]):
+        packed_case(cuda, heads, kv, dim, [n], [past], dim + heads + i)
+    packed_case(cuda, heads, kv, dim, [5, 70], [900, 30], dim + heads + 9)
+
+
 def test_packed_attention_in_parts_captured(cuda):
     """One captured launch for lengths that are cut and that are not; calls on two streams share nothing."""
     g = gen(41)
