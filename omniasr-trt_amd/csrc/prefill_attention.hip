@@ -134,12 +134,12 @@ __device__ __forceinline__ int64_t pf_readlane64(int64_t v, int lane) {
 // Few blocks behind many keys: the longest block is the launch, ~1.4 us for each of its 64-key tiles, while other CUs have
 // nothing.  So a block is cut along its keys into parts, each a workgroup's, and a second launch (packed_attn_join_kernel)
 // joins their (O, m, l).  A part costs its start and end (~8 us) and 128 KB of O written and read (~1 us of the join, which
-// takes 3 by itself): parts of kPartLeast tiles and more, at most kPartMost of a block; where CUs are plenty of
-// 0.8 sqrt(the block's tiles), so that the longest part and the join of all take the least together; where the longest block has kPartLong tiles and 1.5 times what all have for
-// each CU, or kPartBlock and four times.  Measured, us, whole and in parts: 20 queries behind 1000 keys, 8 heads x 512 30.0 /
-// 21.9, 32 over 8 x 128 29.0 / 19.4, 16 over 2 x 256 29.1 / 19.9; behind 4000, 8 x 512 72 / 31.0, 32 over 8 x 128 75 / 29.5; 64
-// behind 8000, 8 x 512 200 / 57; 300 behind 1000 38.3 / 30.8; 500 behind 6000 116 / 80.  Parts of 2 tiles and more, of any
-// block: one prompt of 1433 45 / 57, four of 200-800 28 / 46.
+// takes 3 by itself): parts of kPartLeast tiles and more, at most kPartMost of a block; where CUs are plenty of 0.8 sqrt(the
+// block's tiles), so that a part and the join of all take the least together.  Only where the longest block has kPartLong
+// tiles and 1.5 times what all have for each CU, or kPartBlock and four times.  Measured, us, whole and in parts: 20 queries
+// behind 1000 keys, 8 heads x 512 30.0 / 21.9, 32 over 8 x 128 29.0 / 19.4, 16 over 2 x 256 29.1 / 19.9; behind 4000, 8 x
+// 512 72 / 31.0, 32 over 8 x 128 75 / 29.5; 64 behind 8000, 8 x 512 200 / 57; 300 behind 1000 38.3 / 30.8; 500 behind 6000
+// 116 / 80.  Parts of 2 tiles and more, of any block: one prompt of 1433 45 / 57, four of 200-800 28 / 46.
 constexpr int kPartCus = 256, kPartLeast = 4, kPartBlock = 12, kPartLong = 24, kPartMost = 16;
 
 // The rank of a lane's sequence by work (queries x keys, less what causality hides), the most first.
