@@ -421,8 +421,8 @@ int omni_silu_mul(const void *gate_inner, int64_t gate_inner_stride, void *out, 
  * head_dim] bf16 (q | k | v).  The rotated q goes to ``q_out`` [n_tokens, heads, head_dim]; the rotated k and the v of
  * token n to position cache_pos[n] (NULL: pos[n]) of cache row slots[n] (NULL: n).  Tokens whose row, position or page is
  * outside the cache are not written.  A call's (row, position) pairs are distinct: of two equal ones either token's values
- * may stay, in part.  K and V have pages and exponents of their own.  ``k_out`` [n_tokens, kv_heads, head_dim], if not NULL, gets the rotated k in bf16 as well, for
- * omni_packed_attention over the same prompts.
+ * may stay, in part.  K and V have pages and exponents of their own.  ``k_out`` [n_tokens, kv_heads, head_dim], if not
+ * NULL, gets the rotated k in bf16 as well, for omni_packed_attention over the same prompts.
  * OMNI_E4M3: exponent e of a vector x is the least integer with max |x| <= 448 * 2^e, over the finite x and at least -126
  * (0 for a vector of zeros); the code is x * 2^-e to the nearest e4m3, ties to even, from the rotated fp32 k (at e = 120, where
  * bf16 ends, at most 240); infinities, which e4m3 lacks, and NaN become NaN.
@@ -464,7 +464,8 @@ int omni_paged_attention(const void *q, const void *k_pages, const void *v_pages
 
 /*
  * Bytes of workspace omni_packed_attention needs: 0 but for few queries behind many keys.  ``keys``: as for the call, or
- * ``longest``, if less, where ``k_starts`` is ``starts``.
+ * ``longest``, if less, where ``k_starts`` is ``starts``.  Fewer keys or queries may take more than many do (other cuts):
+ * one workspace for calls of every size is 66 MiB.
  */
 size_t omni_packed_attention_workspace(int32_t sequences, int64_t keys, int32_t longest, int32_t heads,
                                        int32_t kv_heads, int32_t head_dim);

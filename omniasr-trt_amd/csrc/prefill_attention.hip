@@ -8,7 +8,7 @@
 // keys [0, i + nk - nq] of nk.  What bounds a tile is the same; what they add is lengths from the device, rows of any stride, a
 // mask on every tile that not all of a wave's queries see, and at head dim 128 up to four heads of a kv head in a block (64
 // queries of each: a short prompt fills a block, and the heads share its tiles).  Measured, us: 8 prompts of 750-2400, 8 heads
-// x 512 195 (705 TFLOP/s), 32 over 8 x 128 175; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 80 (a head to a block
+// x 512 195 (705 TFLOP/s), 32 over 8 x 128 175; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 76 (a head to a block
 // 113); one of 1433, 32 x 128 42.
 #include <math.h>
 

@@ -168,3 +168,12 @@ def test_c_abi_refusals_before_launch():
     big = [*packed[:9], 65535, 2 ** 30, 2 ** 30, 2 ** 24, 4, 4, 512, *packed[16:]]  # 65535 x 2^18 x 4 blocks
     assert lib.omni_packed_attention(*big) == -3
     assert lib.omni_packed_attention(*big[:9], 1, 2 ** 30, 2 ** 30, 2 ** 30, 4, 1, 128, *big[16:]) == -3  # 2^25 along x
+
+
+def test_packed_attention_workspace_of_every_size():
+    lib = _lib.load()
+    most = max(lib.omni_packed_attention_workspace(sequences, keys, longest, kv * group, kv, dim)
+               for sequences in (1, 2, 3, 9, 40, 64) for keys in (500, 704, 1472, 1473, 9000, 200000)
+               for longest in (1, 64, 65, 128, 257, 1000, 5000) for kv in (1, 3, 8, 25) for group in (1, 2, 4, 7)
+               for dim in (128, 256, 512))
+    assert 32 << 20 < most <= 66 << 20
