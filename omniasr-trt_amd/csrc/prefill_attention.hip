@@ -165,8 +165,12 @@ __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequen
   const PfSequence mine = pf_sequence(a, min(lane, sequences - 1));
   if (a.parts > 1) {
     const int nq = min(mine.nq, a.width), blocks = (nq + queries - 1) / queries;
-    const int64_t mean = ((int64_t)min(nq, queries) + mine.nk - mine.nq + mine.nk) / 2;  // keys of a block, about
-    const int64_t tiles = mean > 0 ? blocks * ((mean + 63) / 64) : 0;
+    // Keys of the first block and, about, of a block's mean.  With more queries than keys and a block's worth the first ones
+    // see none: only the last nk queries' blocks have any, nk / 2 about.
+    const int64_t first = (int64_t)min(nq, queries) + mine.nk - mine.nq;
+    const int64_t mean = first > 0 ? (first + mine.nk) / 2 : (mine.nk + 1) / 2;
+    const int seeing = first > 0 ? blocks : (int)(((int64_t)mine.nk + queries - 1) / queries);
+    const int64_t tiles = blocks > 0 ? seeing * ((mean + 63) / 64) : 0;
     int all = lane < sequences ? (int)(tiles < 65536 ? tiles : 65536) : 0;
     int longest = all > 0 ? (mine.nk + 63) / 64 : 0, count = lane < sequences ? blocks : 0;
 #pragma unroll
@@ -182,7 +186,7 @@ __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequen
     int least = kPartLeast;
     while (25 * least * least < 16 * longest && least < 64) ++least;
     const bool cut = longest >= kPartLong ? 2 * longest >= 3 * even : longest >= kPartBlock && longest >= 4 * even;
-    share = cut ? max(even, least) : longest;
+    share = cut ? max(even, least) : max(longest, 1);
   }
   const int l = __builtin_ctzll(__ballot(lane < sequences && pf_rank(mine, sequences) == r));
   PfSequence p;

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import paged as op
-from omniasr_trt_amd import batching, kernels, modeling
+from omniasr_trt_amd import _lib, batching, kernels, modeling
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -565,6 +565,26 @@ def test_packed_attention_in_parts_does_not_see_what_is_masked(cuda, heads, kv, 
     assert all(torch.equal(o.view(torch.int16), out[0].view(torch.int16)) for o in out)
     close(torch.where(fine, out[0].double(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, size, 0.0), q, k,
           dim ** -0.5)
+
+
+def litter(cuda):
+    """Finite numbers in the memory that the next tensors and workspaces take: what is read unwritten shows."""
+    torch.cuda.empty_cache()
+    torch.full((512 << 20,), 0x40, dtype=torch.uint8, device=cuda)
+
+
+@pytest.mark.parametrize("heads,kv,dim,queries,keys,behind", [
+    (8, 8, 512, [100], [10], 1990), (8, 8, 512, [600], [200], 1800), (8, 8, 128, [300], [20], 1980),
+    (16, 2, 256, [300], [20], 1980), (2, 2, 512, [600] * 8, [200] * 8, 0), (2, 1, 128, [400, 30, 7], [40, 0, 900], 1200),
+    (4, 4, 256, [1000, 64], [1, 3], 3000), (1, 1, 512, [900, 900], [800, 30], 700)])
+def test_packed_attention_in_parts_of_many_queries_over_few_keys(cuda, heads, kv, dim, queries, keys, behind):
+    """A buffer long enough to be cut, sequences of more queries than keys: their first blocks see no key, and no block has
+    many tiles."""
+    longest, rows = max(queries), sum(keys) + behind
+    assert _lib.load().omni_packed_attention_workspace(len(queries), rows, longest, heads, kv, dim) > 0
+    for _ in range(2):
+        litter(cuda)
+        packed_case(cuda, heads, kv, dim, queries, [k - n for n, k in zip(queries, keys)], dim + heads, behind=behind)
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(2, 1, 128), (8, 8, 128), (2, 1, 256), (2, 1, 512)])
