@@ -462,7 +462,7 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
     for (int k = 0; k < kBatch; ++k) {
       const int part = p0 + k * kPaWaves;
       const int64_t s = slot(min(part, w1));
-      mp[k] = part <= w1 ? a.part_ml[s * 2] : -INFINITY;
+      mp[k] = part <= w1 ? a.part_ml[s * 2] : -INFINITY;  // (past the last part: its loads again, not used)
       lp[k] = a.part_ml[s * 2 + 1];
 #pragma unroll
       for (int e = 0; e < kPer; ++e) op[k][e] = a.part_o[s * D + kPer * lane + e];
@@ -476,8 +476,9 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
     for (int e = 0; e < kPer; ++e) o[e] *= f0;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (mp[k] == -INFINITY) continue;  // no key seen
-      const float f = __builtin_amdgcn_exp2f(mp[k] - top);
+      if (p0 + k * kPaWaves > w1) break;
+      // -inf: no key seen, or scores that are all NaN, which 0 times the part's sums keeps.
+      const float f = mp[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp[k] - top);
       l += f * lp[k];
 #pragma unroll
       for (int e = 0; e < kPer; ++e) o[e] += f * op[k][e];

@@ -358,6 +358,29 @@ def test_paged_attention_of_values_whose_exponent_makes_them_infinite(cuda):
     close(out[:1], want, size, q, torch.full((1, 128), 4.0, device=cuda), 0.1)
 
 
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (16, 2, 256), (32, 8, 128), (8, 8, 128)])
+@pytest.mark.parametrize("n", [33, 65, 1433])
+def test_paged_attention_of_nan_where_units_are_cut(cuda, heads, kv, dim, n, fp8):
+    """A query with a NaN, and one whose newest key, the only one of its tile, has one: NaN wherever the cuts fall."""
+    say(f"NaN heads={heads} kv={kv} dim={dim} n={n} fp8={fp8}")
+    g = gen(n + dim)
+    k, v, table, scales = make_cache(cuda, g, kv, dim, 16, [n, n, n], fp8)
+    q, lengths = normal((3, heads, dim), g, cuda), torch.tensor([n, n, n], device=cuda)
+    q[0, :, 7] = float("nan")
+    page, off = op.cell(table, 16, k.size(0), 1, n - 1)
+    if fp8:
+        k.view(torch.uint8)[page, :, off, 9] = 0x7F
+    else:
+        k[page, :, off, 9] = float("nan")
+    out = kernels.paged_attention(q, k, v, table, lengths, 1, dim ** -0.5, **scales)
+    torch.cuda.synchronize()
+    assert out[:2].isnan().all()
+    want, size = op.paged_attention(q, k, v, table, [n, n, n], 1, dim ** -0.5, **scales)
+    assert want[:2].isnan().all()
+    close(out[2], want[2], size[2], q[2:], torch.full((1, dim), 4.0, device=cuda), dim ** -0.5)
+
+
 # ---------------------------------------------------------------------------------------------- packed attention
 
 def packed_case(cuda, heads, kv, dim, queries, past, seed, longest=None, behind=0, strided=True, scale=None):
