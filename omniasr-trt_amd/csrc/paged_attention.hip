@@ -35,6 +35,7 @@ struct PagedAttn {
   float scale_log2;
   float* part_o;   // [2 * workgroups][16 NB][D]: share w's unit begun before it at 2 w, its unit that goes on at 2 w + 1
   float* part_ml;  // [2 * workgroups][16 NB][2]
+  int* ahead;      // [rows + 1]: places ahead of each row, and all; from the first launch for the second
   uint16_t* out;   // [rows * T, H, D]
 };
 
@@ -70,10 +71,15 @@ struct PagedLine {
   }
 };
 
-// All rows' places; ``line`` is left at the last 64 rows.
-__device__ __forceinline__ int paged_total(const PagedAttn& a, int lane, PagedLine& line) {
+// All rows' places; ``line`` is left at the last 64 rows.  One wave keeps them (``keep``) for the second launch, whose
+// workgroups, one for each query and head, would each have to pass over all rows.
+__device__ __forceinline__ int paged_total(const PagedAttn& a, int lane, PagedLine& line, bool keep) {
   int total = 0;
-  for (int b0 = 0; b0 < a.rows; b0 += kWave) total = line.take(a, lane, b0, total);
+  for (int b0 = 0; b0 < a.rows; b0 += kWave) {
+    total = line.take(a, lane, b0, total);
+    if (keep && b0 + lane < a.rows) a.ahead[b0 + lane] = line.before;
+  }
+  if (keep && lane == 0) a.ahead[a.rows] = total;
   return total;
 }
 
@@ -87,10 +93,10 @@ struct PagedUnit {
   int b, n, unit, tiles, from;
 };
 
-// The unit that holds place ``x`` (in its start or its tiles).
+// The unit that holds place ``x`` (in its start or its tiles).  A workgroup's places follow each other, so the search goes
+// on from the rows it is at and passes over all of them once.
 __device__ __forceinline__ PagedUnit paged_find(const PagedAttn& a, int lane, PagedLine& line, int x) {
-  int ahead = 0;
-  if (a.rows > kWave) ahead = line.take(a, lane, 0, 0);
+  if (x < __builtin_amdgcn_readlane(line.before, 0)) line.take(a, lane, 0, 0);
   for (;;) {
     const uint64_t hit = __ballot(x >= line.before && x < line.before + line.places * a.units);
     if (hit) {
@@ -106,7 +112,7 @@ __device__ __forceinline__ PagedUnit paged_find(const PagedAttn& a, int lane, Pa
     }
     // (Past the last row only where another stream changed the lengths meanwhile: no unit, so that the search ends.)
     if (line.b0 + kWave >= a.rows) return PagedUnit{0, 0, 0, 0, x};
-    ahead = line.take(a, lane, line.b0 + kWave, ahead);
+    line.take(a, lane, line.b0 + kWave, __builtin_amdgcn_readlane(line.before + line.places * a.units, kWave - 1));
   }
 }
 
@@ -161,7 +167,7 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), sl = w % kSlices, stream = w / kSlices;
 
   PagedLine line;
-  const int total = paged_total(a, lane, line), share = paged_share(total);
+  const int total = paged_total(a, lane, line, blockIdx.x == 0 && w == 0), share = paged_share(total);
   int x = blockIdx.x * share;
   if (x >= total) return;
   const int x_end = min(x + share, total);
@@ -435,21 +441,14 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attn_merge_kernel(PagedAt
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x, b = row / a.T, h = blockIdx.y;
   const int col = (row - b * a.T) * a.group + h % a.group, unit = h / a.group * a.qblocks + col / (16 * NB);
-  PagedLine line;
-  int total = 0, tiles = 0, before = 0;
-  for (int b0 = 0; b0 < a.rows; b0 += kWave) {
-    total = line.take(a, lane, b0, total);
-    if (b >= b0 && b < b0 + kWave) {
-      tiles = __builtin_amdgcn_readlane(line.tiles, b - b0);
-      before = __builtin_amdgcn_readlane(line.before, b - b0);
-    }
-  }
+  const int total = a.ahead[a.rows], before = a.ahead[b], places = (int)((uint32_t)(a.ahead[b + 1] - before) / (uint32_t)a.units);
+  const int tiles = places > 0 ? places - a.start : 0;
   uint16_t* out = a.out + ((int64_t)row * a.H + h) * D;
   if (tiles == 0) {
     for (int e = threadIdx.x; e < D; e += 64 * kPaWaves) out[e] = 0;
     return;
   }
-  const uint32_t from = before + unit * (tiles + a.start) + a.start, share = paged_share(total);
+  const uint32_t from = before + unit * places + a.start, share = paged_share(total);
   const int w0 = from / share, w1 = (from + tiles - 1) / share;
   if (w0 == w1) return;
   auto slot = [&](int part) { return (2 * (int64_t)part + (part == w0 ? 1 : 0)) * 16 * NB + col % (16 * NB); };
@@ -543,7 +542,8 @@ extern "C" size_t omni_paged_attention_workspace(int64_t rows, int32_t tokens, i
   if (rows <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
   const int cols = tokens * (heads / kv_heads), wide = 16 * paged_blocks(cols);
   const int64_t units = rows * kv_heads * ((cols + wide - 1) / wide);
-  return (size_t)(2LL * paged_workgroups(units, (int64_t)width * page, paged_start(head_dim, true)) * wide * (head_dim + 2) * 4);
+  const int64_t parts = 2LL * paged_workgroups(units, (int64_t)width * page, paged_start(head_dim, true)) * wide;
+  return (size_t)(parts * (head_dim + 2) * 4 + (rows + 1) * 4);
 }
 
 extern "C" int omni_paged_attention(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
@@ -589,6 +589,7 @@ extern "C" int omni_paged_attention(const void* q, const void* k_pages, const vo
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + 2LL * workgroups * wide * head_dim;
+  a.ahead = (int*)(a.part_ml + 2LL * workgroups * wide * 2);
   a.out = (uint16_t*)out;
   const hipStream_t s = (hipStream_t)stream;
   if (head_dim == 128) {

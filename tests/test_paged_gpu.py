@@ -284,6 +284,34 @@ def test_paged_attention_of_long_rows_and_many_rows(cuda):
     attention_case(cuda, 2, 1, 128, 16, 2, [(37 * i) % 91 for i in range(70)], True, 3)
 
 
+def test_paged_attention_of_very_many_rows(cuda):
+    """131072 rows of 0 to 16 keys: right, and in time that grows with the rows (8 times as many: not 64 times)."""
+    g, page, dim, heads, took = gen(35), 16, 128, 2, []
+    pool = [normal((64, 1, page, dim), g, cuda) for _ in "kv"]
+    for rows in (1 << 14, 1 << 17):
+        say("paged attention of", rows, "rows")
+        at = torch.arange(rows, device=cuda)
+        table, lengths = ((at * 7) % 64).int()[:, None], at % 17
+        q = normal((4096, heads, dim), g, cuda).repeat(rows // 4096, 1, 1)
+        out = kernels.paged_attention(q, *pool, table, lengths, 1, 0.1)
+        events = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
+        events[0].record()
+        for e in events[1:]:
+            kernels.paged_attention(q, *pool, table, lengths, 1, 0.1)
+            e.record()
+        torch.cuda.synchronize()
+        took.append(min(a.elapsed_time(b) for a, b in zip(events, events[1:])))
+        for some in at.split(1 << 14):
+            k, v = (x[table[some, 0].long(), 0].double() for x in pool)
+            scores = (q[some].double()[:, :, None] * k[:, None]).sum(-1) * 0.1
+            hidden = (torch.arange(page, device=cuda) >= lengths[some, None])[:, None]
+            w = torch.softmax(scores.masked_fill(hidden, -torch.inf), -1).masked_fill(hidden, 0.0)
+            want, size = ((w[..., None] * x[:, None]).sum(2) for x in (v, v.abs()))
+            close(out[some], want, size, q[some], pool[0], 0.1)
+    say("ms", took)
+    assert took[1] < 24 * took[0]
+
+
 def test_paged_attention_with_large_scores(cuda):
     """Scores of hundreds: the reference maximum moves, weights underflow."""
     attention_case(cuda, 4, 2, 128, 32, 3, [500, 40], False, 5, scale=1.0)
