@@ -436,7 +436,8 @@ int omni_rope_kv_paged(const void *qkv, int64_t qkv_row_stride, const float *cs,
 
 /*
  * Cached vectors read back: k_out[n], v_out[n] ([n_tokens, kv_heads, head_dim] bf16) = the K and V of position pos[n] of
- * cache row slots[n]; zeros where the row, position or page is outside the cache.  Exact: bf16 holds code * 2^e.
+ * cache row slots[n]; zeros where the row, position or page is outside the cache.  Exact, but for e4m3 with an exponent
+ * byte of 1 or 2 (|x| <= 448 * 2^-125): there code * 2^e to the nearest multiple of 2^-133, bf16's least number.
  */
 int omni_paged_read(const void *k_pages, const void *v_pages, const void *k_scale, const void *v_scale,
                     int32_t pages, int32_t page, const int32_t *table, int64_t table_stride, int64_t rows,

@@ -4,7 +4,7 @@
 // The products and lane layouts are those of attn_tiles.h (S^T = K Q^T and O = P V on v_mfma_f32_16x16x32_bf16), with the
 // key rows behind pointers of each lane's own: lane (c = lane % 16, g = lane / 16) reads K rows 8 (c / 4) + 4 mb + c % 4
 // (mb = 0, 1) and V rows 8g + j (j < 8) of a tile, each within 8 keys in a row, so that a page of 16 or more positions
-// holds them.  e4m3 is multiplied as bf16: code * 2^e is exact there.
+// holds them.  e4m3 is multiplied as bf16, which holds code * 2^e (e4m3x2_to_bf16).
 #pragma once
 
 #include "attn_tiles.h"

@@ -35,7 +35,8 @@ __device__ __forceinline__ int64_t paged_cell(const PagedCache& a, int64_t r, in
 // 2^(b - 127) of an exponent byte.  (b = 0 would be 2^-127, which is no normal number; no vector is written with it.)
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// Two e4m3 codes (the low or the high half of ``w``) times ``scale``, a power of two, as bf16: exact.
+// Two e4m3 codes (the low or the high half of ``w``) times ``scale``, a power of two, as bf16: exact from
+// 2^-124 on, below to the nearest multiple of bf16's least number, 2^-133 (the least code is 2^-9).
 template <bool kHigh>
 __device__ __forceinline__ uint32_t e4m3x2_to_bf16(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHigh));

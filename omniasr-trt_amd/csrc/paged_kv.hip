@@ -3,7 +3,8 @@
 // Write: the new tokens' q and k rotated as rope_kv_append rotates them (each product rounded on its own), k and v put
 // into their pages in bf16 or quantised to e4m3.  A quantised vector x of one (token, kv head) keeps one exponent e, the
 // least with max |x| <= 448 * 2^e: x * 2^-e is exact, so a value is rounded once, to the nearest e4m3 (ties to even), and
-// what is read back, code * 2^e, is exact in bf16.  (A scale max |x| / 448 would use up to one more binade of e4m3's range
+// what is read back, code * 2^e, is exact in bf16 from e = -124 on (below, multiples of bf16's least number, 2^-133, at most
+// half of it off).  (A scale max |x| / 448 would use up to one more binade of e4m3's range
 // and cost a second rounding at the division and a third when read; e4m3's relative precision is the same in every
 // binade above 2^-6, 14 below the largest.)  k is quantised from the rotated fp32 values, not from their bf16 rounding.
 //

@@ -724,9 +724,10 @@ def rope_kv_paged(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
 def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, slots: torch.Tensor,
                pos: torch.Tensor, *, k_scale: torch.Tensor | None = None,
                v_scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """The cached k and v at position ``pos[n]`` of cache row ``slots[n]``, bf16 [N, kv heads, D] each (exact: e4m3 times
-    its power of two is a bf16 number), zeros where the row, position or page is outside the cache.  What a prompt that
-    goes on behind cached positions attends to (:func:`packed_attention`).  The cache as for :func:`rope_kv_paged`."""
+    """The cached k and v at position ``pos[n]`` of cache row ``slots[n]``, bf16 [N, kv heads, D] each, zeros where the
+    row, position or page is outside the cache.  Exact: e4m3 times its power of two is a bf16 number, but for vectors of up to
+    448 * 2^-125, whose values are rounded to multiples of 2^-133, bf16's least.  What a prompt that goes on behind cached
+    positions attends to (:func:`packed_attention`).  The cache as for :func:`rope_kv_paged`."""
     lib = _lib.load()
     device = k_pages.get_device()
     (_, kv, _, dim), pages, cache, here = _paged(k_pages, v_pages, table, k_scale, v_scale, device)

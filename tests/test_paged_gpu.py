@@ -180,6 +180,28 @@ def test_quantised_vectors_of_zeros_extremes_and_what_is_not_finite(cuda):
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0), want.nan_to_num(0))
 
 
+def test_every_code_at_every_exponent_read_back(cuda):
+    """code * 2^(byte - 127) in bf16: exact from byte 3 on; at 1 and 2 the least codes lie below bf16's least number, 2^-133,
+    and are rounded to a multiple of it."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    pages = codes.repeat(1, 1, 256, 1).to(cuda).view(torch.float8_e4m3fn)
+    byte = torch.arange(256, dtype=torch.uint8)[None, None]
+    byte[..., 0], byte[..., 255] = 1, 254  # what is never written
+    table, at = torch.zeros(1, 1, dtype=torch.int32, device=cuda), torch.arange(256, device=cuda)
+    kk, vv = kernels.paged_read(pages, pages.clone(), table, torch.zeros_like(at), at, k_scale=byte.to(cuda),
+                                v_scale=byte.to(cuda))
+    torch.cuda.synchronize()
+    exact = codes.view(torch.float8_e4m3fn).double() * torch.exp2(byte[0, 0].double() - 127)[:, None]
+    want = exact.to(BF)
+    fits = exact.abs() < 2.0 ** 128
+    assert torch.equal(want[3:].double()[fits[3:]], exact[3:][fits[3:]])
+    for got in (kk, vv):
+        got = got[:, 0].cpu()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0.0, posinf=1.0, neginf=-1.0), want.nan_to_num(0.0, posinf=1.0, neginf=-1.0))
+        assert torch.equal(got.isinf(), want.isinf())
+
+
 def test_read_and_write_nothing(cuda):
     k, v, table, scales = make_cache(cuda, gen(1), 2, 128, 16, [20], True)
     none = torch.zeros(0, dtype=torch.long, device=cuda)
