@@ -758,6 +758,27 @@ def test_packed_attention_does_not_see_what_is_masked(cuda, heads, kv, dim):
           torch.full((1, dim), 4.0, device=cuda), dim ** -0.5)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 512), (32, 8, 128), (8, 8, 128), (16, 2, 256), (3, 1, 512), (3, 1, 128)])
+@pytest.mark.parametrize("queries,past", [([130, 70], [0, 0]), ([20, 65], [1500, 63]), ([150] * 30, [64] * 30)])
+def test_packed_attention_of_nan_alone_in_a_tile(cuda, heads, kv, dim, queries, past):
+    """Queries with a NaN, and a NaN in a key that starts a tile of 64 (the only one that some query sees of it): one block by
+    one, in parts and in chains."""
+    say(f"packed NaN heads={heads} kv={kv} dim={dim} queries={queries[:2]} past={past[:2]}")
+    g = gen(dim + heads)
+    starts = torch.tensor([0, *queries]).cumsum(0)
+    k_starts = torch.tensor([0, *(a + b for a, b in zip(queries, past))]).cumsum(0)
+    q, k, v = (normal((int(n), h, dim), g, cuda) for n, h in ((starts[-1], heads), (k_starts[-1], kv), (k_starts[-1], kv)))
+    q[3, :, 7], q[-1, 0, dim - 1] = float("nan"), float("nan")
+    k[int(k_starts[1]) + 64, :, 9] = float("nan")  # of the second sequence
+    out = kernels.packed_attention(q, k, v, starts.to(cuda), max(queries), dim ** -0.5, k_starts=k_starts.to(cuda))
+    torch.cuda.synchronize()
+    want, size = op.packed_attention(q, k, v, starts.tolist(), k_starts.tolist(), dim ** -0.5)
+    fine = want.isfinite()
+    assert want[3].isnan().all() and want[-1, 0].isnan().all() and torch.equal(out.isnan(), want.isnan())
+    close(torch.where(fine, out.double(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, size, 0.0),
+          torch.full((1, dim), 4.0, device=cuda), torch.full((1, dim), 4.0, device=cuda), dim ** -0.5)
+
+
 # ---------------------------------------------------------------------------------------------- together
 
 @pytest.mark.parametrize("fp8", [True, False])
