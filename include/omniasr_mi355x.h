@@ -445,7 +445,7 @@ int omni_paged_read(const void *k_pages, const void *v_pages, const void *k_scal
                     int32_t kv_heads, int32_t head_dim, int32_t cache_dtype, void *k_out, void *v_out,
                     void *stream);
 
-/* Bytes of workspace omni_paged_attention needs. */
+/* Bytes of workspace omni_paged_attention needs: parts for up to 512 workgroups (67 MB at most), and 4 for each row. */
 size_t omni_paged_attention_workspace(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
                                       int32_t head_dim, int32_t page, int32_t width);
 

@@ -86,7 +86,8 @@ __device__ __forceinline__ void chunk_scores(const KvChunk<kF8>& t, const u32x4_
 }
 
 // The softmax step of a tile: lane (c, g) holds query c's raw scores of its 8 keys, of which it sees the first ``seen``;
-// returns their probabilities relative to the lazy reference maximum (see attend_scored) as the P operand.
+// returns their probabilities relative to the lazy reference maximum (see attend_scored) as the P operand: bf16, what the
+// matrix instruction takes, each rounded once (2^-8 of itself at most); their sum stays in fp32, of the unrounded ones.
 template <int NB>
 __device__ __forceinline__ u32x4_t tile_softmax(const f32x4_t (&acc)[2], float c_scale, SoftmaxState& st,
                                                 f32x4_t (&o)[NB], int g, int seen) {

@@ -9,9 +9,9 @@
 // What bounds it is the HBM stream of the keys, so every CU is to stream the same share from start to end.  The 32-key
 // tiles of all units stand in one line (row after row, unit after unit), cut into equal shares, one for each workgroup of
 // four waves, whatever the rows' lengths: a share is the end of one unit, whole units, and the beginning of another.  A
-// unit's start counts as some more tiles (paged_start), about what it costs.  A wave holds 128 dimensions, so the waves take a unit's
-// tiles in turn at head dim 128, in pairs at 256 and together at 512, where their partial scores are added through LDS;
-// each has the next tiles' loads in flight in registers.  A unit within one share is written at once; of the others each
+// unit's start counts as some more tiles (paged_start), about what it costs.  A wave holds 128 dimensions, so the waves
+// take a unit's tiles in turn at head dim 128, in pairs at 256 and together at 512, where their partial scores are added
+// through LDS; each has the next tiles' loads in flight in registers.  A unit within one share is written at once; of the others each
 // share leaves (O, m, l) in fp32, and a second launch joins them:
 //   w_s = exp(m_s - max m), out = sum w_s O_s / sum w_s l_s.
 // All of it is found from the lengths on the device, so one launch shape serves every length (graphs), and results do not
@@ -39,7 +39,9 @@ struct PagedAttn {
   uint16_t* out;   // [rows * T, H, D]
 };
 
-constexpr int kPaSlots = 512;  // workgroups that run at once: two on each of 256 CUs
+// Workgroups of a launch at most: as many as run at once, two on each of 256 CUs.  (One at head dim 256 with two blocks of
+// columns, whose LDS, 83456 bytes, fits a CU once: there the shares take two rounds.)
+constexpr int kPaSlots = 512;
 
 // Keys that the row's first and last query see.
 struct PagedReach {
@@ -155,7 +157,9 @@ struct PagedPiece {
 template <int D, bool kF8, int NB>
 __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2))) void paged_attn_kernel(PagedAttn a) {
   constexpr int kRowB = D * (kF8 ? 1 : 2), kAhead = paged_ahead<kF8, NB>();
-  constexpr bool kOnce = NB == 1;  // two blocks may be a part of more columns, whose other units read the same keys
+  // Two blocks may be a part of more than 32 columns, whose other units read the same keys.  (17 to 32 columns are one unit's,
+  // and kept in the caches all the same.)
+  constexpr bool kOnce = NB == 1;
   constexpr int kSlices = D / 128, kStep = kPaWaves / kSlices;  // waves to a tile, tiles at a time
   constexpr int kQRow = D * 2 + 16;  // LDS bytes of a query, padded against bank conflicts
   constexpr int kQPieces = 16 * NB * (D / 8) / (64 * kPaWaves);  // of 16 bytes, of the blocks' queries, for a thread

@@ -8,8 +8,8 @@
 // keys [0, i + nk - nq] of nk.  What bounds a tile is the same; what they add is lengths from the device, rows of any stride, a
 // mask on every tile that not all of a wave's queries see, and at head dim 128 up to four heads of a kv head in a block (64
 // queries of each: a short prompt fills a block, and the heads share its tiles).  Measured, us: 8 prompts of 750-2400, 8 heads
-// x 512 195 (705 TFLOP/s), 32 over 8 x 128 175; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 76 (a head to a block
-// 113); one of 1433, 32 x 128 42.
+// x 512 197 (700 TFLOP/s), 32 over 8 x 128 175; 16 of up to 500 behind up to 900 keys, 32 over 8 x 128 76-80 (a head to a
+// block 113); one of 1433, 32 x 128 42.
 #include <math.h>
 
 #include <algorithm>
@@ -154,8 +154,8 @@ __device__ __forceinline__ int pf_rank(const PfSequence& mine, int sequences) {
   return rank;
 }
 
-// The sequence of rank r by work, the most first: so the last blocks of a
-// launch, whose CUs wait for each other, are the short ones.  Past 64 sequences, the order of the call.
+// The sequence of rank r by work, the most first: so the last blocks of a launch, whose CUs wait for each other, are the
+// short ones.  Past 64 sequences, more than a wave has lanes, the order of the call.
 // ``share``, where blocks (of ``queries``, ``heads`` for each) may be in parts: the key tiles of a part, about what all blocks
 // have for each CU, or what no block is longer than.
 __device__ __forceinline__ PfSequence pf_ranked(const PrefillArgs& a, int sequences, int r, int queries, int heads,
@@ -944,6 +944,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 16; ++i) over |= sv[i] > thr;
         if (__any(over) && lane == 0) moved[t & 3] = 1;
         float lt = 0.f;
+        // Probabilities as the value waves' operand: bf16, what the matrix instruction takes, each rounded once (2^-8 of itself
+        // at most); their sum is of the unrounded ones, in fp32.
         auto put_p = [&](float m) {
           lt = 0.f;
 #pragma unroll
@@ -1049,7 +1051,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int u = 0; u < 2; ++u) p[u][s & 1] = ps[t & 1][u][s][lane];
   };
   // O^T += V^T P^T for the workgroup's tile t; ``ahead``: the next tile's V loads as its registers fall free.  Step
-  // s + 1's operands are built beside step s's products; the scheduler keeps each step's loads behind the permutes that read their registers.
+  // s + 1's operands are built beside step s's products; the scheduler keeps each step's loads behind the permutes that read
+  // their registers.
   auto attend_v = [&](int t, const WsTile* ahead) {
     u32x4_t vop[2][4];
     auto operands = [&](int s) {
@@ -1364,7 +1367,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       f32x16_t zero;
 #pragma unroll
       for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-      // One 16-key step's probabilities of query half u: keys 16 (2m + hf) .., as the value wave's operand.
+      // One 16-key step's probabilities of query half u: keys 16 (2m + hf) .., as the value wave's operand, in bf16 as
+      // prefill_attn_ws_kernel's.
       auto put_p = [&](const Scores& sc, int t, int m, int hf, int u, float mu) {
         u32x4_t pop;
 #pragma unroll
@@ -1679,7 +1683,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       f32x16_t zero;
 #pragma unroll
       for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-      // One 16-key step's probabilities: keys 16 (2m + hf) .., as the value wave's operand.
+      // One 16-key step's probabilities: keys 16 (2m + hf) .., as the value wave's operand, in bf16 as
+      // prefill_attn_ws_kernel's.
       auto put_p = [&](const Scores& sc, int t, int m, int hf, float mu) {
         u32x4_t pop;
 #pragma unroll
@@ -2039,9 +2044,10 @@ inline int packed_block(int rows, int64_t longest, int64_t units) {
   return rows;
 }
 
-// Whether a launch runs its blocks in chains: where an XCD has two (head dims 128 and 256: three; 10 of 260-300, 32 heads, 2.5 for each,
-// take 48 us in place of 45.5) or more for each of its workgroups (no more than their lists hold, and sequences that one wave's
-// lanes hold), and the same ``heads`` blocks of heads for every sequence.
+// Whether a launch runs its blocks in chains: where an XCD has two (head dims 128 and 256: three; 10 of 260-300, 32 heads,
+// 2.5 for each, take 48 us in place of 45.5) or more for each of its workgroups (no more than their lists hold, and sequences
+// that one wave's lanes hold), and the same ``heads`` blocks of heads for every sequence.  64 sequences of 20-600 and, block
+// by block, 65, us: 8 heads x 512 200 / 239, 16 over 2 x 256 182 / 196, 32 over 8 x 128 181 / 188, 32 x 128 255 / 242.
 inline bool packed_chains(int64_t nqb, int heads, int sequences, int head_dim) {
   const int64_t each = nqb * sequences * (heads / 8);  // blocks of an XCD, at most
   return heads % 8 == 0 && sequences <= kWave && each >= (head_dim == 512 ? 2 : 3) * kWsPerXcd &&
